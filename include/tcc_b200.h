@@ -274,6 +274,92 @@ tcc_status tcc_scatter_add_rows(const float* in, uint64_t ldi, const int64_t* id
                                 float* out, uint64_t ldo, uint64_t num_rows, uint32_t F,
                                 uint32_t* bad_flag, cudaStream_t stream);
 
+/* ------------------------------------ training operators of the models ---- */
+/* No counterparts in the reference, which leaves these to torch.  Element
+ * types, index types and activations: */
+#define TCC_F32 0
+#define TCC_F16 1
+#define TCC_BF16 2
+#define TCC_I32 0
+#define TCC_I64 1
+#define TCC_ACT_NONE 0
+#define TCC_ACT_RELU 1
+#define TCC_ACT_SILU 2 /* z * sigmoid(z) */
+#define TCC_ACT_GELU 3 /* z * Phi(z), the exact form */
+#define TCC_NO_PADDING INT64_MIN
+
+/* Rows of a learned table by index, scaled: out[i, :F] = scale * table[idx[i], :F]
+ * for i < n, computed in fp32 and rounded once.  out has the table's type or
+ * fp32.  An index equal to padding_idx (any value, also one outside the table;
+ * TCC_NO_PADDING for none) gives a zero row.  Any other index outside
+ * [0, num_rows) gives a zero row and sets the device word *bad_flag (may be
+ * NULL).  Any F up to 2^20, strides >= F, pointers aligned to their element;
+ * 16-byte accesses where F, strides and pointers allow them. */
+tcc_status tcc_embedding_forward(const void* table, int table_type, uint64_t ld_table,
+                                 uint64_t num_rows, const void* idx, int idx_type, uint64_t n,
+                                 int64_t padding_idx, float scale, void* out, int out_type,
+                                 uint64_t ld_out, uint32_t F, uint32_t* bad_flag,
+                                 cudaStream_t stream);
+/* Its gradient, the whole dense table: grad_table[v, :F] = scale * sum of
+ * grad_out[i, :F] over the i with idx[i] = v; rows without an index become 0,
+ * columns F..ld_table stay as they were.  grad_out has the table's type or
+ * fp32; sums are fp32, in an order that depends on the indices alone (the same
+ * call gives the same bits).  Padded and bad indices contribute nothing.  n and
+ * num_rows below 2^31; scratch 256-byte aligned, of at least
+ * tcc_embedding_backward_scratch_bytes(n, num_rows, F) bytes, not shared with
+ * a call that may run at the same time. */
+size_t tcc_embedding_backward_scratch_bytes(uint64_t n, uint64_t num_rows, uint32_t F);
+tcc_status tcc_embedding_backward(const void* grad_out, int grad_type, uint64_t ld_grad,
+                                  const void* idx, int idx_type, uint64_t n, int64_t padding_idx,
+                                  float scale, void* grad_table, int table_type,
+                                  uint64_t ld_table, uint64_t num_rows, uint32_t F, void* scratch,
+                                  size_t scratch_bytes, uint32_t* bad_flag, cudaStream_t stream);
+
+/* Group norm over channels-last features, then an activation.  x is N samples
+ * of S rows of C channels (row r of sample n at x + (n * S + r) * ldx), G
+ * groups of C / G neighbouring channels; per (sample, group): h = (x - mean) /
+ * sqrt(var + eps) with the population variance, y = act(h * weight + bias).
+ * weight and bias ([C], may be NULL) have their own type.  Statistics are fp32;
+ * mean and rstd ([N * G] fp32, both or neither) are what the backward reads.
+ * y may be x.  scratch as above, of tcc_group_norm_scratch_bytes(.., 0). */
+size_t tcc_group_norm_scratch_bytes(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int backward);
+tcc_status tcc_group_norm_forward(const void* x, int type, uint64_t ldx, const void* weight,
+                                  const void* bias, int param_type, void* y, uint64_t ldy,
+                                  float* mean, float* rstd, uint64_t N, uint64_t S, uint32_t C,
+                                  uint32_t G, float eps, int act, void* scratch,
+                                  size_t scratch_bytes, cudaStream_t stream);
+/* dx, dweight and dbias (each may be NULL) from dy and the forward's x, mean
+ * and rstd; the activation is computed again.  dx may be dy.  The order of
+ * every sum is fixed. */
+tcc_status tcc_group_norm_backward(const void* dy, uint64_t lddy, const void* x, uint64_t ldx,
+                                   int type, const void* weight, const void* bias, int param_type,
+                                   const float* mean, const float* rstd, void* dx, uint64_t lddx,
+                                   void* dweight, void* dbias, uint64_t N, uint64_t S, uint32_t C,
+                                   uint32_t G, int act, void* scratch, size_t scratch_bytes,
+                                   cudaStream_t stream);
+
+/* The 2-norm of all the elements of `count` tensors (a host array; dense, of
+ * any size and element alignment), and clipping by it: every element times
+ * max_norm / (norm + eps) where that is below 1.  A NaN or infinite element
+ * makes the norm NaN or infinite, and clipping then spreads NaN (or, for an
+ * infinite norm, zeros and NaN).  The norm is a device word; nothing
+ * synchronises and nothing is copied from the host, so a call can be captured.
+ * Sums are 64-bit in a fixed order.  Clipped tensors must not overlap. */
+typedef struct tcc_tensor {
+    void* data;
+    uint64_t n;
+    int32_t type;
+    int32_t reserved;
+} tcc_tensor;
+size_t tcc_grad_norm_scratch_bytes(void);
+tcc_status tcc_grad_norm(const tcc_tensor* tensors, uint32_t count, float* norm, void* scratch,
+                         size_t scratch_bytes, cudaStream_t stream);
+tcc_status tcc_clip_grads_with_norm(const tcc_tensor* tensors, uint32_t count, const float* norm,
+                                    float max_norm, float eps, cudaStream_t stream);
+tcc_status tcc_clip_grad_norm(const tcc_tensor* tensors, uint32_t count, float max_norm, float eps,
+                              float* norm, void* scratch, size_t scratch_bytes,
+                              cudaStream_t stream);
+
 /* ------------------------------------------- halo exchange over NVLink ---- */
 /* No counterpart in the reference, whose multi-GPU path reads peer feature
  * caches inside the SpMM kernel (cnic/src/core/spmm_kernel.cu:145-147).  The

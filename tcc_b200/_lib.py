@@ -106,11 +106,25 @@ class Bcsc(C.Structure):
                 ("sparseA2C", C.c_void_p), ("tcLocalBit", C.c_void_p)]
 
 
+# element types, index types and activations of the training operators
+F32, F16, BF16 = 0, 1, 2        # TCC_F32, TCC_F16, TCC_BF16
+I32, I64 = 0, 1                 # TCC_I32, TCC_I64
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}  # TCC_ACT_*
+NO_PADDING = -(1 << 63)         # TCC_NO_PADDING
+
+
+class Tensor(C.Structure):
+    """tcc_tensor."""
+    _fields_ = [("data", C.c_void_p), ("n", C.c_uint64), ("type", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
 # name -> (restype, argtypes); the symbols include/tcc_b200.h declares
 _vp = C.c_void_p
 _u32 = C.c_uint32
 _u64 = C.c_uint64
 _i = C.c_int
+_i64 = C.c_int64
 _st = C.c_int
 PROTOTYPES = {
     "tcc_last_error": (C.c_char_p, []),
@@ -159,6 +173,20 @@ PROTOTYPES = {
     "tcc_dist_step": (_st, [C.POINTER(DistStepArgs), _vp, _vp]),
     "tcc_relu_dropout_forward": (_st, [_vp, _vp, _u64, C.c_float, _u64, _vp]),
     "tcc_relu_dropout_backward": (_st, [_vp, _vp, _vp, _u64, C.c_float, _vp]),
+    "tcc_embedding_forward": (_st, [_vp, _i, _u64, _u64, _vp, _i, _u64, _i64, C.c_float, _vp, _i,
+                                    _u64, _u32, _vp, _vp]),
+    "tcc_embedding_backward_scratch_bytes": (C.c_size_t, [_u64, _u64, _u32]),
+    "tcc_embedding_backward": (_st, [_vp, _i, _u64, _vp, _i, _u64, _i64, C.c_float, _vp, _i, _u64,
+                                     _u64, _u32, _vp, C.c_size_t, _vp, _vp]),
+    "tcc_group_norm_scratch_bytes": (C.c_size_t, [_u64, _u64, _u32, _u32, _i]),
+    "tcc_group_norm_forward": (_st, [_vp, _i, _u64, _vp, _vp, _i, _vp, _u64, _vp, _vp, _u64, _u64,
+                                     _u32, _u32, C.c_float, _i, _vp, C.c_size_t, _vp]),
+    "tcc_group_norm_backward": (_st, [_vp, _u64, _vp, _u64, _i, _vp, _vp, _i, _vp, _vp, _vp, _u64,
+                                      _vp, _vp, _u64, _u64, _u32, _u32, _i, _vp, C.c_size_t, _vp]),
+    "tcc_grad_norm_scratch_bytes": (C.c_size_t, []),
+    "tcc_grad_norm": (_st, [_vp, _u32, _vp, _vp, C.c_size_t, _vp]),
+    "tcc_clip_grads_with_norm": (_st, [_vp, _u32, _vp, C.c_float, C.c_float, _vp]),
+    "tcc_clip_grad_norm": (_st, [_vp, _u32, C.c_float, C.c_float, _vp, _vp, C.c_size_t, _vp]),
     "tcc_bcsr_spmm_t": (_st, [C.POINTER(Bcsr), _vp, _u64, _vp, _u64, _u32, _u32, _vp, _vp, _vp]),
     "tcc_bcsc_spmm": (_st, [C.POINTER(Bcsc), _vp, _u64, _vp, _u64, _u32, _u32, _vp, _vp, _vp]),
     "tcc_bcsc_spmm_t": (_st, [C.POINTER(Bcsc), _vp, _u64, _vp, _u64, _u32, _u32, _vp, _vp, _i,

@@ -1,0 +1,108 @@
+"""The global norm of a model's gradients, and clipping by it.
+
+The reference steps its optimiser on unclipped gradients
+(TAC_training_backend/train/tcgnn_conv_release.py); ``train_gcn`` clips with
+``--clip-norm``.  The norm stays on the GPU: nothing synchronises, and the calls
+can be captured in a CUDA graph.
+"""
+from __future__ import annotations
+
+from array import array
+
+import torch
+
+from . import _lib as L
+from ._args import TYPES, launch, scratch_for
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t's elements fill one block of memory, in any order."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for size, stride in sorted(((s, st) for s, st in zip(t.shape, t.stride()) if s > 1), key=lambda p: p[1]):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _table(tensors):
+    """(tcc_tensor array of the tensors, its length, their device)."""
+    device, words = None, array("Q")
+    for t in tensors:
+        code = TYPES.get(t.dtype)
+        if code is None:
+            raise TypeError(f"gradients must be float32, float16 or bfloat16, not {t.dtype}")
+        if t.layout != torch.strided or not t.is_cuda:
+            raise ValueError("gradients must be dense CUDA tensors")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError("gradients must be on one device")
+        if not _dense(t):
+            raise ValueError("a gradient's elements must fill one block of memory (no gaps, no broadcast)")
+        words.extend((t.data_ptr(), t.numel(), code))  # data, n, type and reserved
+    return words, len(words) // 3, device
+
+
+def _list(tensors) -> list:
+    return [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+
+
+def _written(tensors) -> None:
+    """The tensors were changed in place: a graph that saved one notices."""
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
+def grad_norm(tensors) -> torch.Tensor:
+    """The 2-norm of all elements of the tensors (one, or an iterable), a float32 scalar on
+    their device; 64-bit sums in a fixed order.  Without tensors a CPU zero."""
+    words, count, device = _table(_list(tensors))
+    if count == 0:
+        return torch.zeros(())
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    nbytes = L.lib().tcc_grad_norm_scratch_bytes()
+    hold, scratch = scratch_for(nbytes, device)
+    launch(device, "tcc_grad_norm", words.buffer_info()[0], count, norm.data_ptr(), scratch, nbytes)
+    return norm
+
+
+def clip_grads_with_norm_(tensors, max_norm: float, total_norm: torch.Tensor, eps: float = 1e-6) -> None:
+    """Scale the tensors in place by max_norm / (total_norm + eps) where that is below 1.
+    total_norm: a float32 scalar on their device (e.g. combined over the ranks that each
+    hold a part of the parameters: the root of the sum of their squared norms)."""
+    tensors = _list(tensors)
+    words, count, device = _table(tensors)
+    if count == 0:
+        return
+    if total_norm.dtype != torch.float32 or total_norm.numel() != 1 or total_norm.device != device:
+        raise ValueError("total_norm must be a float32 scalar on the gradients' device")
+    launch(device, "tcc_clip_grads_with_norm", words.buffer_info()[0], count, total_norm.data_ptr(), max_norm, eps)
+    _written(tensors)
+
+
+def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Clip the gradients of the parameters (one, or an iterable; those without a
+    gradient are passed over) in place to a global 2-norm of max_norm, and return
+    the norm they had, a float32 scalar.  Gradients of different types may mix;
+    two that share memory are refused.  ``error_if_nonfinite`` waits for the norm
+    and raises where it is NaN or infinite, before anything is scaled."""
+    grads = [p.grad for p in _list(parameters) if p.grad is not None]
+    if error_if_nonfinite:
+        norm = grad_norm(grads)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError("the gradients' norm is not finite, so they cannot be clipped")
+        if grads:
+            clip_grads_with_norm_(grads, max_norm, norm, eps)
+        return norm
+    words, count, device = _table(grads)
+    if count == 0:
+        return torch.zeros(())
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    nbytes = L.lib().tcc_grad_norm_scratch_bytes()
+    hold, scratch = scratch_for(nbytes, device)
+    launch(device, "tcc_clip_grad_norm", words.buffer_info()[0], count, max_norm, eps, norm.data_ptr(), scratch,
+           nbytes)
+    _written(grads)
+    return norm

@@ -3,6 +3,7 @@
 // and records a message for tcc_last_error().
 #include "convert.cuh"
 #include "spmm.cuh"
+#include "train_ops.cuh"
 
 #include <nvtx3/nvToolsExt.h>
 
@@ -651,6 +652,95 @@ tcc_status tcc_relu_dropout_backward(const float* grad_out, const float* out, fl
     return guarded("tcc_relu_dropout_backward", [&] {
         TCC_REQUIRE(n == 0 || (grad_out && out && grad_in), "null argument");
         tcc::relu_dropout_backward(grad_out, out, grad_in, n, p, stream);
+    });
+}
+
+tcc_status tcc_embedding_forward(const void* table, int table_type, uint64_t ld_table,
+                                 uint64_t num_rows, const void* idx, int idx_type, uint64_t n,
+                                 int64_t padding_idx, float scale, void* out, int out_type,
+                                 uint64_t ld_out, uint32_t F, uint32_t* bad_flag,
+                                 cudaStream_t stream) {
+    return guarded("tcc_embedding_forward", [&] {
+        const tcc::EmbeddingArgs a{const_cast<void*>(table), table_type, ld_table, num_rows, idx,
+                                   idx_type, n, padding_idx, scale, out, out_type, ld_out, F,
+                                   bad_flag};
+        tcc::embedding_forward(a, stream);
+    });
+}
+
+size_t tcc_embedding_backward_scratch_bytes(uint64_t n, uint64_t num_rows, uint32_t F) {
+    return tcc::embedding_backward_scratch_bytes(n, num_rows, F);
+}
+
+tcc_status tcc_embedding_backward(const void* grad_out, int grad_type, uint64_t ld_grad,
+                                  const void* idx, int idx_type, uint64_t n, int64_t padding_idx,
+                                  float scale, void* grad_table, int table_type,
+                                  uint64_t ld_table, uint64_t num_rows, uint32_t F, void* scratch,
+                                  size_t scratch_bytes, uint32_t* bad_flag, cudaStream_t stream) {
+    return guarded("tcc_embedding_backward", [&] {
+        const tcc::EmbeddingArgs a{grad_table, table_type, ld_table, num_rows, idx, idx_type, n,
+                                   padding_idx, scale, const_cast<void*>(grad_out), grad_type,
+                                   ld_grad, F, bad_flag};
+        tcc::embedding_backward(a, scratch, scratch_bytes, stream);
+    });
+}
+
+size_t tcc_group_norm_scratch_bytes(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int backward) {
+    return tcc::group_norm_scratch_bytes(N, S, C, G, backward != 0);
+}
+
+tcc_status tcc_group_norm_forward(const void* x, int type, uint64_t ldx, const void* weight,
+                                  const void* bias, int param_type, void* y, uint64_t ldy,
+                                  float* mean, float* rstd, uint64_t N, uint64_t S, uint32_t C,
+                                  uint32_t G, float eps, int act, void* scratch,
+                                  size_t scratch_bytes, cudaStream_t stream) {
+    return guarded("tcc_group_norm_forward", [&] {
+        tcc::GroupNormArgs a{};
+        a.x = x, a.type = type, a.ldx = ldx;
+        a.weight = weight, a.bias = bias, a.param_type = param_type;
+        a.y = y, a.ldy = ldy, a.mean = mean, a.rstd = rstd;
+        a.N = N, a.S = S, a.C = C, a.G = G, a.eps = eps, a.act = act;
+        tcc::group_norm_forward(a, scratch, scratch_bytes, stream);
+    });
+}
+
+tcc_status tcc_group_norm_backward(const void* dy, uint64_t lddy, const void* x, uint64_t ldx,
+                                   int type, const void* weight, const void* bias, int param_type,
+                                   const float* mean, const float* rstd, void* dx, uint64_t lddx,
+                                   void* dweight, void* dbias, uint64_t N, uint64_t S, uint32_t C,
+                                   uint32_t G, int act, void* scratch, size_t scratch_bytes,
+                                   cudaStream_t stream) {
+    return guarded("tcc_group_norm_backward", [&] {
+        tcc::GroupNormArgs a{};
+        a.x = x, a.type = type, a.ldx = ldx, a.dy = dy, a.lddy = lddy, a.dx = dx, a.lddx = lddx;
+        a.weight = weight, a.bias = bias, a.param_type = param_type;
+        a.dweight = dweight, a.dbias = dbias;
+        a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd);
+        a.N = N, a.S = S, a.C = C, a.G = G, a.act = act;
+        tcc::group_norm_backward(a, scratch, scratch_bytes, stream);
+    });
+}
+
+size_t tcc_grad_norm_scratch_bytes(void) { return tcc::grad_norm_scratch_bytes(); }
+
+tcc_status tcc_grad_norm(const tcc_tensor* tensors, uint32_t count, float* norm, void* scratch,
+                         size_t scratch_bytes, cudaStream_t stream) {
+    return guarded("tcc_grad_norm",
+                   [&] { tcc::grad_norm(tensors, count, norm, scratch, scratch_bytes, stream); });
+}
+
+tcc_status tcc_clip_grads_with_norm(const tcc_tensor* tensors, uint32_t count, const float* norm,
+                                    float max_norm, float eps, cudaStream_t stream) {
+    return guarded("tcc_clip_grads_with_norm", [&] {
+        tcc::clip_grads_with_norm(tensors, count, norm, max_norm, eps, stream);
+    });
+}
+
+tcc_status tcc_clip_grad_norm(const tcc_tensor* tensors, uint32_t count, float max_norm, float eps,
+                              float* norm, void* scratch, size_t scratch_bytes,
+                              cudaStream_t stream) {
+    return guarded("tcc_clip_grad_norm", [&] {
+        tcc::clip_grad_norm(tensors, count, max_norm, eps, norm, scratch, scratch_bytes, stream);
     });
 }
 

@@ -1,0 +1,324 @@
+// clip.cu -- the 2-norm of all gradients of a model, and their clipping.
+//
+//   norm = sqrt(sum over tensors and elements of g^2)
+//   g *= min(1, max_norm / (norm + eps))
+//
+// Bound by memory: the norm reads every gradient once, the clipping reads and
+// writes it once.  The tensors' addresses travel in the kernel's parameters,
+// so a call copies nothing to the device first and can be captured in a graph.
+// Every CTA writes one partial sum in a fixed order and the sums are added in a
+// fixed order: the same gradients give the same norm, bit for bit.
+#include "elem.cuh"
+#include "train_ops.cuh"
+
+#include <algorithm>
+#include <vector>
+
+namespace tcc {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr uint32_t kChunkBytes = 32768;  // of one tensor, for one CTA at a time
+constexpr uint32_t kMaxBlocks = 148 * 8;
+
+// K tensors of one launch; chunk i of the launch belongs to the tensor t with
+// first[t] <= i < first[t + 1].
+template <int K>
+struct TensorTable {
+    uint32_t count;
+    void* data[K];
+    uint64_t n[K];
+    uint32_t first[K + 1];
+    uint8_t type[K];
+};
+
+struct Span {
+    void* data;  // first element of the chunk
+    uint32_t n;  // elements
+    int type;
+};
+
+template <int K>
+__device__ __forceinline__ Span chunk_span(const TensorTable<K>& t, uint32_t chunk) {
+    uint32_t lo = 0, hi = t.count;  // last tensor with first <= chunk
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (t.first[mid] <= chunk) lo = mid;
+        else hi = mid;
+    }
+    Span s;
+    s.type = t.type[lo];
+    const uint32_t bytes = s.type == TCC_F32 ? 4 : 2;
+    const uint64_t per = kChunkBytes / bytes, at = (uint64_t)(chunk - t.first[lo]) * per;
+    s.data = static_cast<char*>(t.data[lo]) + at * bytes;
+    s.n = (uint32_t)min(per, t.n[lo] - at);
+    return s;
+}
+
+// Sum of squares of one pack.  fp32 inside a pack where that is safe; where a
+// square could leave fp32's range (or all are zero) the pack is summed in
+// 64 bits, so a norm of 1e30 or 1e-30 comes out right.
+template <typename T, int V>
+__device__ __forceinline__ double pack_squares(const Pack<T, V>& p) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const float v = to_f32(p.v[k]);
+        s = fmaf(v, v, s);
+    }
+    if (s > 1e-25f && s < 1e37f) return (double)s;
+    double d = 0.0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const double v = (double)to_f32(p.v[k]);
+        d += v * v;
+    }
+    return d;
+}
+
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double ws[kThreads / 32];
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double t = 0.0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) t += ws[i];
+    __syncthreads();
+    return t;
+}
+
+// Elements before the first 16-byte boundary.
+__device__ __forceinline__ uint32_t head_of(const void* p, uint32_t n, uint32_t bytes) {
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15u);
+    return min(n, off ? (16 - off) / bytes : 0u);
+}
+
+template <typename T>
+__device__ __forceinline__ double span_squares(const Span& sp) {
+    constexpr int V = 16 / sizeof(T);
+    const T* p = static_cast<const T*>(sp.data);
+    const uint32_t head = head_of(p, sp.n, sizeof(T));
+    const uint32_t packs = (sp.n - head) / V, body = head + packs * V;
+    double s = 0.0;
+#pragma unroll 4
+    for (uint32_t q = threadIdx.x; q < packs; q += kThreads)
+        s += pack_squares<T, V>(load_pack<T, V>(p + head + (uint64_t)q * V));
+    if (threadIdx.x < head) s += pack_squares<T, 1>(load_pack<T, 1>(p + threadIdx.x));
+    if (body + threadIdx.x < sp.n) s += pack_squares<T, 1>(load_pack<T, 1>(p + body + threadIdx.x));
+    return s;
+}
+
+template <int K>
+__global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ TensorTable<K> t,
+                                                           double* __restrict__ partial, bool add) {
+    double s = 0.0;
+    const uint32_t chunks = t.first[t.count];
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const Span sp = chunk_span<K>(t, c);
+        if (sp.type == TCC_F32) s += span_squares<float>(sp);
+        else if (sp.type == TCC_F16) s += span_squares<__half>(sp);
+        else s += span_squares<__nv_bfloat16>(sp);
+    }
+    s = block_sum(s);
+    if (threadIdx.x == 0) partial[blockIdx.x] = add ? partial[blockIdx.x] + s : s;
+}
+
+__device__ __forceinline__ float norm_of(const double* __restrict__ partial, uint32_t blocks) {
+    double s = 0.0;
+    for (uint32_t i = threadIdx.x; i < blocks; i += kThreads) s += partial[i];
+    return (float)sqrt(block_sum(s));
+}
+
+__global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ partial, uint32_t blocks,
+                                                        float* __restrict__ norm) {
+    const float n = norm_of(partial, blocks);
+    if (threadIdx.x == 0) *norm = n;
+}
+
+template <typename T>
+__device__ __forceinline__ void span_scale(const Span& sp, float f) {
+    constexpr int V = 16 / sizeof(T);
+    T* p = static_cast<T*>(sp.data);
+    const uint32_t head = head_of(p, sp.n, sizeof(T));
+    const uint32_t packs = (sp.n - head) / V, body = head + packs * V;
+#pragma unroll 4
+    for (uint32_t q = threadIdx.x; q < packs; q += kThreads) {
+        Pack<T, V> v = load_pack<T, V>(p + head + (uint64_t)q * V);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v.v[k] = from_f32<T>(to_f32(v.v[k]) * f);
+        store_pack<T, V>(p + head + (uint64_t)q * V, v);
+    }
+    if (threadIdx.x < head) p[threadIdx.x] = from_f32<T>(to_f32(p[threadIdx.x]) * f);
+    if (body + threadIdx.x < sp.n) {
+        T* e = p + body + threadIdx.x;
+        *e = from_f32<T>(to_f32(*e) * f);
+    }
+}
+
+// Scales in the reverse of the order in which the norm was read: what was read
+// last is still in L2.  partial == NULL: the norm is read from norm_in.
+template <int K>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ TensorTable<K> t,
+                                                         const double* __restrict__ partial, uint32_t blocks,
+                                                         const float* norm_in, float* norm_out, float max_norm,
+                                                         float eps) {
+    const float norm = partial ? norm_of(partial, blocks) : *norm_in;
+    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+    // a factor of exactly 1 changes no value; a NaN norm spreads, as it should
+    const float f = max_norm / (norm + eps);
+    if (f >= 1.f) return;
+    const uint32_t chunks = t.first[t.count];
+    for (uint32_t i = blockIdx.x; i < chunks; i += gridDim.x) {
+        const Span sp = chunk_span<K>(t, chunks - 1 - i);
+        if (sp.type == TCC_F32) span_scale<float>(sp, f);
+        else if (sp.type == TCC_F16) span_scale<__half>(sp, f);
+        else span_scale<__nv_bfloat16>(sp, f);
+    }
+}
+
+// Fills a table from the tensors at `at` on (empty ones are skipped); returns
+// where the next launch starts.
+template <int K>
+uint32_t fill(const tcc_tensor* t, uint32_t count, uint32_t at, TensorTable<K>& out) {
+    out.count = 0;
+    uint64_t chunks = 0;
+    for (; at < count && out.count < (uint32_t)K; ++at) {
+        if (t[at].n == 0) continue;
+        const uint64_t per = kChunkBytes / type_bytes(t[at].type);
+        const uint64_t c = (t[at].n + per - 1) / per;
+        if (chunks + c >= (1ull << 32)) {
+            TCC_REQUIRE(out.count, "a tensor is too large");
+            break;
+        }
+        out.data[out.count] = t[at].data;
+        out.n[out.count] = t[at].n;
+        out.type[out.count] = (uint8_t)t[at].type;
+        out.first[out.count++] = (uint32_t)chunks;
+        chunks += c;
+    }
+    out.first[out.count] = (uint32_t)chunks;
+    return at;
+}
+
+void check_tensors(const tcc_tensor* t, uint32_t count, bool written) {
+    TCC_REQUIRE(count == 0 || t, "tensors must not be NULL");
+    for (uint32_t i = 0; i < count; ++i) {
+        TCC_REQUIRE(valid_type(t[i].type), "unknown element type");
+        TCC_REQUIRE(t[i].n == 0 || (t[i].data && (uintptr_t)t[i].data % type_bytes(t[i].type) == 0),
+                    "a tensor is NULL or not aligned to its type");
+        TCC_REQUIRE(t[i].n < (1ull << 46), "a tensor is too large");
+    }
+    if (!written) return;
+    // a value that two tensors share would be scaled twice, by two CTAs at once
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    for (uint32_t i = 0; i < count; ++i)
+        if (t[i].n)
+            spans.emplace_back((uintptr_t)t[i].data, (uintptr_t)t[i].data + t[i].n * type_bytes(t[i].type));
+    if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        TCC_REQUIRE(spans[i - 1].second <= spans[i].first, "two tensors share memory");
+}
+
+constexpr int kSmall = 32, kLarge = 480;
+
+// fn(table) for each launch's tensors; the small table keeps the parameters of
+// a launch over a few tensors short.
+template <typename Fn>
+void each_launch(const tcc_tensor* t, uint32_t count, Fn&& fn) {
+    if (count <= (uint32_t)kSmall) {
+        TensorTable<kSmall> tab;
+        for (uint32_t at = 0; at < count;) {
+            at = fill<kSmall>(t, count, at, tab);
+            if (tab.count) fn(tab);
+        }
+    } else {
+        TensorTable<kLarge> tab;
+        for (uint32_t at = 0; at < count;) {
+            at = fill<kLarge>(t, count, at, tab);
+            if (tab.count) fn(tab);
+        }
+    }
+}
+
+template <int K>
+void launch_squares(const TensorTable<K>& tab, double* partial, unsigned blocks, bool add, cudaStream_t s) {
+    squares_kernel<K><<<blocks, kThreads, 0, s>>>(tab, partial, add);
+    TCC_CUDA(cudaGetLastError());
+}
+
+// Partial sums of every tensor; returns how many there are.
+uint32_t squares(const tcc_tensor* t, uint32_t count, double* partial, cudaStream_t s) {
+    uint32_t blocks = 0;
+    each_launch(t, count, [&](const auto& tab) {
+        const uint32_t chunks = tab.first[tab.count];
+        // a later launch adds to the partial sums of the first, so all use its grid
+        if (blocks == 0) {
+            blocks = std::min(chunks, kMaxBlocks);
+            launch_squares(tab, partial, blocks, false, s);
+        } else {
+            launch_squares(tab, partial, blocks, true, s);
+        }
+    });
+    return blocks;
+}
+
+double* partials(void* scratch, size_t scratch_bytes) {
+    TCC_REQUIRE(scratch && (uintptr_t)scratch % 256 == 0, "scratch must be 256-byte aligned");
+    if (scratch_bytes < grad_norm_scratch_bytes())
+        throw Error(TCC_ERR_CAPACITY, "scratch is smaller than tcc_grad_norm_scratch_bytes");
+    return static_cast<double*>(scratch);
+}
+
+void scale(const tcc_tensor* t, uint32_t count, const double* partial, uint32_t blocks, const float* norm_in,
+           float* norm_out, float max_norm, float eps, cudaStream_t s) {
+    each_launch(t, count, [&](const auto& tab) {
+        const unsigned grid = std::min(tab.first[tab.count], kMaxBlocks);
+        scale_kernel<<<grid, kThreads, 0, s>>>(tab, partial, blocks, norm_in, norm_out, max_norm, eps);
+        TCC_CUDA(cudaGetLastError());
+    });
+}
+
+void check_clip(float max_norm, float eps) {
+    TCC_REQUIRE(max_norm >= 0.f, "max_norm must not be negative");
+    TCC_REQUIRE(eps >= 0.f, "eps must not be negative");
+}
+
+}  // namespace
+
+size_t grad_norm_scratch_bytes() { return kMaxBlocks * sizeof(double); }
+
+void grad_norm(const tcc_tensor* t, uint32_t count, float* norm, void* scratch, size_t scratch_bytes,
+               cudaStream_t s) {
+    check_tensors(t, count, false);
+    TCC_REQUIRE(norm, "norm must not be NULL");
+    double* partial = partials(scratch, scratch_bytes);
+    const uint32_t blocks = squares(t, count, partial, s);
+    norm_kernel<<<1, kThreads, 0, s>>>(partial, blocks, norm);
+    TCC_CUDA(cudaGetLastError());
+}
+
+void clip_grads_with_norm(const tcc_tensor* t, uint32_t count, const float* norm, float max_norm, float eps,
+                          cudaStream_t s) {
+    check_tensors(t, count, true);
+    check_clip(max_norm, eps);
+    TCC_REQUIRE(norm, "norm must not be NULL");
+    scale(t, count, nullptr, 0, norm, nullptr, max_norm, eps, s);
+}
+
+void clip_grad_norm(const tcc_tensor* t, uint32_t count, float max_norm, float eps, float* norm, void* scratch,
+                    size_t scratch_bytes, cudaStream_t s) {
+    check_tensors(t, count, true);
+    check_clip(max_norm, eps);
+    TCC_REQUIRE(norm, "norm must not be NULL");
+    double* partial = partials(scratch, scratch_bytes);
+    const uint32_t blocks = squares(t, count, partial, s);
+    if (blocks == 0) {  // no elements: the norm is 0
+        TCC_CUDA(cudaMemsetAsync(norm, 0, sizeof(float), s));
+        return;
+    }
+    scale(t, count, partial, blocks, nullptr, norm, max_norm, eps, s);
+}
+
+}  // namespace tcc

@@ -1,0 +1,110 @@
+// elem.cuh -- element types (fp32, fp16, bf16) and 16-byte packs shared by the
+// embedding, group norm and clipping kernels.  All arithmetic is fp32 or wider;
+// a value is rounded to its storage type once, when it is stored.
+#pragma once
+
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace tcc {
+
+inline bool valid_type(int t) { return t == TCC_F32 || t == TCC_F16 || t == TCC_BF16; }
+inline uint32_t type_bytes(int t) { return t == TCC_F32 ? 4u : 2u; }
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// One element of an array whose type is known at run time (parameters that a
+// thread reads once).
+__device__ __forceinline__ float load_typed(const void* p, int type, uint64_t i) {
+    if (type == TCC_F32) return static_cast<const float*>(p)[i];
+    if (type == TCC_F16) return __half2float(static_cast<const __half*>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_typed(void* p, int type, uint64_t i, float v) {
+    if (type == TCC_F32) static_cast<float*>(p)[i] = v;
+    else if (type == TCC_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// V elements moved as one aligned load or store (V * sizeof(T) <= 16).
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+    T v[V];
+};
+
+template <int BYTES>
+struct RawOf;
+template <> struct RawOf<2> { using type = unsigned short; };
+template <> struct RawOf<4> { using type = unsigned int; };
+template <> struct RawOf<8> { using type = uint2; };
+template <> struct RawOf<16> { using type = uint4; };
+
+template <typename T, int V>
+union PackBits {
+    typename RawOf<sizeof(T) * V>::type raw;
+    Pack<T, V> pack;
+    __device__ PackBits() {}
+};
+
+// Plain, read-only and streaming (evict-first) accesses to one pack.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+    PackBits<T, V> b;
+    b.raw = *reinterpret_cast<const decltype(b.raw)*>(p);
+    return b.pack;
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack_nc(const T* p) {
+    PackBits<T, V> b;
+    b.raw = __ldg(reinterpret_cast<const decltype(b.raw)*>(p));
+    return b.pack;
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack_cs(const T* p) {
+    PackBits<T, V> b;
+    b.raw = __ldcs(reinterpret_cast<const decltype(b.raw)*>(p));
+    return b.pack;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
+    PackBits<T, V> b;
+    b.pack = v;
+    *reinterpret_cast<decltype(b.raw)*>(p) = b.raw;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack_cs(T* p, const Pack<T, V>& v) {
+    PackBits<T, V> b;
+    b.pack = v;
+    __stcs(reinterpret_cast<decltype(b.raw)*>(p), b.raw);
+}
+
+// The widest V (of 8, 4, 2, 1; V * bytes <= 16) that divides every count in
+// `counts` and keeps every pointer aligned to V elements of its own size.
+struct VecRule {
+    uint64_t bits = 8;  // or-ed element counts; starts at the widest V
+    uint32_t max_bytes = 2;
+    void count(uint64_t n) { bits |= n; }
+    void pointer(const void* p, uint32_t bytes) {
+        bits |= reinterpret_cast<uintptr_t>(p) / bytes;
+        if (bytes > max_bytes) max_bytes = bytes;
+    }
+    int width() const {
+        int v = 8;
+        while ((uint64_t)v * max_bytes > 16 || (bits & (uint64_t)(v - 1))) v >>= 1;
+        return v;
+    }
+};
+
+}  // namespace tcc
