@@ -39,9 +39,10 @@ def test_embedding_refusals(lib):
         assert lib.tcc_last_error().startswith(b"tcc_embedding_backward")
     assert forward(n=0) == 0  # nothing to do
     assert backward(rows=0) == 0
-    assert backward(scratch=None) == 1
-    assert backward(scratch=P + 16) == 1
-    assert backward(nbytes=8) == 6  # TCC_ERR_CAPACITY
+    assert backward(n=5000, scratch=None) == 1
+    assert backward(n=5000, scratch=P + 16) == 1
+    assert backward(n=5000, nbytes=8) == 6  # TCC_ERR_CAPACITY
+    assert lib.tcc_embedding_backward_scratch_bytes(200, 1 << 20, 64) == 0  # few indices: none
     assert lib.tcc_embedding_backward_scratch_bytes(1 << 20, 1 << 20, 64) > 8 << 20
 
 
