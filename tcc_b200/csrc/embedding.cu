@@ -121,13 +121,13 @@ void lookup_by_width(const EmbeddingArgs& a, cudaStream_t s) {
 // by a last small kernel.  Nothing depends on the order in which CTAs run.
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 8;  // gradient rows in flight per team
-constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+constexpr uint32_t kUnroll = 8;  // gradient rows in flight per team
 
 using Entry = unsigned long long;  // row << 32 | position
 __device__ __forceinline__ uint32_t row_of(Entry e) { return (uint32_t)(e >> 32); }
 
-// Lanes of a team: one pack of a gradient row each (grid.y covers the rest).
+// Lanes of a team (8, 16 or 32): one pack of a gradient row each (grid.y covers
+// the rest).
 struct TeamShape {
     uint32_t lanes, teams, packs, blocks;  // blocks: the grid's y
 };
@@ -135,7 +135,7 @@ struct TeamShape {
 TeamShape team_shape(uint32_t packs) {
     TeamShape t;
     t.packs = packs;
-    t.lanes = 1;
+    t.lanes = kUnroll;
     while (t.lanes < 32 && t.lanes < packs) t.lanes <<= 1;
     t.teams = kThreads / t.lanes;
     t.blocks = (packs + t.lanes - 1) / t.lanes;
@@ -149,142 +149,235 @@ struct Border {
     uint32_t row;    // of the tail
 };
 
-// Sums the runs of entries [lo, hi) of `entries`, team t the entries
-// [lo + t * per, lo + (t + 1) * per).  Rows whose run lies inside are written;
-// for the others head / tail (fp32, [F]) and *border are, where they are given
-// (entries then go on outside [lo, hi) within [0, end)).  Entries of rows >=
-// num_rows are passed over.
+// A lane's packs of the next kUnroll rows lie in a ring in shared memory, which
+// asynchronous copies fill while earlier rows are added; a lane reads back only
+// what it copied itself.  (Rows held in registers instead took 64 to 200
+// registers a thread: 199 us for the sums of 1 M x 128 in place of 130.)
+template <typename TG, int V>
+struct Ring {
+    Pack<TG, V> slot[kUnroll][kThreads];
+};
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* smem, const void* global) {
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(smem);
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(global) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(global), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// Sums the runs of `count` entries in shared memory, team t the entries
+// [t * per, (t + 1) * per).  ent[-1] and ent[count] are the entries before and
+// after them (~0: none).  Rows whose run lies inside are written; for the
+// others head / tail (fp32, [F]) and *border are, where they are given.  Entries
+// of rows >= num_rows, which are the last, are passed over.
 template <typename TG, typename TT, int V>
-__device__ __forceinline__ void sum_runs(const Entry* entries, uint32_t lo, uint32_t hi, uint32_t end, uint32_t per,
-                                         const TG* __restrict__ grad, uint64_t ldg, float scale,
-                                         TT* __restrict__ dtable, uint64_t ldt, uint32_t num_rows,
-                                         const TeamShape& sh, float* head, float* tail, Border* border) {
-    __shared__ float sm_head[kThreads * V], sm_tail[kThreads * V];
-    __shared__ uint8_t sm_flags[kThreads];
-    const uint32_t team = threadIdx.x / sh.lanes, lane = threadIdx.x % sh.lanes;
-    const uint32_t pack = blockIdx.y * sh.lanes + lane;
-    const bool on = pack < sh.packs;
-    const uint64_t col = (uint64_t)pack * V;
-    const uint64_t first = (uint64_t)lo + (uint64_t)team * per;
-    const uint32_t e0 = (uint32_t)min(first, (uint64_t)hi), e1 = (uint32_t)min(first + per, (uint64_t)hi);
-    float acc[V];
-    auto clear = [&] {
+struct RunSums {
+    const Entry* ent;
+    uint32_t count, per;
+    const TG* grad;
+    uint32_t grad_stride;  // bytes
+    float scale;
+    TT* dtable;
+    uint64_t ldt;
+    uint32_t num_rows;
+    TeamShape sh;
+    Ring<TG, V>* ring;  // afterwards the teams' heads and tails
+
+    static_assert(sizeof(Ring<TG, V>) >= 2 * kThreads * V * sizeof(float), "heads and tails fit");
+    static constexpr bool kAsync = sizeof(Pack<TG, V>) >= 4;
+
+    bool on;
+    uint64_t col;
+    float acc[V], kept[V];  // kept: the head, while the ring is in use
+    uint32_t cur;
+    bool open, begun;  // a run is open; it began in this team's range
+
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int k = 0; k < V; ++k) acc[k] = 0.f;
-    };
-    auto write_row = [&](uint32_t row) {
-        if (!on || row >= num_rows) return;
+    }
+    __device__ __forceinline__ void write_row() {
+        if (!on) return;
         Pack<TT, V> o;
 #pragma unroll
         for (int k = 0; k < V; ++k) o.v[k] = from_f32<TT>(acc[k] * scale);
-        store_pack_cs<TT, V>(dtable + (uint64_t)row * ldt + col, o);
-    };
-    auto to_shared = [&](float* s) {
+        store_pack_cs<TT, V>(dtable + (uint64_t)cur * ldt + col, o);
+    }
+    __device__ __forceinline__ const TG* source(Entry e) const {
+        return reinterpret_cast<const TG*>(reinterpret_cast<const char*>(grad) +
+                                           (uint64_t)(uint32_t)e * grad_stride) + col;
+    }
+    __device__ __forceinline__ void consume(uint32_t i, uint32_t slot) {
+        const uint32_t row = row_of(ent[i]);
+        if (row != cur) {
+            if (open) {
+                if (begun) {
+                    write_row();
+                } else {
 #pragma unroll
-        for (int k = 0; k < V; ++k) s[threadIdx.x * V + k] = acc[k];
-    };
-    clear();
-    uint32_t flags = 0, cur = kNoRow;
-    bool begun = true;  // the current run began in this team's range
-    if (e0 < e1) {
-        cur = row_of(entries[e0]);
-        if (e0 > 0 && row_of(entries[e0 - 1]) == cur) {
-            flags |= kHead;
-            begun = false;
-        }
-        for (uint32_t j = e0; j < e1; j += kUnroll) {
-            uint32_t row[kUnroll];
-            Pack<TG, V> g[kUnroll];
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const Entry e = j + u < e1 ? entries[j + u] : ~0ull;
-                row[u] = row_of(e);
-                if (on && row[u] < num_rows)
-                    g[u] = load_pack_cs<TG, V>(grad + (uint64_t)(uint32_t)e * ldg + col);
-            }
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                if (j + u >= e1) break;
-                if (row[u] != cur) {
-                    if (begun) write_row(cur);
-                    else to_shared(sm_head);
-                    begun = true;
-                    cur = row[u];
-                    clear();
-                }
-                if (row[u] < num_rows) {
-#pragma unroll
-                    for (int k = 0; k < V; ++k) acc[k] += to_f32(g[u].v[k]);
+                    for (int k = 0; k < V; ++k) kept[k] = acc[k];
                 }
             }
+            open = begun = true;
+            cur = row;
+            clear();
         }
-        const bool goes_on = e1 < end && row_of(entries[e1]) == cur;
-        if (!begun) {
-            to_shared(sm_head);
-            if (goes_on) flags |= kThrough;
-        } else if (goes_on) {
-            to_shared(sm_tail);
-            flags |= kTail;
-        } else {
-            write_row(cur);
-        }
+        const Pack<TG, V> g = load_pack<TG, V>(ring->slot[slot][threadIdx.x].v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += to_f32(g.v[k]);
     }
-    if (lane == 0) sm_flags[team] = (uint8_t)flags;
-    __syncthreads();
-    // runs that cross teams: the team where a run begins adds the others' parts
-    const uint32_t used = min(sh.teams, (hi - lo + per - 1) / per);
-    auto add_heads = [&](uint32_t u) {  // from team u on; true where the run ends before `used`
-        while (u < used) {
-#pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] += sm_head[(u * sh.lanes + lane) * V + k];
-            if (!(sm_flags[u] & kThrough)) return true;
-            ++u;
-        }
-        return false;
-    };
-    auto to_global = [&](float* out) {
-        if (!on || !out) return;
-#pragma unroll
-        for (int k = 0; k < V; ++k) out[col + k] = acc[k];
-    };
-    uint32_t left = 0;
-    if (team < used && (flags & kTail)) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] = sm_tail[threadIdx.x * V + k];
-        if (add_heads(team + 1)) {
-            write_row(cur);
-        } else {
-            to_global(tail);
-            if (lane == 0 && blockIdx.y == 0 && border) border->row = cur;
-            left |= kTail;
-        }
-    }
-    if (team == 0 && (flags & kHead)) {
+
+    __device__ __forceinline__ void run(float* head, float* tail, Border* border) {
+        __shared__ uint8_t sm_flags[kThreads];
+        const uint32_t team = threadIdx.x / sh.lanes, lane = threadIdx.x % sh.lanes;
+        const uint32_t pack = blockIdx.y * sh.lanes + lane;
+        on = pack < sh.packs;
+        col = (uint64_t)pack * V;
+        const uint32_t e0 = min(team * per, count);
+        uint32_t e1 = min(e0 + per, count);
+        while (e1 > e0 && row_of(ent[e1 - 1]) >= num_rows) --e1;  // at the end of the whole list only
         clear();
-        left |= kHead | (add_heads(0) ? 0u : kThrough);
-        to_global(head);
+#pragma unroll
+        for (int k = 0; k < V; ++k) kept[k] = 0.f;
+        uint32_t flags = 0;
+        cur = row_of(ent[(int)e0 - 1]);
+        open = begun = false;
+        if (e0 < e1 && row_of(ent[e0]) == cur) {  // goes on from an earlier team
+            open = true;
+            flags = kHead;
+        }
+        if constexpr (kAsync) {
+            auto fetch = [&](uint32_t i) {
+                if (i < e1 && on)
+                    copy_async<sizeof(Pack<TG, V>)>(&ring->slot[(i - e0) % kUnroll][threadIdx.x], source(ent[i]));
+                commit_copies();
+            };
+            for (uint32_t u = 0; u < kUnroll; ++u) fetch(e0 + u);
+#pragma unroll 1
+            for (uint32_t i = e0; i < e1; ++i) {
+                wait_copies<kUnroll - 1>();
+                consume(i, (i - e0) % kUnroll);
+                fetch(i + kUnroll);
+            }
+            wait_copies<0>();
+        } else {
+#pragma unroll 1
+            for (uint32_t i = e0; i < e1; i += kUnroll) {
+                Pack<TG, V> g[kUnroll];
+#pragma unroll
+                for (uint32_t u = 0; u < kUnroll; ++u)
+                    if (i + u < e1 && on) g[u] = load_pack_cs<TG, V>(source(ent[i + u]));
+#pragma unroll
+                for (uint32_t u = 0; u < kUnroll; ++u) ring->slot[u][threadIdx.x] = g[u];
+                for (uint32_t u = 0; u < kUnroll && i + u < e1; ++u) consume(i + u, u);
+            }
+        }
+        __syncthreads();  // the ring is free
+        float* sm_head = reinterpret_cast<float*>(ring);
+        float* sm_tail = sm_head + kThreads * V;
+        bool is_tail = false;
+        if (open) {
+            const bool goes_on = row_of(ent[e1]) == cur;
+            if (!begun) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) kept[k] = acc[k];
+                if (goes_on) flags |= kThrough;
+            } else if (goes_on) {
+                is_tail = true;
+                flags |= kTail;
+            } else {
+                write_row();
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            if (flags & kHead) sm_head[threadIdx.x * V + k] = kept[k];
+            if (is_tail) sm_tail[threadIdx.x * V + k] = acc[k];
+        }
+        if (lane == 0) sm_flags[team] = (uint8_t)flags;
+        __syncthreads();
+        // runs that cross teams: the team where a run begins adds the others' parts
+        const uint32_t used = min(sh.teams, (count + per - 1) / per);
+        auto add_heads = [&](uint32_t u) {  // from team u on; true where the run ends before `used`
+            for (; u < used; ++u) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) acc[k] += sm_head[(u * sh.lanes + lane) * V + k];
+                if (!(sm_flags[u] & kThrough)) return true;
+            }
+            return false;
+        };
+        auto to_global = [&](float* out) {
+            if (!on || !out) return;
+#pragma unroll
+            for (int k = 0; k < V; ++k) out[col + k] = acc[k];
+        };
+        uint32_t left = 0;
+        if (is_tail) {
+            if (add_heads(team + 1)) {
+                write_row();
+            } else {
+                to_global(tail);
+                if (lane == 0 && blockIdx.y == 0 && border) border->row = cur;
+                left |= kTail;
+            }
+        }
+        if (team == 0 && (flags & kHead)) {
+            clear();
+            left |= kHead | (add_heads(0) ? 0u : kThrough);
+            to_global(head);
+        }
+        if (border) {
+            __shared__ uint32_t sm_left;
+            if (threadIdx.x == 0) sm_left = 0;
+            __syncthreads();
+            if (left && lane == 0) atomicOr(&sm_left, left);
+            __syncthreads();
+            if (threadIdx.x == 0 && blockIdx.y == 0) border->flags = sm_left;
+        }
     }
-    if (border) {
-        __shared__ uint32_t sm_left;
-        if (threadIdx.x == 0) sm_left = 0;
-        __syncthreads();
-        if (left && lane == 0) atomicOr(&sm_left, left);
-        __syncthreads();
-        if (threadIdx.x == 0 && blockIdx.y == 0) border->flags = sm_left;
+};
+
+// The table's gradient as bytes, for rows that become zero: `step` is the
+// widest store (16, 8, 4 or 2 bytes) that rows and stride are multiples of.
+struct ZeroRows {
+    char* base;
+    uint64_t stride;
+    uint32_t bytes, step;
+};
+
+template <typename W>
+__device__ __forceinline__ void zero_rows_by(const uint8_t* touched, uint32_t r0, uint32_t r1, const ZeroRows& z) {
+    const uint32_t words = z.bytes / (uint32_t)sizeof(W);
+    uint32_t lanes = 1;
+    while (lanes < 32 && lanes < words) lanes <<= 1;
+    const uint32_t lane = threadIdx.x % lanes;
+    for (uint32_t r = r0 + threadIdx.x / lanes; r < r1; r += blockDim.x / lanes) {
+        if (touched[r - r0]) continue;
+        W* row = reinterpret_cast<W*>(z.base + (uint64_t)r * z.stride);
+        for (uint32_t c = lane; c < words; c += lanes) __stcs(row + c, W{});
     }
 }
 
-// Zeroes the rows [r0, r1) whose flag is 0: a team's lanes the same packs as above.
-template <typename TT, int V>
-__device__ __forceinline__ void zero_rows(const uint8_t* touched, uint32_t r0, uint32_t r1, const TeamShape& sh,
-                                          TT* __restrict__ dtable, uint64_t ldt) {
-    Pack<TT, V> z;
-#pragma unroll
-    for (int k = 0; k < V; ++k) z.v[k] = from_f32<TT>(0.f);
-    const uint32_t pack = blockIdx.y * sh.lanes + threadIdx.x % sh.lanes;
-    if (pack >= sh.packs) return;
-    for (uint32_t r = r0 + threadIdx.x / sh.lanes; r < r1; r += sh.teams)
-        if (!touched[r - r0]) store_pack_cs<TT, V>(dtable + (uint64_t)r * ldt + (uint64_t)pack * V, z);
+// Rows [r0, r1) whose flag is 0, by the whole CTA.
+__device__ __forceinline__ void zero_rows(const uint8_t* touched, uint32_t r0, uint32_t r1, const ZeroRows& z) {
+    if (z.step == 16) zero_rows_by<uint4>(touched, r0, r1, z);
+    else if (z.step == 8) zero_rows_by<uint2>(touched, r0, r1, z);
+    else if (z.step == 4) zero_rows_by<uint32_t>(touched, r0, r1, z);
+    else zero_rows_by<uint16_t>(touched, r0, r1, z);
+}
+
+ZeroRows rows_to_zero(const EmbeddingArgs& a) {
+    const uint64_t es = type_bytes(a.table_type);
+    ZeroRows z{static_cast<char*>(a.table), a.ldt * es, (uint32_t)(a.F * es), 16};
+    while (((uintptr_t)z.base | z.stride | z.bytes) & (z.step - 1)) z.step >>= 1;
+    return z;
 }
 
 // ------------------------------------------------------------ owner form --
@@ -295,11 +388,13 @@ constexpr int kOwnerEach = kOwnerMax / kThreads;
 
 template <typename TG, typename TT, int V>
 __global__ void __launch_bounds__(kThreads) grad_owner_kernel(
-    const TG* __restrict__ grad, uint64_t ldg, const void* __restrict__ idx, int idx_type, uint32_t n,
+    const TG* __restrict__ grad, uint32_t grad_stride, const void* __restrict__ idx, int idx_type, uint32_t n,
     int64_t padding, float scale, TT* __restrict__ dtable, uint64_t ldt, uint32_t num_rows, uint32_t rows,
-    const TeamShape sh, uint32_t* __restrict__ bad) {
-    __shared__ Entry entries[kOwnerMax];
-    __shared__ uint8_t touched[kOwnerRows];
+    const TeamShape sh, const ZeroRows zero, uint32_t* __restrict__ bad) {
+    extern __shared__ uint4 smem[];
+    Ring<TG, V>* ring = reinterpret_cast<Ring<TG, V>*>(smem);
+    Entry* entries = reinterpret_cast<Entry*>(ring + 1) + 1;  // one before, one after
+    uint8_t* touched = reinterpret_cast<uint8_t*>(entries + kOwnerMax + 1);
     __shared__ uint32_t warp_hits[kThreads / 32];
     const uint32_t r0 = blockIdx.x * rows, r1 = min(r0 + rows, num_rows);
     for (uint32_t i = threadIdx.x; i < r1 - r0; i += kThreads) touched[i] = 0;
@@ -359,10 +454,16 @@ __global__ void __launch_bounds__(kThreads) grad_owner_kernel(
                 }
                 __syncthreads();
             }
-        sum_runs<TG, TT, V>(entries, 0, total, total, (total + sh.teams - 1) / sh.teams, grad, ldg, scale, dtable,
-                            ldt, num_rows, sh, nullptr, nullptr, nullptr);
+        if (threadIdx.x == 0) entries[-1] = entries[total] = ~0ull;  // the padding of the sort is read no more
+        __syncthreads();
+        RunSums<TG, TT, V> sums{entries, total, (total + sh.teams - 1) / sh.teams, grad, grad_stride, scale,
+                                dtable,  ldt,   num_rows, sh, ring};
+        sums.run(nullptr, nullptr, nullptr);
     }
-    zero_rows<TT, V>(touched, r0, r1, sh, dtable, ldt);
+    // the CTAs of the other columns take their share of the rows
+    const uint32_t share = (r1 - r0 + gridDim.y - 1) / gridDim.y;
+    const uint32_t z0 = min(r0 + blockIdx.y * share, r1), z1 = min(z0 + share, r1);
+    zero_rows(touched + (z0 - r0), z0, z1, zero);
 }
 
 template <typename TG, typename TT, int V>
@@ -372,9 +473,13 @@ void launch_owner(const EmbeddingArgs& a, cudaStream_t s) {
     // four CTAs per SM, or what a CTA can own at most
     const uint32_t rows = std::min(kOwnerRows, std::max(1u, ceil_div(num_rows, 148 * 4)));
     const dim3 grid(ceil_div(num_rows, rows), sh.blocks);
-    grad_owner_kernel<TG, TT, V><<<grid, kThreads, 0, s>>>(
-        static_cast<const TG*>(a.rows), a.ldr, a.idx, a.idx_type, (uint32_t)a.n, a.padding, a.scale,
-        static_cast<TT*>(a.table), a.ldt, num_rows, rows, sh, a.bad);
+    const size_t smem = sizeof(Ring<TG, V>) + (kOwnerMax + 2) * sizeof(Entry) + (rows + 15) / 16 * 16;
+    // per-device attribute: set on every call (cheap), the current device may change
+    TCC_CUDA(cudaFuncSetAttribute(grad_owner_kernel<TG, TT, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  sizeof(Ring<TG, V>) + (kOwnerMax + 2) * sizeof(Entry) + kOwnerRows));
+    grad_owner_kernel<TG, TT, V><<<grid, kThreads, smem, s>>>(
+        static_cast<const TG*>(a.rows), (uint32_t)(a.ldr * sizeof(TG)), a.idx, a.idx_type, (uint32_t)a.n,
+        a.padding, a.scale, static_cast<TT*>(a.table), a.ldt, num_rows, rows, sh, rows_to_zero(a), a.bad);
     TCC_CUDA(cudaGetLastError());
 }
 
@@ -384,52 +489,56 @@ void launch_owner(const EmbeddingArgs& a, cudaStream_t s) {
 // 4 M rows), three kernels a pass: digit counts per tile, offsets, scatter.  No
 // CTA waits for another.
 
-constexpr int kTileEach = 16;
-constexpr uint32_t kTile = kThreads * kTileEach;  // entries of a tile
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kTileEach = 8;
+constexpr uint32_t kTile = kSortThreads * kTileEach;  // entries of a tile
 constexpr int kMaxDigitBits = 11;
 constexpr uint32_t kMaxDigits = 1u << kMaxDigitBits;
-constexpr int kWarps = kThreads / 32;
 
 struct IndexSource {  // pass 0: the indices themselves; rows without a gradient sort last
     const void* idx;
     int type;
     int64_t padding;
     uint32_t num_rows;
-    uint8_t* touched;
     uint32_t* bad;
-    __device__ __forceinline__ Entry load(uint32_t i, bool note) const {
+    __device__ __forceinline__ Entry load(uint32_t i) const {
         const int64_t id = load_index(idx, type, i);
-        const bool inside = id >= 0 && id < (int64_t)num_rows;
-        const bool real = inside && id != padding;
-        if (note) {
-            if (!inside && id != padding && bad) atomicExch(bad, 1u);
-            if (real) touched[id] = 1;
-        }
+        const bool real = id >= 0 && id < (int64_t)num_rows && id != padding;
         return (Entry)(real ? (uint32_t)id : num_rows) << 32 | i;
+    }
+    __device__ __forceinline__ void note(uint32_t i, Entry e) const {
+        if (bad && row_of(e) == num_rows && load_index(idx, type, i) != padding) atomicExch(bad, 1u);
     }
 };
 
 struct EntrySource {
     const Entry* entries;
-    __device__ __forceinline__ Entry load(uint32_t i, bool) const { return entries[i]; }
+    __device__ __forceinline__ Entry load(uint32_t i) const { return entries[i]; }
+    __device__ __forceinline__ void note(uint32_t, Entry) const {}
 };
 
 // counts [tile][digit], totals [digit] (zero before).
 template <typename Source>
-__global__ void __launch_bounds__(kThreads) digit_counts_kernel(const Source src, uint32_t n, int shift,
-                                                                uint32_t digits, uint32_t* __restrict__ counts,
-                                                                uint32_t* __restrict__ totals) {
+__global__ void __launch_bounds__(kSortThreads) digit_counts_kernel(const Source src, uint32_t n, int shift,
+                                                                    uint32_t digits, uint32_t* __restrict__ counts,
+                                                                    uint32_t* __restrict__ totals) {
     __shared__ uint32_t hist[kMaxDigits];
-    for (uint32_t d = threadIdx.x; d < digits; d += kThreads) hist[d] = 0;
+    for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) hist[d] = 0;
+    const uint32_t base = blockIdx.x * kTile + threadIdx.x;
+    Entry e[kTileEach];
+#pragma unroll
+    for (int k = 0; k < kTileEach; ++k)
+        if (base + k * kSortThreads < n) e[k] = src.load(base + k * kSortThreads);
     __syncthreads();
-    const uint32_t base = blockIdx.x * kTile;
-#pragma unroll 8
-    for (int k = 0; k < kTileEach; ++k) {
-        const uint32_t i = base + k * kThreads + threadIdx.x;
-        if (i < n) atomicAdd(&hist[(row_of(src.load(i, true)) >> shift) & (digits - 1)], 1u);
-    }
+#pragma unroll
+    for (int k = 0; k < kTileEach; ++k)
+        if (base + k * kSortThreads < n) {
+            atomicAdd(&hist[(row_of(e[k]) >> shift) & (digits - 1)], 1u);
+            src.note(base + k * kSortThreads, e[k]);
+        }
     __syncthreads();
-    for (uint32_t d = threadIdx.x; d < digits; d += kThreads) {
+    for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) {
         counts[(uint64_t)blockIdx.x * digits + d] = hist[d];
         if (hist[d]) atomicAdd(&totals[d], hist[d]);
     }
@@ -485,79 +594,125 @@ __global__ void __launch_bounds__(1024) digit_offsets_kernel(uint32_t* __restric
     }
 }
 
-// Stable: warp w ranks the tile's entries [w * 512, (w + 1) * 512) against its
+// Stable: warp w ranks the tile's entries [w * 256, (w + 1) * 256) against its
 // own digit counts; a prefix over the warps puts them in order.
 template <typename Source>
-__global__ void __launch_bounds__(kThreads) digit_scatter_kernel(const Source src, uint32_t n, int shift,
-                                                                 uint32_t digits,
-                                                                 const uint32_t* __restrict__ offsets,
-                                                                 Entry* __restrict__ out) {
-    __shared__ uint16_t cnt[kWarps][kMaxDigits];
+__global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const Source src, uint32_t n, int shift,
+                                                                     uint32_t digits,
+                                                                     const uint32_t* __restrict__ offsets,
+                                                                     Entry* __restrict__ out) {
+    extern __shared__ uint4 smem[];
+    uint16_t* all = reinterpret_cast<uint16_t*>(smem);  // [kSortWarps][digits]
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (uint32_t d = lane; d < digits; d += 32) cnt[warp][d] = 0;
-    __syncwarp();
-    const uint32_t base = blockIdx.x * kTile + warp * (kTile / kWarps) + lane;
+    uint16_t* cnt = all + warp * digits;
+    const uint32_t base = blockIdx.x * kTile + warp * (kTile / kSortWarps) + lane;
     Entry e[kTileEach];
     uint32_t place[kTileEach];  // digit, and the rank among the warp's entries of that digit
 #pragma unroll
     for (int k = 0; k < kTileEach; ++k) {
         const uint32_t i = base + k * 32;
-        e[k] = i < n ? src.load(i, false) : ~0ull;
+        e[k] = i < n ? src.load(i) : ~0ull;
     }
+    for (uint32_t i = threadIdx.x; i < kSortWarps * digits / 8; i += kSortThreads) smem[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < kTileEach; ++k) {
         const bool in = base + k * 32 < n;
         const uint32_t d = in ? (row_of(e[k]) >> shift) & (digits - 1) : kMaxDigits;
         const unsigned peers = __match_any_sync(0xffffffffu, d);
         const uint32_t rank = __popc(peers & lanemask_lt());
-        const uint32_t seen = in ? cnt[warp][d] : 0;
+        const uint32_t seen = in ? cnt[d] : 0;
         __syncwarp();
-        if (in && rank == 0) cnt[warp][d] = (uint16_t)(seen + __popc(peers));
+        if (in && rank == 0) cnt[d] = (uint16_t)(seen + __popc(peers));
         __syncwarp();
         place[k] = d << 16 | (seen + rank);
     }
     __syncthreads();
-    const uint32_t* offset = offsets + (uint64_t)blockIdx.x * digits;
-    for (uint32_t d = threadIdx.x; d < digits; d += kThreads) {
+    // two digits at a time, one in each half of a word (a tile has 2^12 entries)
+    for (uint32_t d = threadIdx.x; d < digits / 2; d += kSortThreads) {
+        uint32_t* col = reinterpret_cast<uint32_t*>(all) + d;
         uint32_t run = 0;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const uint32_t c = cnt[w][d];
-            cnt[w][d] = (uint16_t)run;
+        for (int w = 0; w < kSortWarps; ++w) {
+            const uint32_t c = col[w * (digits / 2)];
+            col[w * (digits / 2)] = run;
             run += c;
         }
     }
+    const uint32_t* offset = offsets + (uint64_t)blockIdx.x * digits;
+    uint32_t start[kTileEach];
+#pragma unroll
+    for (int k = 0; k < kTileEach; ++k) start[k] = base + k * 32 < n ? __ldg(offset + (place[k] >> 16)) : 0;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kTileEach; ++k) {
-        if (base + k * 32 >= n) continue;
-        const uint32_t d = place[k] >> 16;
-        out[__ldg(offset + d) + cnt[warp][d] + (place[k] & 0xFFFFu)] = e[k];
-    }
+    for (int k = 0; k < kTileEach; ++k)
+        if (base + k * 32 < n) out[start[k] + cnt[place[k] >> 16] + (place[k] & 0xFFFFu)] = e[k];
 }
 
-// Blocks [0, sums) of the grid's x: ranges of entries.  The others: rows
-// without an entry, which become zero.
+// The rows of a table range that have no entry become zero; the range's
+// entries are found by search, and rows looked up in them one by one where
+// they are too many to walk (a hub's).
+constexpr uint32_t kFillRows = 1024;
+constexpr uint32_t kFillWalk = 16384;
+
+__device__ __forceinline__ uint32_t first_of(const Entry* entries, uint32_t lo, uint32_t hi, uint32_t row) {
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (row_of(entries[mid]) < row) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ void fill_range(const Entry* __restrict__ entries, uint32_t n, uint32_t r0, uint32_t r1,
+                                           const ZeroRows& zero, uint8_t* touched, uint32_t* bounds) {
+    if (threadIdx.x < 2) bounds[threadIdx.x] = first_of(entries, 0, n, threadIdx.x ? r1 : r0);
+    for (uint32_t i = threadIdx.x; i < r1 - r0; i += kThreads) touched[i] = 0;
+    __syncthreads();
+    const uint32_t lo = bounds[0], hi = bounds[1];
+    if (hi - lo <= kFillWalk) {
+#pragma unroll 4
+        for (uint32_t i = lo + threadIdx.x; i < hi; i += kThreads) touched[row_of(entries[i]) - r0] = 1;
+    } else {
+        for (uint32_t r = r0 + threadIdx.x; r < r1; r += kThreads) {
+            const uint32_t at = first_of(entries, lo, hi, r);
+            touched[r - r0] = at < hi && row_of(entries[at]) == r;
+        }
+    }
+    __syncthreads();
+    zero_rows(touched, r0, r1, zero);
+}
+
+// CTAs [0, fills) of the grid's x fill; of the others i takes range i of the entries.
 struct SortedShape {
-    uint32_t per, range, sums, fill_rows;  // entries of a team, of a CTA; CTAs; rows of a fill CTA
+    uint32_t per, range, sums, fills;  // entries of a team, of a CTA; CTAs
 };
 
 template <typename TG, typename TT, int V>
 __global__ void __launch_bounds__(kThreads) grad_sorted_kernel(
-    const TG* __restrict__ grad, uint64_t ldg, const Entry* __restrict__ entries, uint32_t n, float scale,
+    const TG* __restrict__ grad, uint32_t grad_stride, const Entry* __restrict__ entries, uint32_t n, float scale,
     TT* __restrict__ dtable, uint64_t ldt, uint32_t num_rows, const TeamShape sh, const SortedShape so,
-    const uint8_t* __restrict__ touched, float* __restrict__ heads, float* __restrict__ tails,
-    Border* __restrict__ borders) {
-    const uint32_t width = sh.packs * V;
-    if (blockIdx.x < so.sums) {
-        const uint32_t lo = blockIdx.x * so.range, hi = min(lo + so.range, n);
-        sum_runs<TG, TT, V>(entries, lo, hi, n, so.per, grad, ldg, scale, dtable, ldt, num_rows, sh,
-                            heads + (uint64_t)blockIdx.x * width, tails + (uint64_t)blockIdx.x * width,
-                            borders + blockIdx.x);
-    } else {
-        const uint32_t r0 = (blockIdx.x - so.sums) * so.fill_rows;
-        zero_rows<TT, V>(touched + r0, r0, min(r0 + so.fill_rows, num_rows), sh, dtable, ldt);
+    const ZeroRows zero, float* __restrict__ heads, float* __restrict__ tails, Border* __restrict__ borders) {
+    extern __shared__ uint4 smem[];
+    if (blockIdx.x < so.fills) {
+        __shared__ uint32_t bounds[2];
+        static_assert(kFillRows <= sizeof(Ring<TG, V>), "flags fit");
+        // the CTAs of the other columns take their share of the rows
+        const uint32_t share = (kFillRows + gridDim.y - 1) / gridDim.y;
+        const uint32_t r0 = blockIdx.x * kFillRows + min(blockIdx.y * share, kFillRows);
+        const uint32_t r1 = min(min(r0 + share, (blockIdx.x + 1) * kFillRows), num_rows);
+        if (r0 < r1) fill_range(entries, n, r0, r1, zero, reinterpret_cast<uint8_t*>(smem), bounds);
+        return;
     }
+    const uint32_t i = blockIdx.x - so.fills, width = sh.packs * V;
+    const uint32_t lo = i * so.range, count = min(so.range, n - lo);
+    Ring<TG, V>* ring = reinterpret_cast<Ring<TG, V>*>(smem);
+    Entry* ent = reinterpret_cast<Entry*>(ring + 1);  // the entry before, the range, the entry after
+    for (uint32_t k = threadIdx.x; k < count + 2; k += kThreads)
+        ent[k] = lo + k > 0 && lo + k <= n ? entries[lo + k - 1] : ~0ull;
+    __syncthreads();
+    RunSums<TG, TT, V> sums{ent + 1, count, so.per, grad, grad_stride, scale, dtable, ldt, num_rows, sh, ring};
+    sums.run(heads + (uint64_t)i * width, tails + (uint64_t)i * width, borders + i);
 }
 
 // A block per range: where a run begins in it and goes on, its parts are added.
@@ -599,37 +754,36 @@ SortPlan sort_plan(uint64_t n, uint64_t num_rows) {
     SortPlan p;
     const int total = std::max(1, bits_for(num_rows + 1));
     p.passes = (total + kMaxDigitBits - 1) / kMaxDigitBits;
-    p.bits = (total + p.passes - 1) / p.passes;
+    p.bits = std::max(3, (total + p.passes - 1) / p.passes);  // whole 16-byte words of counts
     p.digits = 1u << p.bits;
     p.tiles = ceil_div(n, kTile);
     return p;
 }
 
 // Entries of a team: about 16 CTAs per SM over the whole list (ranges long
-// enough that few runs cross), at least 16.
+// enough that few runs cross), at least 16; of a CTA at most 1024.
+constexpr uint32_t kRangeMax = 1024;
 SortedShape sorted_shape(uint64_t n, uint64_t num_rows, const TeamShape& sh) {
     SortedShape so;
     const uint64_t per = (n / (148 * 16) + sh.teams - 1) / sh.teams;
-    so.per = (uint32_t)std::max<uint64_t>(16, (per + kUnroll - 1) / kUnroll * kUnroll);
+    so.per = (uint32_t)std::min<uint64_t>(kRangeMax / sh.teams, std::max<uint64_t>(16, per));
     so.range = so.per * sh.teams;
     so.sums = ceil_div(n, so.range);
-    so.fill_rows = 64;
-    while (num_rows / so.fill_rows > (1u << 16)) so.fill_rows <<= 1;
+    so.fills = ceil_div(num_rows, kFillRows);
     return so;
 }
 
 // Ranges whatever the vector width: a range is never below 16 entries of the
 // eight teams that full warps give.
-uint64_t max_sums(uint64_t n) { return n / (16 * kWarps) + 1; }
+uint64_t max_sums(uint64_t n) { return n / (16 * (kThreads / 32)) + 1; }
 
 struct GradScratch {
     Entry *a, *b;
     uint32_t* counts;
-    uint32_t* totals;   // [passes][digits], then `touched`: zeroed together
-    uint8_t* touched;
+    uint32_t* totals;  // [passes][digits], zero before
     float *heads, *tails;
     Border* borders;
-    size_t zero_bytes, bytes;
+    size_t total_bytes, bytes;
 };
 
 GradScratch lay_out(uint64_t n, uint64_t num_rows, uint32_t F, char* base) {
@@ -644,10 +798,8 @@ GradScratch lay_out(uint64_t n, uint64_t num_rows, uint32_t F, char* base) {
     g.a = reinterpret_cast<Entry*>(take(n * 8));
     g.b = reinterpret_cast<Entry*>(take(n * 8));
     g.counts = reinterpret_cast<uint32_t*>(take((uint64_t)p.tiles * p.digits * 4));
-    const uint64_t zero = at;
-    g.totals = reinterpret_cast<uint32_t*>(take((uint64_t)p.passes * p.digits * 4));
-    g.touched = reinterpret_cast<uint8_t*>(take(num_rows));
-    g.zero_bytes = at - zero;
+    g.total_bytes = (size_t)p.passes * p.digits * 4;
+    g.totals = reinterpret_cast<uint32_t*>(take(g.total_bytes));
     g.heads = reinterpret_cast<float*>(take(max_sums(n) * F * 4));
     g.tails = reinterpret_cast<float*>(take(max_sums(n) * F * 4));
     g.borders = reinterpret_cast<Border*>(take(max_sums(n) * sizeof(Border)));
@@ -662,8 +814,14 @@ void launch_sorted(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
     const SortPlan p = sort_plan(n, num_rows);
     const TeamShape sh = team_shape(a.F / V);
     const SortedShape so = sorted_shape(n, num_rows, sh);
-    TCC_CUDA(cudaMemsetAsync(g.totals, 0, g.zero_bytes, s));
-    const IndexSource from_idx{a.idx, a.idx_type, a.padding, num_rows, g.touched, a.bad};
+    TCC_CUDA(cudaMemsetAsync(g.totals, 0, g.total_bytes, s));
+    const IndexSource from_idx{a.idx, a.idx_type, a.padding, num_rows, a.bad};
+    const size_t smem = (size_t)kSortWarps * p.digits * sizeof(uint16_t);
+    // per-device attribute: set on every call (cheap), the current device may change
+    TCC_CUDA(cudaFuncSetAttribute(digit_scatter_kernel<IndexSource>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  kSortWarps * kMaxDigits * sizeof(uint16_t)));
+    TCC_CUDA(cudaFuncSetAttribute(digit_scatter_kernel<EntrySource>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  kSortWarps * kMaxDigits * sizeof(uint16_t)));
     Entry* in = g.b;
     Entry* out = g.a;
     for (int pass = 0; pass < p.passes; ++pass) {
@@ -671,20 +829,22 @@ void launch_sorted(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
         uint32_t* totals = g.totals + (size_t)pass * p.digits;
         const EntrySource from_entries{in};
         if (pass == 0)
-            digit_counts_kernel<<<p.tiles, kThreads, 0, s>>>(from_idx, n, shift, p.digits, g.counts, totals);
+            digit_counts_kernel<<<p.tiles, kSortThreads, 0, s>>>(from_idx, n, shift, p.digits, g.counts, totals);
         else
-            digit_counts_kernel<<<p.tiles, kThreads, 0, s>>>(from_entries, n, shift, p.digits, g.counts, totals);
+            digit_counts_kernel<<<p.tiles, kSortThreads, 0, s>>>(from_entries, n, shift, p.digits, g.counts, totals);
         digit_offsets_kernel<<<ceil_div(p.digits, 32), 1024, 0, s>>>(g.counts, p.tiles, p.digits, totals);
         if (pass == 0)
-            digit_scatter_kernel<<<p.tiles, kThreads, 0, s>>>(from_idx, n, shift, p.digits, g.counts, out);
+            digit_scatter_kernel<<<p.tiles, kSortThreads, smem, s>>>(from_idx, n, shift, p.digits, g.counts, out);
         else
-            digit_scatter_kernel<<<p.tiles, kThreads, 0, s>>>(from_entries, n, shift, p.digits, g.counts, out);
+            digit_scatter_kernel<<<p.tiles, kSortThreads, smem, s>>>(from_entries, n, shift, p.digits, g.counts, out);
         std::swap(in, out);
     }
-    const uint32_t fills = ceil_div(num_rows, so.fill_rows);
-    grad_sorted_kernel<TG, TT, V><<<dim3(so.sums + fills, sh.blocks), kThreads, 0, s>>>(
-        static_cast<const TG*>(a.rows), a.ldr, in, n, a.scale, static_cast<TT*>(a.table), a.ldt, num_rows, sh, so,
-        g.touched, g.heads, g.tails, g.borders);
+    const size_t sum_smem = sizeof(Ring<TG, V>) + (so.range + 2) * sizeof(Entry);
+    TCC_CUDA(cudaFuncSetAttribute(grad_sorted_kernel<TG, TT, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  sizeof(Ring<TG, V>) + (kRangeMax + 2) * sizeof(Entry)));
+    grad_sorted_kernel<TG, TT, V><<<dim3(so.fills + so.sums, sh.blocks), kThreads, sum_smem, s>>>(
+        static_cast<const TG*>(a.rows), (uint32_t)(a.ldr * sizeof(TG)), in, n, a.scale, static_cast<TT*>(a.table),
+        a.ldt, num_rows, sh, so, rows_to_zero(a), g.heads, g.tails, g.borders);
     if (so.sums > 1)
         grad_join_kernel<TT><<<so.sums, 128, 0, s>>>(g.borders, so.sums, g.heads, g.tails, a.F, a.scale,
                                                      static_cast<TT*>(a.table), a.ldt, num_rows);
@@ -707,7 +867,9 @@ void grad_by_width(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
     rule.count(a.ldr);
     rule.pointer(a.table, sizeof(TT));
     rule.pointer(a.rows, sizeof(TG));
-    switch (rule.width()) {
+    int width = rule.width();
+    while (width > 1 && a.F / width < kUnroll) width >>= 1;  // a team has at least kUnroll lanes
+    switch (width) {
         case 8:
             if constexpr (sizeof(TT) == 2 && sizeof(TG) == 2) launch_grad<TG, TT, 8>(a, scratch, s);
             break;
@@ -733,6 +895,7 @@ void check_embedding(const EmbeddingArgs& a) {
     TCC_REQUIRE(a.idx_type == TCC_I32 || a.idx_type == TCC_I64, "unknown index type");
     TCC_REQUIRE(a.F > 0 && a.F <= kMaxWidth, "F must be in [1, 2^20]");
     TCC_REQUIRE(a.ldt >= a.F && a.ldr >= a.F, "row strides must be >= F");
+    TCC_REQUIRE(a.ldr < (1ull << 30) && a.ldt < (1ull << 40), "row strides are too large");
     TCC_REQUIRE(a.n < (1ull << 31) && a.num_rows < (1ull << 31),
                 "fewer than 2^31 indices and table rows are supported");
     TCC_REQUIRE(a.n == 0 || (a.idx && a.rows), "indices and rows must not be NULL");
