@@ -25,69 +25,84 @@ __device__ __forceinline__ int64_t load_index(const void* idx, int type, uint64_
 // ---------------------------------------------------------------- lookup --
 
 constexpr int kLookupThreads = 256;
-constexpr int kLookupUnroll = 4;
+constexpr int kLookupUnroll = 8;
+constexpr uint32_t kZeroRow = 0xFFFFFFFFu;  // of padding and of bad indices
 
-// A CTA owns `tile` consecutive rows of the output and walks their packs in
-// memory order, so stores are contiguous at any width; the four loads of a
-// step are independent.
+// A team of 8, 16 or 32 lanes copies whole rows, a pack a lane; it holds the
+// rows of `lanes` indices at a time, one a lane, and keeps kLookupUnroll of them
+// (or of their parts, if wide) in flight.  The index is read once per row, not
+// per pack, and nothing is divided in the loop.
 template <typename TT, typename TO, int V>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(
-    const TT* __restrict__ table, uint64_t ldt, uint64_t num_rows, const void* __restrict__ idx,
-    int idx_type, uint64_t n, int64_t padding, float scale, TO* __restrict__ out, uint64_t ldo,
-    uint32_t packs, uint32_t tile, uint64_t div_magic, uint32_t* __restrict__ bad) {
-    const uint64_t row0 = (uint64_t)blockIdx.x * tile;
-    const uint32_t rows = (uint32_t)min((uint64_t)tile, n - row0);
-    const uint32_t total = rows * packs;
-    for (uint32_t base = threadIdx.x; base < total; base += kLookupThreads * kLookupUnroll) {
-        Pack<TT, V> val[kLookupUnroll];
-        uint32_t r[kLookupUnroll], c[kLookupUnroll];
-        int64_t id[kLookupUnroll];
-#pragma unroll
-        for (int u = 0; u < kLookupUnroll; ++u) {
-            const uint32_t q = base + u * kLookupThreads;
-            r[u] = tile == 1 ? 0 : (uint32_t)((q * div_magic) >> 32);
-            c[u] = q - r[u] * packs;
-            id[u] = q < total ? load_index(idx, idx_type, row0 + r[u]) : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < kLookupUnroll; ++u) {
-            const uint32_t q = base + u * kLookupThreads;
-            if (q >= total) continue;
-            const bool inside = id[u] >= 0 && (uint64_t)id[u] < num_rows;
-            if (inside && id[u] != padding) {
-                val[u] = load_pack_nc<TT, V>(table + (uint64_t)id[u] * ldt + (uint64_t)c[u] * V);
-            } else {
-#pragma unroll
-                for (int k = 0; k < V; ++k) val[u].v[k] = from_f32<TT>(0.f);
-                if (!inside && id[u] != padding && c[u] == 0 && bad) atomicExch(bad, 1u);
+    const TT* __restrict__ table, uint32_t table_stride, uint32_t num_rows, const void* __restrict__ idx,
+    int idx_type, uint32_t n, int64_t padding, float scale, TO* __restrict__ out, uint32_t out_stride,
+    uint32_t packs, uint32_t lanes, uint32_t per, uint32_t* __restrict__ bad) {
+    const uint32_t lane = threadIdx.x % lanes;
+    const uint64_t team = (uint64_t)blockIdx.x * (kLookupThreads / lanes) + threadIdx.x / lanes;
+    const uint32_t e0 = (uint32_t)min(team * per, (uint64_t)n), e1 = min(e0 + per, n);
+#pragma unroll 1
+    for (uint32_t b = 0; b < per; b += lanes) {  // the same for the whole CTA
+        const uint32_t at = e0 + b;
+        uint32_t mine = kZeroRow;
+        if (b + lane < per && at + lane < e1) {
+            const int64_t id = load_index(idx, idx_type, at + lane);
+            if (id != padding) {
+                if (id >= 0 && id < (int64_t)num_rows) mine = (uint32_t)id;
+                else if (bad) atomicExch(bad, 1u);
             }
         }
+        const uint32_t rows = e1 > at ? min(min(lanes, per - b), e1 - at) : 0;
+#pragma unroll 1
+        for (uint32_t j = 0; j < lanes && __any_sync(0xffffffffu, j < rows); j += kLookupUnroll) {
+#pragma unroll 1
+            for (uint32_t c0 = 0; c0 < packs; c0 += lanes) {
+                const uint32_t c = c0 + lane;
+                const TT* from = table + (uint64_t)c * V;
+                char* to = reinterpret_cast<char*>(out + (uint64_t)c * V) + (uint64_t)(at + j) * out_stride;
+                Pack<TT, V> val[kLookupUnroll];
+                uint32_t real = 0;  // bit u: row u is one of the table's
 #pragma unroll
-        for (int u = 0; u < kLookupUnroll; ++u) {
-            const uint32_t q = base + u * kLookupThreads;
-            if (q >= total) continue;
-            // padded rows are zero whatever the scale (an infinite scale too)
-            const bool zero = id[u] == padding || id[u] < 0 || (uint64_t)id[u] >= num_rows;
-            Pack<TO, V> o;
+                for (int u = 0; u < kLookupUnroll; ++u) {
+                    const uint32_t row = __shfl_sync(0xffffffffu, mine, j + u, lanes);
+                    if (row != kZeroRow) real |= 1u << u;
+                    if (j + u < rows && c < packs && row != kZeroRow)
+                        val[u] = load_pack_nc<TT, V>(reinterpret_cast<const TT*>(
+                            reinterpret_cast<const char*>(from) + (uint64_t)row * table_stride));
+                }
 #pragma unroll
-            for (int k = 0; k < V; ++k)
-                o.v[k] = from_f32<TO>(zero ? 0.f : to_f32(val[u].v[k]) * scale);
-            store_pack_cs<TO, V>(out + (row0 + r[u]) * ldo + (uint64_t)c[u] * V, o);
+                for (int u = 0; u < kLookupUnroll; ++u) {
+                    if (j + u >= rows || c >= packs) continue;
+                    Pack<TO, V> o;
+#pragma unroll
+                    for (int k = 0; k < V; ++k)
+                        o.v[k] = from_f32<TO>(real >> u & 1u ? to_f32(val[u].v[k]) * scale : 0.f);
+                    store_pack_cs<TO, V>(reinterpret_cast<TO*>(to + (uint64_t)u * out_stride), o);
+                }
+            }
         }
     }
+}
+
+// Teams of at least as many lanes as rows in flight: narrower packs for
+// narrow rows.
+inline int team_width(int width, uint32_t F) {
+    while (width > 1 && F / width < 8) width >>= 1;
+    return width;
 }
 
 template <typename TT, typename TO, int V>
 void launch_lookup(const EmbeddingArgs& a, cudaStream_t s) {
     const uint32_t packs = a.F / V;
-    // about eight packs a thread; whole rows per CTA
-    const uint32_t tile = std::max(1u, (uint32_t)(kLookupThreads * 8) / packs);
-    const uint64_t blocks = (a.n + tile - 1) / tile;
-    TCC_REQUIRE(blocks < (1ull << 31), "too many indices for one call");
-    const uint64_t magic = (1ull << 32) / packs + 1;  // exact for q < tile * packs <= 2048, or tile 1
-    lookup_kernel<TT, TO, V><<<(unsigned)blocks, kLookupThreads, 0, s>>>(
-        static_cast<const TT*>(a.table), a.ldt, a.num_rows, a.idx, a.idx_type, a.n, a.padding,
-        a.scale, static_cast<TO*>(a.rows), a.ldr, packs, tile, magic, a.bad);
+    uint32_t lanes = 8;
+    while (lanes < 32 && lanes < packs) lanes <<= 1;
+    // a team takes as many rows as it has lanes, fewer where that would leave SMs idle
+    const uint32_t teams = kLookupThreads / lanes;
+    uint32_t per = lanes;
+    while (per > 1 && a.n / per < 148ull * 4 * teams) per >>= 1;
+    lookup_kernel<TT, TO, V><<<ceil_div(a.n, (uint64_t)per * teams), kLookupThreads, 0, s>>>(
+        static_cast<const TT*>(a.table), (uint32_t)(a.ldt * sizeof(TT)), (uint32_t)a.num_rows, a.idx, a.idx_type,
+        (uint32_t)a.n, a.padding, a.scale, static_cast<TO*>(a.rows), (uint32_t)(a.ldr * sizeof(TO)), packs, lanes,
+        per, a.bad);
     TCC_CUDA(cudaGetLastError());
 }
 
@@ -99,7 +114,7 @@ void lookup_by_width(const EmbeddingArgs& a, cudaStream_t s) {
     rule.count(a.ldr);
     rule.pointer(a.table, sizeof(TT));
     rule.pointer(a.rows, sizeof(TO));
-    switch (rule.width()) {
+    switch (team_width(rule.width(), a.F)) {
         case 8:
             if constexpr (sizeof(TT) == 2 && sizeof(TO) == 2) launch_lookup<TT, TO, 8>(a, s);
             break;
@@ -716,18 +731,22 @@ __global__ void __launch_bounds__(kThreads) grad_sorted_kernel(
 }
 
 // A block per range: where a run begins in it and goes on, its parts are added.
-template <typename TT>
-__global__ void __launch_bounds__(128) grad_join_kernel(const Border* __restrict__ borders, uint32_t sums,
-                                                        const float* __restrict__ heads,
-                                                        const float* __restrict__ tails, uint32_t width, float scale,
-                                                        TT* __restrict__ dtable, uint64_t ldt, uint32_t num_rows) {
+// The threads are columns (of W floats) times groups; a group adds a contiguous
+// part of the ranges, and the groups' sums are added in order.
+template <typename TT, int W>
+__global__ void __launch_bounds__(kThreads) grad_join_kernel(const Border* __restrict__ borders, uint32_t sums,
+                                                             const float* __restrict__ heads,
+                                                             const float* __restrict__ tails, uint32_t width,
+                                                             float scale, TT* __restrict__ dtable, uint64_t ldt,
+                                                             uint32_t num_rows) {
     const Border b = borders[blockIdx.x];
     if (!(b.flags & kTail) || b.row >= num_rows) return;
     // the ranges after it that hold a part: up to the first that is not passed through
     __shared__ uint32_t last;
-    uint32_t from = blockIdx.x + 1;
+    __shared__ Pack<float, W> part[kThreads];
+    const uint32_t begin = blockIdx.x + 1;
     if (threadIdx.x == 0) last = sums;
-    for (;; from += 128) {
+    for (uint32_t from = begin;; from += kThreads) {
         const uint32_t i = from + threadIdx.x;
         const bool ends = i >= sums || !(borders[i].flags & kThrough);
         __syncthreads();
@@ -735,11 +754,37 @@ __global__ void __launch_bounds__(128) grad_join_kernel(const Border* __restrict
         __syncthreads();
         if (last < sums) break;
     }
-    for (uint32_t f = threadIdx.x; f < width; f += 128) {
-        float acc = tails[(uint64_t)blockIdx.x * width + f];
-#pragma unroll 8
-        for (uint32_t i = blockIdx.x + 1; i <= last; ++i) acc += heads[(uint64_t)i * width + f];
-        dtable[(uint64_t)b.row * ldt + f] = from_f32<TT>(acc * scale);
+    const uint32_t cols = width / W, parts = last + 1 - begin;
+    uint32_t across = 1;  // columns side by side
+    while (across < kThreads && across < cols) across <<= 1;
+    const uint32_t groups = kThreads / across, group = threadIdx.x / across;
+    const uint32_t each = (parts + groups - 1) / groups;
+    const uint32_t p0 = begin + min(group * each, parts), p1 = begin + min((group + 1) * each, parts);
+    for (uint32_t c0 = 0; c0 < cols; c0 += across) {
+        const uint32_t c = c0 + threadIdx.x % across;
+        Pack<float, W> acc;
+#pragma unroll
+        for (int k = 0; k < W; ++k) acc.v[k] = 0.f;
+        if (c < cols) {
+            if (group == 0) acc = load_pack<float, W>(tails + (uint64_t)blockIdx.x * width + c * W);
+#pragma unroll 4
+            for (uint32_t i = p0; i < p1; ++i) {
+                const Pack<float, W> h = load_pack<float, W>(heads + (uint64_t)i * width + c * W);
+#pragma unroll
+                for (int k = 0; k < W; ++k) acc.v[k] += h.v[k];
+            }
+        }
+        part[threadIdx.x] = acc;
+        __syncthreads();
+        if (group == 0 && c < cols) {
+            for (uint32_t g = 1; g < groups && g * each < parts; ++g)
+#pragma unroll
+                for (int k = 0; k < W; ++k) acc.v[k] += part[g * across + threadIdx.x].v[k];
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+                dtable[(uint64_t)b.row * ldt + c * W + k] = from_f32<TT>(acc.v[k] * scale);
+        }
+        __syncthreads();
     }
 }
 
@@ -845,9 +890,11 @@ void launch_sorted(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
     grad_sorted_kernel<TG, TT, V><<<dim3(so.fills + so.sums, sh.blocks), kThreads, sum_smem, s>>>(
         static_cast<const TG*>(a.rows), (uint32_t)(a.ldr * sizeof(TG)), in, n, a.scale, static_cast<TT*>(a.table),
         a.ldt, num_rows, sh, so, rows_to_zero(a), g.heads, g.tails, g.borders);
-    if (so.sums > 1)
-        grad_join_kernel<TT><<<so.sums, 128, 0, s>>>(g.borders, so.sums, g.heads, g.tails, a.F, a.scale,
-                                                     static_cast<TT*>(a.table), a.ldt, num_rows);
+    if (so.sums > 1) {
+        auto join = a.F % 4 ? grad_join_kernel<TT, 1> : grad_join_kernel<TT, 4>;
+        join<<<so.sums, kThreads, 0, s>>>(g.borders, so.sums, g.heads, g.tails, a.F, a.scale,
+                                          static_cast<TT*>(a.table), a.ldt, num_rows);
+    }
     TCC_CUDA(cudaGetLastError());
 }
 
@@ -867,9 +914,7 @@ void grad_by_width(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
     rule.count(a.ldr);
     rule.pointer(a.table, sizeof(TT));
     rule.pointer(a.rows, sizeof(TG));
-    int width = rule.width();
-    while (width > 1 && a.F / width < kUnroll) width >>= 1;  // a team has at least kUnroll lanes
-    switch (width) {
+    switch (team_width(rule.width(), a.F)) {
         case 8:
             if constexpr (sizeof(TT) == 2 && sizeof(TG) == 2) launch_grad<TG, TT, 8>(a, scratch, s);
             break;
@@ -895,7 +940,7 @@ void check_embedding(const EmbeddingArgs& a) {
     TCC_REQUIRE(a.idx_type == TCC_I32 || a.idx_type == TCC_I64, "unknown index type");
     TCC_REQUIRE(a.F > 0 && a.F <= kMaxWidth, "F must be in [1, 2^20]");
     TCC_REQUIRE(a.ldt >= a.F && a.ldr >= a.F, "row strides must be >= F");
-    TCC_REQUIRE(a.ldr < (1ull << 30) && a.ldt < (1ull << 40), "row strides are too large");
+    TCC_REQUIRE(a.ldr < (1ull << 30) && a.ldt < (1ull << 30), "row strides are too large");
     TCC_REQUIRE(a.n < (1ull << 31) && a.num_rows < (1ull << 31),
                 "fewer than 2^31 indices and table rows are supported");
     TCC_REQUIRE(a.n == 0 || (a.idx && a.rows), "indices and rows must not be NULL");
