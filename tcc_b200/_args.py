@@ -19,13 +19,25 @@ def type_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
+_bound = {}
+# The current stream's handle without building a Stream object: 0.1 us in place
+# of 2, of the 9 to 13 that a call takes on the host.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def launch(device: torch.device, name: str, *args) -> None:
     """The C call with ``device`` current, on its current stream (the last argument)."""
-    if device.index == torch.cuda.current_device():
-        L.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    call = _bound.get(name)
+    if call is None:
+        call = _bound[name] = getattr(L.lib(), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = call(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            L.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+            status = call(*args, _raw_stream(index))
+    if status:
+        L.check(status, name)
 
 
 def rows_of(t: torch.Tensor, width: int):

@@ -7,6 +7,7 @@ can be captured in a CUDA graph.
 """
 from __future__ import annotations
 
+import functools
 from array import array
 
 import torch
@@ -16,9 +17,7 @@ from ._args import TYPES, launch, scratch_for
 
 
 def _dense(t: torch.Tensor) -> bool:
-    """Whether t's elements fill one block of memory, in any order."""
-    if t.is_contiguous():
-        return True
+    """Whether the elements of a tensor that is not contiguous fill one block of memory all the same."""
     want = 1
     for size, stride in sorted(((s, st) for s, st in zip(t.shape, t.stride()) if s > 1), key=lambda p: p[1]):
         if stride != want:
@@ -29,21 +28,26 @@ def _dense(t: torch.Tensor) -> bool:
 
 def _table(tensors):
     """(tcc_tensor array of the tensors, its length, their device)."""
-    device, words = None, array("Q")
+    device, words = None, []
     for t in tensors:
         code = TYPES.get(t.dtype)
         if code is None:
             raise TypeError(f"gradients must be float32, float16 or bfloat16, not {t.dtype}")
-        if t.layout != torch.strided or not t.is_cuda:
+        if t.layout is not torch.strided or not t.is_cuda:
             raise ValueError("gradients must be dense CUDA tensors")
         if device is None:
             device = t.device
         elif t.device != device:
             raise ValueError("gradients must be on one device")
-        if not _dense(t):
+        if not (t.is_contiguous() or _dense(t)):
             raise ValueError("a gradient's elements must fill one block of memory (no gaps, no broadcast)")
-        words.extend((t.data_ptr(), t.numel(), code))  # data, n, type and reserved
-    return words, len(words) // 3, device
+        words += (t.data_ptr(), t.numel(), code)  # data, n, type and reserved
+    return array("Q", words), len(words) // 3, device
+
+
+@functools.cache
+def _scratch_bytes() -> int:
+    return L.lib().tcc_grad_norm_scratch_bytes()
 
 
 def _list(tensors) -> list:
@@ -62,7 +66,7 @@ def grad_norm(tensors) -> torch.Tensor:
     if count == 0:
         return torch.zeros(())
     norm = torch.empty((), dtype=torch.float32, device=device)
-    nbytes = L.lib().tcc_grad_norm_scratch_bytes()
+    nbytes = _scratch_bytes()
     hold, scratch = scratch_for(nbytes, device)
     launch(device, "tcc_grad_norm", words.buffer_info()[0], count, norm.data_ptr(), scratch, nbytes)
     return norm
@@ -88,7 +92,7 @@ def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6, error_if_non
     the norm they had, a float32 scalar.  Gradients of different types may mix;
     two that share memory are refused.  ``error_if_nonfinite`` waits for the norm
     and raises where it is NaN or infinite, before anything is scaled."""
-    grads = [p.grad for p in _list(parameters) if p.grad is not None]
+    grads = [g for g in (p.grad for p in _list(parameters)) if g is not None]
     if error_if_nonfinite:
         norm = grad_norm(grads)
         if not bool(torch.isfinite(norm)):
@@ -100,7 +104,7 @@ def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6, error_if_non
     if count == 0:
         return torch.zeros(())
     norm = torch.empty((), dtype=torch.float32, device=device)
-    nbytes = L.lib().tcc_grad_norm_scratch_bytes()
+    nbytes = _scratch_bytes()
     hold, scratch = scratch_for(nbytes, device)
     launch(device, "tcc_clip_grad_norm", words.buffer_info()[0], count, max_norm, eps, norm.data_ptr(), scratch,
            nbytes)

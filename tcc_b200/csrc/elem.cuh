@@ -90,6 +90,24 @@ __device__ __forceinline__ void store_pack_cs(T* p, const Pack<T, V>& v) {
     __stcs(reinterpret_cast<decltype(b.raw)*>(p), b.raw);
 }
 
+// Asynchronous copies global -> shared of one pack (4 bytes at least); a
+// thread waits for its own.
+template <typename T, int V>
+__device__ __forceinline__ void copy_pack_async(Pack<T, V>* smem, const T* global) {
+    constexpr int bytes = sizeof(T) * V;
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(smem);
+    if constexpr (bytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(global) : "memory");
+    else if constexpr (bytes >= 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(global), "n"(bytes) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// until at most LEFT of the thread's groups of copies are under way
+template <int LEFT>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
 // The widest V (of 8, 4, 2, 1; V * bytes <= 16) that divides every count in
 // `counts` and keeps every pointer aligned to V elements of its own size.
 struct VecRule {

@@ -173,20 +173,6 @@ struct Ring {
     Pack<TG, V> slot[kUnroll][kThreads];
 };
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* smem, const void* global) {
-    const uint32_t to = (uint32_t)__cvta_generic_to_shared(smem);
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(global) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(global), "n"(BYTES) : "memory");
-}
-__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void wait_copies() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-}
-
 // Sums the runs of `count` entries in shared memory, team t the entries
 // [t * per, (t + 1) * per).  ent[-1] and ent[count] are the entries before and
 // after them (~0: none).  Rows whose run lies inside are written; for the
@@ -271,7 +257,7 @@ struct RunSums {
         if constexpr (kAsync) {
             auto fetch = [&](uint32_t i) {
                 if (i < e1 && on)
-                    copy_async<sizeof(Pack<TG, V>)>(&ring->slot[(i - e0) % kUnroll][threadIdx.x], source(ent[i]));
+                    copy_pack_async<TG, V>(&ring->slot[(i - e0) % kUnroll][threadIdx.x], source(ent[i]));
                 commit_copies();
             };
             for (uint32_t u = 0; u < kUnroll; ++u) fetch(e0 + u);

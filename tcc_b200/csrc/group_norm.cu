@@ -15,15 +15,17 @@
 //
 // Two forms:
 //  * rows  (S = 1, a group within a warp): every group of a row is reduced by
-//    a few lanes of one warp, x is read once.
+//    a few lanes of one warp, x is read once; the next rows are on their way
+//    into a ring in shared memory meanwhile.
 //  * split (any other): the rows of a sample are cut into chunks, a CTA each;
 //    moments (or channel sums) per chunk, a merge over the chunks, and a
-//    second pass that normalises, in reverse order, so that what the first
-//    pass read last is still in L2.
+//    second pass that normalises, walking each chunk from its end, so that what
+//    the first pass read last is still in L2.
 #include "elem.cuh"
 #include "train_ops.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tcc {
 
@@ -32,42 +34,148 @@ namespace {
 constexpr int kThreads = 256;
 constexpr uint64_t kSms = 148;
 
-// ------------------------------------------------------------ activation --
+// ---------------------------------------------------------------- values --
 
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
-
+// V fp32 values of one thread; pairs go through the two-wide fp32
+// instructions of sm_100 (one issue slot for two values).
 template <int V>
-__device__ __forceinline__ void activate(int act, float (&z)[V]) {
-    if (act == TCC_ACT_RELU) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) z[k] = z[k] <= 0.f ? 0.f : z[k];
-    } else if (act == TCC_ACT_SILU) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) z[k] *= sigmoid(z[k]);
-    } else if (act == TCC_ACT_GELU) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) z[k] *= 0.5f * (1.f + erff(z[k] * 0.70710678118654752f));
+struct Vec {
+    float v[V];
+};
+
+#define TCC_PAIRWISE(NAME, OP, SCALAR)                                                                     \
+    template <int V>                                                                                       \
+    __device__ __forceinline__ Vec<V> NAME(const Vec<V>& a, const Vec<V>& b) {                             \
+        Vec<V> o;                                                                                          \
+        if constexpr (V % 2 == 0) {                                                                        \
+            _Pragma("unroll") for (int k = 0; k < V; k += 2)                                               \
+                asm("{.reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n " OP              \
+                    ".rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;}"                                           \
+                    : "=f"(o.v[k]), "=f"(o.v[k + 1])                                                       \
+                    : "f"(a.v[k]), "f"(a.v[k + 1]), "f"(b.v[k]), "f"(b.v[k + 1]));                         \
+        } else {                                                                                           \
+            _Pragma("unroll") for (int k = 0; k < V; ++k) o.v[k] = SCALAR;                                 \
+        }                                                                                                  \
+        return o;                                                                                          \
     }
+TCC_PAIRWISE(add, "add", a.v[k] + b.v[k])
+TCC_PAIRWISE(mul, "mul", a.v[k] * b.v[k])
+#undef TCC_PAIRWISE
+
+// a * b + c
+template <int V>
+__device__ __forceinline__ Vec<V> fma(const Vec<V>& a, const Vec<V>& b, const Vec<V>& c) {
+    Vec<V> o;
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < V; k += 2)
+            asm("{.reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n "
+                "fma.rn.f32x2 z, x, y, z;\n mov.b64 {%0, %1}, z;}"
+                : "=f"(o.v[k]), "=f"(o.v[k + 1])
+                : "f"(a.v[k]), "f"(a.v[k + 1]), "f"(b.v[k]), "f"(b.v[k + 1]), "f"(c.v[k]), "f"(c.v[k + 1]));
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) o.v[k] = fmaf(a.v[k], b.v[k], c.v[k]);
+    }
+    return o;
 }
 
-// d *= act'(z)
 template <int V>
-__device__ __forceinline__ void activate_grad(int act, const float (&z)[V], float (&d)[V]) {
+__device__ __forceinline__ Vec<V> splat(float x) {
+    Vec<V> o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) o.v[k] = x;
+    return o;
+}
+template <int V>
+__device__ __forceinline__ float sum(const Vec<V>& a) {
+    float s = a.v[0];
+#pragma unroll
+    for (int k = 1; k < V; ++k) s += a.v[k];
+    return s;
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<V> widen(const Pack<T, V>& p) {
+    Vec<V> o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) o.v[k] = to_f32(p.v[k]);
+    return o;
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> narrow(const Vec<V>& a) {
+    Pack<T, V> p;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {  // one conversion for two values
+#pragma unroll
+        for (int k = 0; k < V; k += 2) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const __half2 h = __floats2half2_rn(a.v[k], a.v[k + 1]);
+                p.v[k] = h.x, p.v[k + 1] = h.y;
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(a.v[k], a.v[k + 1]);
+                p.v[k] = h.x, p.v[k + 1] = h.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) p.v[k] = from_f32<T>(a.v[k]);
+    }
+    return p;
+}
+
+// ------------------------------------------------------------ activation --
+
+// 1 / (1 + 2^(-z log2 e)), off by a few units in the last place: the
+// hardware's exponential and reciprocal, which take one issue slot each.
+template <int V>
+__device__ __forceinline__ Vec<V> sigmoid(const Vec<V>& z) {
+    Vec<V> e = mul(z, splat<V>(-1.4426950408889634f));
+#pragma unroll
+    for (int k = 0; k < V; ++k) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.v[k]));
+    e = add(e, splat<V>(1.f));
+#pragma unroll
+    for (int k = 0; k < V; ++k) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.v[k]));
+    return e;
+}
+
+template <int V>
+__device__ __forceinline__ Vec<V> activate(int act, Vec<V> z) {
     if (act == TCC_ACT_RELU) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) d[k] = z[k] <= 0.f ? 0.f : d[k];
+        for (int k = 0; k < V; ++k) z.v[k] = z.v[k] <= 0.f ? 0.f : z.v[k];
     } else if (act == TCC_ACT_SILU) {
+        z = mul(z, sigmoid(z));
+    } else if (act == TCC_ACT_GELU) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float s = sigmoid(z[k]);
-            d[k] *= s * (1.f + z[k] * (1.f - s));
-        }
+        for (int k = 0; k < V; ++k) z.v[k] *= 0.5f * (1.f + erff(z.v[k] * 0.70710678118654752f));
+    }
+    return z;
+}
+
+// d * act'(z)
+template <int V>
+__device__ __forceinline__ Vec<V> activate_grad(int act, const Vec<V>& z, Vec<V> d) {
+    if (act == TCC_ACT_RELU) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) d.v[k] = z.v[k] <= 0.f ? 0.f : d.v[k];
+    } else if (act == TCC_ACT_SILU) {  // s + z s (1 - s)
+        const Vec<V> s = sigmoid(z), rest = fma(s, splat<V>(-1.f), splat<V>(1.f));
+        d = mul(d, fma(mul(z, s), rest, s));
     } else if (act == TCC_ACT_GELU) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const float cdf = 0.5f * (1.f + erff(z[k] * 0.70710678118654752f));
-            d[k] *= cdf + z[k] * 0.39894228040143268f * expf(-0.5f * z[k] * z[k]);
+            const float x = z.v[k], cdf = 0.5f * (1.f + erff(x * 0.70710678118654752f));
+            d.v[k] *= cdf + x * 0.39894228040143268f * expf(-0.5f * x * x);
         }
+    }
+    return d;
+}
+
+template <int V>
+__device__ __forceinline__ void load_params(const GroupNormArgs& a, uint64_t c, bool on, Vec<V>& w, Vec<V>& b) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        w.v[k] = on && a.weight ? load_typed(a.weight, a.param_type, c + k) : 1.f;
+        b.v[k] = on && a.bias ? load_typed(a.bias, a.param_type, c + k) : 0.f;
     }
 }
 
@@ -81,226 +189,225 @@ struct RowsShape {
     uint32_t L, GB, RB, packs;  // packs: of one group
 };
 
-template <int U>
-__device__ __forceinline__ void lane_sum(float (&v)[U], uint32_t L) {
-    for (uint32_t o = L >> 1; o; o >>= 1) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o);
-    }
+__device__ __forceinline__ float lane_sum(float v, uint32_t L) {
+    for (uint32_t o = L >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
-template <int V>
-__device__ __forceinline__ void load_params(const GroupNormArgs& a, uint64_t c, bool on, float (&w)[V],
-                                            float (&b)[V]) {
+// The place of a thread: its slot's group and row, and its packs' channels.
+template <int V, int J>
+struct RowsPlace {
+    uint32_t lane, g, rb;
+    bool on, ok[J];
+    uint64_t c[J];
+    Vec<V> w[J], b[J];
+    __device__ __forceinline__ RowsPlace(const GroupNormArgs& a, const RowsShape& sh) {
+        const uint32_t slot = threadIdx.x / sh.L;
+        lane = threadIdx.x % sh.L;
+        g = blockIdx.y * sh.GB + slot % sh.GB;
+        rb = slot / sh.GB;
+        on = rb < sh.RB && g < a.G;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        w[k] = on && a.weight ? load_typed(a.weight, a.param_type, c + k) : 1.f;
-        b[k] = on && a.bias ? load_typed(a.bias, a.param_type, c + k) : 0.f;
+        for (int j = 0; j < J; ++j) {
+            const uint32_t p = j * sh.L + lane;
+            ok[j] = on && p < sh.packs;
+            c[j] = (uint64_t)g * (a.C / a.G) + (uint64_t)p * V;
+            load_params<V>(a, c[j], ok[j], w[j], b[j]);
+        }
     }
-}
+};
 
-template <typename T, int V, int J, int U>
+// Ring of the packs of the next rows: D rows of J packs of A arrays.  A thread
+// copies and reads its own packs only.
+template <typename T, int V, int J, int A>
+struct RowsRing {
+    static constexpr int D = J >= 8 ? 1 : 8 / (J * A) > 2 ? 8 / (J * A) : 2;
+    static constexpr bool kAsync = sizeof(Pack<T, V>) >= 4;
+    Pack<T, V> slot[D][A][J][kThreads];
+};
+
+template <typename T, int V, int J>
 __global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormArgs a, const RowsShape sh) {
-    const uint32_t slot = threadIdx.x / sh.L, lane = threadIdx.x % sh.L;
-    const uint32_t g = blockIdx.y * sh.GB + slot % sh.GB, rb = slot / sh.GB;
-    const bool on = rb < sh.RB && g < a.G;
-    const uint32_t Cg = a.C / a.G;
-    const float inv = 1.f / (float)Cg;
+    using Ring = RowsRing<T, V, J, 1>;
+    extern __shared__ uint4 smem[];
+    Ring& ring = *reinterpret_cast<Ring*>(smem);
+    const RowsPlace<V, J> p(a, sh);
+    const float inv = 1.f / (float)(a.C / a.G);
     const T* x = static_cast<const T*>(a.x);
     T* y = static_cast<T*>(a.y);
-    bool ok[J];
-    uint64_t c[J];
-    float w[J][V], b[J][V];
+    const uint64_t stride = (uint64_t)gridDim.x * sh.RB, first = (uint64_t)blockIdx.x * sh.RB;
+    auto fetch = [&](uint64_t row0, uint32_t d) {
+        const uint64_t row = row0 + p.rb;
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const uint32_t p = j * sh.L + lane;
-        ok[j] = on && p < sh.packs;
-        c[j] = (uint64_t)g * Cg + (uint64_t)p * V;
-        load_params<V>(a, c[j], ok[j], w[j], b[j]);
-    }
-    const uint64_t stride = (uint64_t)gridDim.x * sh.RB;
-    for (uint64_t row0 = (uint64_t)blockIdx.x * sh.RB; row0 < a.N; row0 += stride * U) {
-        float v[U][J][V], s[U], q[U];
+        for (int j = 0; j < J; ++j)
+            if (p.ok[j] && row < a.N)
+                copy_pack_async<T, V>(&ring.slot[d][0][j][threadIdx.x], x + row * a.ldx + p.c[j]);
+        commit_copies();
+    };
+    if constexpr (Ring::kAsync)
+        for (uint32_t d = 0; d < Ring::D; ++d) fetch(first + d * stride, d);
+    uint32_t d = 0;
+#pragma unroll 1
+    for (uint64_t row0 = first; row0 < a.N; row0 += stride) {  // the same for the whole CTA
+        const uint64_t row = row0 + p.rb;
+        Vec<V> v[J];
+        if constexpr (Ring::kAsync) wait_copies<Ring::D - 1>();
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t row = row0 + u * stride + rb;
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                Pack<T, V> pk;
-                const bool in = ok[j] && row < a.N;
-                if (in) pk = load_pack_cs<T, V>(x + row * a.ldx + c[j]);
-#pragma unroll
-                for (int k = 0; k < V; ++k) v[u][j][k] = in ? to_f32(pk.v[k]) : 0.f;
+        for (int j = 0; j < J; ++j) {
+            v[j] = splat<V>(0.f);
+            if (p.ok[j] && row < a.N) {
+                if constexpr (Ring::kAsync) v[j] = widen<T, V>(load_pack<T, V>(ring.slot[d][0][j][threadIdx.x].v));
+                else v[j] = widen<T, V>(load_pack_cs<T, V>(x + row * a.ldx + p.c[j]));
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            s[u] = 0.f;
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-#pragma unroll
-                for (int k = 0; k < V; ++k) s[u] += v[u][j][k];
+        if constexpr (Ring::kAsync) {
+            fetch(row0 + Ring::D * stride, d);
+            d = d + 1 == Ring::D ? 0 : d + 1;
         }
-        lane_sum<U>(s, sh.L);
+        float s = 0.f, q = 0.f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            s[u] *= inv;
-            q[u] = 0.f;
+        for (int j = 0; j < J; ++j) s += sum(v[j]);
+        const float mean = lane_sum(s, sh.L) * inv;
 #pragma unroll
-            for (int j = 0; j < J; ++j)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    v[u][j][k] -= s[u];
-                    q[u] += ok[j] ? v[u][j][k] * v[u][j][k] : 0.f;
-                }
+        for (int j = 0; j < J; ++j) {
+            v[j] = add(v[j], splat<V>(-mean));
+            if (p.ok[j]) q += sum(mul(v[j], v[j]));
         }
-        lane_sum<U>(q, sh.L);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t row = row0 + u * stride + rb;
-            const float r = __frsqrt_rn(q[u] * inv + a.eps);
-            if (on && row < a.N && lane == 0 && a.mean) {
-                a.mean[row * a.G + g] = s[u];
-                a.rstd[row * a.G + g] = r;
-            }
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                if (!ok[j] || row >= a.N) continue;
-                float z[V];
-#pragma unroll
-                for (int k = 0; k < V; ++k) z[k] = v[u][j][k] * r * w[j][k] + b[j][k];
-                activate<V>(a.act, z);
-                Pack<T, V> o;
-#pragma unroll
-                for (int k = 0; k < V; ++k) o.v[k] = from_f32<T>(z[k]);
-                store_pack_cs<T, V>(y + row * a.ldy + c[j], o);
-            }
+        const float r = __frsqrt_rn(lane_sum(q, sh.L) * inv + a.eps);
+        if (row >= a.N) continue;
+        if (p.on && p.lane == 0 && a.mean) {
+            a.mean[row * a.G + p.g] = mean;
+            a.rstd[row * a.G + p.g] = r;
         }
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            if (p.ok[j])
+                store_pack_cs<T, V>(y + row * a.ldy + p.c[j],
+                                    narrow<T, V>(activate<V>(a.act, fma(mul(v[j], splat<V>(r)), p.w[j], p.b[j]))));
     }
 }
 
 // Parameter gradients: a thread's sums over its rows (kept in two levels, so
 // that the rounding error does not grow with the number of rows), then over
 // the CTA's RB rows in shared memory; one partial row per CTA of the grid's x.
-template <typename T, int V, int J, int U>
+template <typename T, int V, int J>
 __global__ void __launch_bounds__(kThreads) rows_backward_kernel(const GroupNormArgs a, const RowsShape sh,
                                                                  float* __restrict__ partial) {
-    const uint32_t slot = threadIdx.x / sh.L, lane = threadIdx.x % sh.L;
-    const uint32_t g = blockIdx.y * sh.GB + slot % sh.GB, rb = slot / sh.GB;
-    const bool on = rb < sh.RB && g < a.G;
-    const uint32_t Cg = a.C / a.G;
-    const float inv = 1.f / (float)Cg;
+    using Ring = RowsRing<T, V, J, 2>;
+    extern __shared__ uint4 smem[];
+    Ring& ring = *reinterpret_cast<Ring*>(smem);
+    const RowsPlace<V, J> p(a, sh);
+    const float inv = 1.f / (float)(a.C / a.G);
     const T* x = static_cast<const T*>(a.x);
     const T* dy = static_cast<const T*>(a.dy);
     T* dx = static_cast<T*>(a.dx);
-    bool ok[J];
-    uint64_t c[J];
-    float w[J][V], b[J][V], dw[J][V], db[J][V], dw2[J][V], db2[J][V];
+    Vec<V> dw[J], db[J], dw2[J], db2[J];
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const uint32_t p = j * sh.L + lane;
-        ok[j] = on && p < sh.packs;
-        c[j] = (uint64_t)g * Cg + (uint64_t)p * V;
-        load_params<V>(a, c[j], ok[j], w[j], b[j]);
+    for (int j = 0; j < J; ++j) dw[j] = db[j] = dw2[j] = db2[j] = splat<V>(0.f);
+    const uint64_t stride = (uint64_t)gridDim.x * sh.RB, first = (uint64_t)blockIdx.x * sh.RB;
+    auto fetch = [&](uint64_t row0, uint32_t d) {
+        const uint64_t row = row0 + p.rb;
 #pragma unroll
-        for (int k = 0; k < V; ++k) dw[j][k] = db[j][k] = dw2[j][k] = db2[j][k] = 0.f;
-    }
-    const uint64_t stride = (uint64_t)gridDim.x * sh.RB;
-    uint32_t since = 0;
-    for (uint64_t row0 = (uint64_t)blockIdx.x * sh.RB; row0 < a.N; row0 += stride * U) {
-        float h[U][J][V], d[U][J][V], s[U], q[U], r[U];
+        for (int j = 0; j < J; ++j)
+            if (p.ok[j] && row < a.N) {
+                copy_pack_async<T, V>(&ring.slot[d][0][j][threadIdx.x], x + row * a.ldx + p.c[j]);
+                copy_pack_async<T, V>(&ring.slot[d][1][j][threadIdx.x], dy + row * a.lddy + p.c[j]);
+            }
+        commit_copies();
+    };
+    // the statistics of the next row, one row ahead
+    float mean_next = 0.f, rstd_next = 0.f;
+    auto fetch_stats = [&](uint64_t row0) {
+        const uint64_t row = row0 + p.rb;
+        if (p.on && row < a.N) {
+            mean_next = a.mean[row * a.G + p.g];
+            rstd_next = a.rstd[row * a.G + p.g];
+        }
+    };
+    if constexpr (Ring::kAsync)
+        for (uint32_t d = 0; d < Ring::D; ++d) fetch(first + d * stride, d);
+    fetch_stats(first);
+    uint32_t d = 0, since = 0;
+#pragma unroll 1
+    for (uint64_t row0 = first; row0 < a.N; row0 += stride) {
+        const uint64_t row = row0 + p.rb;
+        const float mean = mean_next, r = rstd_next;
+        fetch_stats(row0 + stride);
+        Vec<V> h[J], g[J];
+        if constexpr (Ring::kAsync) wait_copies<Ring::D - 1>();
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t row = row0 + u * stride + rb;
-            const bool live = on && row < a.N;
-            const float mean = live ? a.mean[row * a.G + g] : 0.f;
-            r[u] = live ? a.rstd[row * a.G + g] : 0.f;
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const bool in = ok[j] && row < a.N;
-                Pack<T, V> px, pd;
-                if (in) {
-                    px = load_pack_cs<T, V>(x + row * a.ldx + c[j]);
-                    pd = load_pack_cs<T, V>(dy + row * a.lddy + c[j]);
+        for (int j = 0; j < J; ++j) {
+            h[j] = g[j] = splat<V>(0.f);
+            if (p.ok[j] && row < a.N) {
+                if constexpr (Ring::kAsync) {
+                    h[j] = widen<T, V>(load_pack<T, V>(ring.slot[d][0][j][threadIdx.x].v));
+                    g[j] = widen<T, V>(load_pack<T, V>(ring.slot[d][1][j][threadIdx.x].v));
+                } else {
+                    h[j] = widen<T, V>(load_pack_cs<T, V>(x + row * a.ldx + p.c[j]));
+                    g[j] = widen<T, V>(load_pack_cs<T, V>(dy + row * a.lddy + p.c[j]));
                 }
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    h[u][j][k] = in ? (to_f32(px.v[k]) - mean) * r[u] : 0.f;
-                    d[u][j][k] = in ? to_f32(pd.v[k]) : 0.f;
-                }
+                h[j] = mul(add(h[j], splat<V>(-mean)), splat<V>(r));
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            s[u] = q[u] = 0.f;
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                float z[V];
-#pragma unroll
-                for (int k = 0; k < V; ++k) z[k] = h[u][j][k] * w[j][k] + b[j][k];
-                activate_grad<V>(a.act, z, d[u][j]);
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    db[j][k] += d[u][j][k];
-                    dw[j][k] += d[u][j][k] * h[u][j][k];
-                    d[u][j][k] *= w[j][k];
-                    s[u] += d[u][j][k];
-                    q[u] += d[u][j][k] * h[u][j][k];
-                }
-            }
+        if constexpr (Ring::kAsync) {
+            fetch(row0 + Ring::D * stride, d);
+            d = d + 1 == Ring::D ? 0 : d + 1;
         }
-        lane_sum<U>(s, sh.L);
-        lane_sum<U>(q, sh.L);
+        float s = 0.f, q = 0.f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (a.act != TCC_ACT_NONE) g[j] = activate_grad<V>(a.act, fma(h[j], p.w[j], p.b[j]), g[j]);
+            db[j] = add(db[j], g[j]);
+            dw[j] = fma(g[j], h[j], dw[j]);
+            g[j] = mul(g[j], p.w[j]);
+            s += sum(g[j]);
+            q += sum(mul(g[j], h[j]));
+        }
         if (dx) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint64_t row = row0 + u * stride + rb;
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    if (!ok[j] || row >= a.N) continue;
-                    Pack<T, V> o;
-#pragma unroll
-                    for (int k = 0; k < V; ++k)
-                        o.v[k] = from_f32<T>(r[u] * (d[u][j][k] - (s[u] + h[u][j][k] * q[u]) * inv));
-                    store_pack_cs<T, V>(dx + row * a.lddx + c[j], o);
-                }
-            }
-        }
-        if ((since += U) >= 32) {
-            since = 0;
+            s = lane_sum(s, sh.L) * inv;
+            q = lane_sum(q, sh.L) * inv;
 #pragma unroll
             for (int j = 0; j < J; ++j)
+                if (p.ok[j] && row < a.N)
+                    store_pack_cs<T, V>(dx + row * a.lddx + p.c[j],
+                                        narrow<T, V>(mul(splat<V>(r), fma(h[j], splat<V>(-q),
+                                                                          add(g[j], splat<V>(-s))))));
+        }
+        if (++since == 32) {
+            since = 0;
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    dw2[j][k] += dw[j][k];
-                    db2[j][k] += db[j][k];
-                    dw[j][k] = db[j][k] = 0.f;
-                }
+            for (int j = 0; j < J; ++j) {
+                dw2[j] = add(dw2[j], dw[j]);
+                db2[j] = add(db2[j], db[j]);
+                dw[j] = db[j] = splat<V>(0.f);
+            }
         }
     }
     if (!partial) return;
-    __shared__ float sm[2][kThreads * V];
+    if constexpr (Ring::kAsync) wait_copies<0>();
+    float* sm = reinterpret_cast<float*>(smem);  // [2][kThreads][V], in the ring's place
+    static_assert(sizeof(Ring) >= 2 * kThreads * V * sizeof(float) || !Ring::kAsync, "sums fit");
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            sm[0][threadIdx.x * V + k] = dw2[j][k] + dw[j][k];
-            sm[1][threadIdx.x * V + k] = db2[j][k] + db[j][k];
+            sm[threadIdx.x * V + k] = dw2[j].v[k] + dw[j].v[k];
+            sm[(kThreads + threadIdx.x) * V + k] = db2[j].v[k] + db[j].v[k];
         }
         __syncthreads();
-        if (rb == 0 && ok[j]) {
+        if (p.rb == 0 && p.ok[j]) {
             float* out = partial + (uint64_t)blockIdx.x * 2 * a.C;
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 float tw = 0.f, tb = 0.f;
                 for (uint32_t i = 0; i < sh.RB; ++i) {
                     const uint32_t t = (threadIdx.x + i * sh.GB * sh.L) * V + k;
-                    tw += sm[0][t];
-                    tb += sm[1][t];
+                    tw += sm[t];
+                    tb += sm[kThreads * V + t];
                 }
-                out[c[j] + k] = tw;
-                out[a.C + c[j] + k] = tb;
+                out[p.c[j] + k] = tw;
+                out[a.C + p.c[j] + k] = tb;
             }
         }
     }
@@ -401,31 +508,32 @@ __global__ void __launch_bounds__(kThreads) split_moments_kernel(const GroupNorm
     Moments m{0.f, 0.f, 0.f};
     if (p.on) {
         for (uint64_t r = p.row0 + p.rb; r < p.row1; r += (uint64_t)sh.RB * kBlockRows) {
-            float v[kBlockRows][V], s = 0.f, q = 0.f;
+            Vec<V> v[kBlockRows];
+            float s = 0.f, q = 0.f;
             int rows = 0;
 #pragma unroll
             for (int u = 0; u < kBlockRows; ++u) {
                 const uint64_t row = r + (uint64_t)u * sh.RB;
-                Pack<T, V> pk;
+                v[u] = splat<V>(0.f);
                 if (row < p.row1) {
-                    pk = load_pack<T, V>(x + row * a.ldx);
+                    v[u] = widen<T, V>(load_pack<T, V>(x + row * a.ldx));
                     ++rows;
                 }
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    v[u][k] = row < p.row1 ? to_f32(pk.v[k]) : 0.f;
-                    s += v[u][k];
-                }
             }
+            Vec<V> t = v[0];
+#pragma unroll
+            for (int u = 1; u < kBlockRows; ++u) t = add(t, v[u]);
+            s = sum(t);
             const float n = (float)(rows * V);
-            const float mean = s / n;
+            const float mean = __fdividef(s, n);
+            t = splat<V>(0.f);
 #pragma unroll
             for (int u = 0; u < kBlockRows; ++u)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const float d = v[u][k] - mean;
-                    q += u < rows ? d * d : 0.f;
+                if (u < rows) {
+                    const Vec<V> e = add(v[u], splat<V>(-mean));
+                    t = fma(e, e, t);
                 }
+            q = sum(t);
             m = merge(m, Moments{n, mean, q});
         }
     }
@@ -450,19 +558,14 @@ __global__ void __launch_bounds__(kThreads) split_moments_kernel(const GroupNorm
         partial[(p.n * sh.chunks + p.chunk) * ((uint64_t)a.G * sh.SUB) + p.slot] = sm[threadIdx.x];
 }
 
-// A warp per (sample, group) merges its partial moments.
-__global__ void __launch_bounds__(kThreads) split_stats_kernel(const Moments* __restrict__ partial,
-                                                               uint64_t N, uint32_t G, uint32_t SUB,
-                                                               uint32_t chunks, float eps,
-                                                               float* __restrict__ mean,
-                                                               float* __restrict__ rstd) {
-    const uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
-    if (i >= N * G) return;
-    const uint32_t lane = threadIdx.x & 31;
-    const uint64_t n = i / G;
-    const uint32_t g = (uint32_t)(i - n * G);
+// A CTA of one or eight warps per (sample, group) merges its partial moments.
+__global__ void split_stats_kernel(const Moments* __restrict__ partial, uint32_t G, uint32_t SUB, uint32_t chunks,
+                                   float eps, float* __restrict__ mean, float* __restrict__ rstd) {
+    __shared__ Moments sm[8];
+    const uint64_t n = blockIdx.x / G;
+    const uint32_t g = (uint32_t)(blockIdx.x - n * G);
     Moments m{0.f, 0.f, 0.f};
-    for (uint32_t k = lane; k < chunks * SUB; k += 32) {
+    for (uint32_t k = threadIdx.x; k < chunks * SUB; k += blockDim.x) {
         const uint32_t ch = k / SUB;
         m = merge(m, partial[(n * chunks + ch) * ((uint64_t)G * SUB) + g * SUB + (k - ch * SUB)]);
     }
@@ -473,10 +576,23 @@ __global__ void __launch_bounds__(kThreads) split_stats_kernel(const Moments* __
         t.m2 = __shfl_down_sync(0xffffffffu, m.m2, o);
         m = merge(m, t);
     }
-    if (lane == 0) {
-        mean[i] = m.mean;
-        rstd[i] = __frsqrt_rn(m.m2 / m.n + eps);
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (uint32_t w = 1; w < blockDim.x / 32; ++w) m = merge(m, sm[w]);
+        mean[blockIdx.x] = m.mean;
+        rstd[blockIdx.x] = __frsqrt_rn(m.m2 / m.n + eps);
     }
+}
+
+// fn(row) for the thread's rows, from the chunk's end.
+template <typename Fn>
+__device__ __forceinline__ void rows_backwards(const SplitPlace& p, const SplitShape& sh, Fn&& fn) {
+    if (p.row0 + p.rb >= p.row1) return;
+    const uint64_t steps = (p.row1 - 1 - p.row0 - p.rb) / sh.RB;
+    int64_t r = (int64_t)(p.row0 + p.rb + steps * sh.RB);
+#pragma unroll 4
+    for (; r >= (int64_t)p.row0; r -= sh.RB) fn((uint64_t)r);
 }
 
 template <typename T, int V>
@@ -487,21 +603,13 @@ __global__ void __launch_bounds__(kThreads) split_apply_kernel(const GroupNormAr
     if (!p.on) return;
     const T* x = static_cast<const T*>(a.x) + p.n * a.S * a.ldx + p.c;
     T* y = static_cast<T*>(a.y) + p.n * a.S * a.ldy + p.c;
-    const float mean = mean_[p.n * a.G + p.g], rstd = rstd_[p.n * a.G + p.g];
-    float w[V], b[V];
+    const Vec<V> less = splat<V>(-mean_[p.n * a.G + p.g]), rstd = splat<V>(rstd_[p.n * a.G + p.g]);
+    Vec<V> w, b;
     load_params<V>(a, p.c, true, w, b);
-#pragma unroll 4
-    for (uint64_t r = p.row0 + p.rb; r < p.row1; r += sh.RB) {
-        const Pack<T, V> pk = load_pack<T, V>(x + r * a.ldx);
-        float z[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) z[k] = (to_f32(pk.v[k]) - mean) * rstd * w[k] + b[k];
-        activate<V>(a.act, z);
-        Pack<T, V> o;
-#pragma unroll
-        for (int k = 0; k < V; ++k) o.v[k] = from_f32<T>(z[k]);
-        store_pack_cs<T, V>(y + r * a.ldy, o);
-    }
+    rows_backwards(p, sh, [&](uint64_t r) {
+        const Vec<V> h = mul(add(widen<T, V>(load_pack<T, V>(x + r * a.ldx)), less), rstd);
+        store_pack_cs<T, V>(y + r * a.ldy, narrow<T, V>(activate<V>(a.act, fma(h, w, b))));
+    });
 }
 
 // Per chunk and channel: sums of dz * h and of dz -> partial [N][chunks][2][C].
@@ -509,39 +617,27 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) split_sums_kernel(const GroupNormArgs a, const SplitShape sh,
                                                               float* __restrict__ partial) {
     const SplitPlace p = split_place<V>(a, sh, false);
-    float dw[V], db[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) dw[k] = db[k] = 0.f;
+    Vec<V> dw = splat<V>(0.f), db = dw;
     if (p.on) {
         const T* x = static_cast<const T*>(a.x) + p.n * a.S * a.ldx + p.c;
         const T* dy = static_cast<const T*>(a.dy) + p.n * a.S * a.lddy + p.c;
-        const float mean = a.mean[p.n * a.G + p.g], rstd = a.rstd[p.n * a.G + p.g];
-        float w[V], b[V];
+        const Vec<V> less = splat<V>(-a.mean[p.n * a.G + p.g]), rstd = splat<V>(a.rstd[p.n * a.G + p.g]);
+        Vec<V> w, b;
         load_params<V>(a, p.c, true, w, b);
 #pragma unroll 4
         for (uint64_t r = p.row0 + p.rb; r < p.row1; r += sh.RB) {
-            const Pack<T, V> px = load_pack<T, V>(x + r * a.ldx);
-            const Pack<T, V> pd = load_pack<T, V>(dy + r * a.lddy);
-            float h[V], z[V], d[V];
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                h[k] = (to_f32(px.v[k]) - mean) * rstd;
-                z[k] = h[k] * w[k] + b[k];
-                d[k] = to_f32(pd.v[k]);
-            }
-            activate_grad<V>(a.act, z, d);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                db[k] += d[k];
-                dw[k] += d[k] * h[k];
-            }
+            const Pack<T, V> px = load_pack<T, V>(x + r * a.ldx), pd = load_pack<T, V>(dy + r * a.lddy);
+            const Vec<V> h = mul(add(widen<T, V>(px), less), rstd);
+            const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pd));
+            db = add(db, d);
+            dw = fma(d, h, dw);
         }
     }
     __shared__ float sm[2][kThreads * V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        sm[0][threadIdx.x * V + k] = dw[k];
-        sm[1][threadIdx.x * V + k] = db[k];
+        sm[0][threadIdx.x * V + k] = dw.v[k];
+        sm[1][threadIdx.x * V + k] = db.v[k];
     }
     __syncthreads();
     if (p.on && p.rb == 0) {
@@ -559,42 +655,44 @@ __global__ void __launch_bounds__(kThreads) split_sums_kernel(const GroupNormArg
     }
 }
 
-// sums [N][2][C] over the chunks.
-__global__ void __launch_bounds__(kThreads) split_fold_kernel(const float* __restrict__ partial, uint64_t N,
-                                                              uint32_t C, uint32_t chunks,
-                                                              float* __restrict__ sums) {
-    const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= N * 2 * C) return;
-    const uint64_t n = i / (2ull * C), c = i - n * 2 * C;
-    double s = 0.0;
-#pragma unroll 8
-    for (uint32_t k = 0; k < chunks; ++k) s += (double)partial[(n * chunks + k) * 2 * C + c];
-    sums[i] = (float)s;
-}
-
-// group_sums [N][G][2]: a = sum of weight * (sum dz), b = sum of weight * (sum dz * h); a warp each.
-__global__ void __launch_bounds__(kThreads) split_groups_kernel(const GroupNormArgs a,
-                                                                const float* __restrict__ sums,
-                                                                float* __restrict__ group_sums) {
-    const uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
-    if (i >= a.N * a.G) return;
-    const uint32_t lane = threadIdx.x & 31;
-    const uint64_t n = i / a.G;
-    const uint32_t g = (uint32_t)(i - n * a.G), Cg = a.C / a.G;
-    float s = 0.f, q = 0.f;
-    for (uint32_t k = lane; k < Cg; k += 32) {
+// group_sums [N][G][2]: a = sum of weight * (sum dz), b = sum of weight * (sum
+// dz * h), from the chunks' sums; a CTA per (sample, group), 32 channels at a
+// time by blockDim.y rows of threads over the chunks.
+__global__ void split_groups_kernel(const GroupNormArgs a, const float* __restrict__ partial, uint32_t chunks,
+                                    float* __restrict__ group_sums) {
+    __shared__ double sm[2][32];
+    const uint64_t n = blockIdx.x / a.G;
+    const uint32_t g = (uint32_t)(blockIdx.x - n * a.G), Cg = a.C / a.G;
+    double s = 0.0, q = 0.0;
+    for (uint32_t k = threadIdx.x; k < Cg; k += 32) {
         const uint32_t c = g * Cg + k;
-        const float w = a.weight ? load_typed(a.weight, a.param_type, c) : 1.f;
-        q += w * sums[n * 2 * a.C + c];
-        s += w * sums[n * 2 * a.C + a.C + c];
+        float tw = 0.f, tb = 0.f;
+#pragma unroll 4
+        for (uint32_t i = threadIdx.y; i < chunks; i += blockDim.y) {
+            const float* row = partial + (n * chunks + i) * 2 * a.C + c;
+            tw += row[0];
+            tb += row[a.C];
+        }
+        const double w = a.weight ? (double)load_typed(a.weight, a.param_type, c) : 1.0;
+        q += w * tw;
+        s += w * tb;
     }
     for (int o = 16; o; o >>= 1) {
         s += __shfl_xor_sync(0xffffffffu, s, o);
         q += __shfl_xor_sync(0xffffffffu, q, o);
     }
-    if (lane == 0) {
-        group_sums[2 * i] = s;
-        group_sums[2 * i + 1] = q;
+    if (threadIdx.x == 0) {
+        sm[0][threadIdx.y] = s;
+        sm[1][threadIdx.y] = q;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && threadIdx.y == 0) {
+        for (uint32_t i = 1; i < blockDim.y; ++i) {
+            s += sm[0][i];
+            q += sm[1][i];
+        }
+        group_sums[2 * blockIdx.x] = (float)s;
+        group_sums[2 * blockIdx.x + 1] = (float)q;
     }
 }
 
@@ -608,26 +706,16 @@ __global__ void __launch_bounds__(kThreads) split_grad_kernel(const GroupNormArg
     T* dx = static_cast<T*>(a.dx) + p.n * a.S * a.lddx + p.c;
     const uint64_t i = p.n * a.G + p.g;
     const float inv = 1.f / ((float)a.S * (float)(a.C / a.G));
-    const float mean = a.mean[i], rstd = a.rstd[i], s = group_sums[2 * i] * inv, q = group_sums[2 * i + 1] * inv;
-    float w[V], b[V];
+    const Vec<V> less = splat<V>(-a.mean[i]), rstd = splat<V>(a.rstd[i]);
+    const Vec<V> s = splat<V>(-group_sums[2 * i] * inv), q = splat<V>(-group_sums[2 * i + 1] * inv);
+    Vec<V> w, b;
     load_params<V>(a, p.c, true, w, b);
-#pragma unroll 4
-    for (uint64_t r = p.row0 + p.rb; r < p.row1; r += sh.RB) {
-        const Pack<T, V> px = load_pack<T, V>(x + r * a.ldx);
-        const Pack<T, V> pd = load_pack<T, V>(dy + r * a.lddy);
-        float h[V], z[V], d[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            h[k] = (to_f32(px.v[k]) - mean) * rstd;
-            z[k] = h[k] * w[k] + b[k];
-            d[k] = to_f32(pd.v[k]);
-        }
-        activate_grad<V>(a.act, z, d);
-        Pack<T, V> o;
-#pragma unroll
-        for (int k = 0; k < V; ++k) o.v[k] = from_f32<T>(rstd * (d[k] * w[k] - (s + h[k] * q)));
-        store_pack_cs<T, V>(dx + r * a.lddx, o);
-    }
+    rows_backwards(p, sh, [&](uint64_t r) {
+        const Pack<T, V> px = load_pack<T, V>(x + r * a.ldx), pd = load_pack<T, V>(dy + r * a.lddy);
+        const Vec<V> h = mul(add(widen<T, V>(px), less), rstd);
+        const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pd));
+        store_pack_cs<T, V>(dx + r * a.lddx, narrow<T, V>(mul(rstd, fma(h, q, fma(d, w, s)))));
+    });
 }
 
 // ------------------------------------------------------------------ host --
@@ -647,8 +735,10 @@ int pick_width(const GroupNormArgs& a) {
     return rule.width();
 }
 
-// The rows form holds up to 8 packs a lane.
-bool rows_form(uint64_t S, uint32_t Cg, int V) { return S == 1 && Cg <= 32u * 8u * (uint32_t)V; }
+// The rows form holds up to 8 packs and 32 values a lane.
+bool rows_form(uint64_t S, uint32_t Cg, int V) {
+    return S == 1 && Cg <= 32u * std::min(8u * (uint32_t)V, 32u);
+}
 
 RowsShape rows_shape(uint32_t C, uint32_t G, int V) {
     RowsShape sh;
@@ -661,14 +751,14 @@ RowsShape rows_shape(uint32_t C, uint32_t G, int V) {
     return sh;
 }
 
-// Enough CTAs in x to fill the GPU with eight per SM, whole passes over the rows.
+// CTAs in x: as many as run at once (`per_sm`, which the ring's size allows).
 uint64_t rows_blocks(const RowsShape& sh, uint64_t N, uint32_t G, uint64_t per_sm) {
     const uint64_t y = (G + sh.GB - 1) / sh.GB;
     return std::max<uint64_t>(1, std::min((N + sh.RB - 1) / sh.RB, kSms * per_sm / std::min(kSms, y)));
 }
 
-// Chunks of a sample: about eight CTAs per SM over all samples, at least eight
-// rows a thread, at most 512 chunks to merge.
+// Chunks of a sample: eight CTAs per SM over all samples, which all run at
+// once; at least eight rows a thread.
 SplitShape split_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V) {
     SplitShape sh;
     sh.PG = C / G / V;
@@ -687,7 +777,7 @@ SplitShape split_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V) {
     }
     const uint64_t want = std::max<uint64_t>(1, kSms * 8 / std::max<uint64_t>(1, std::min(N, kSms * 8) * sh.cols));
     const uint64_t most = std::max<uint64_t>(1, S / (8 * sh.RB));
-    const uint64_t chunks = std::min<uint64_t>(512, std::min(want, most));
+    const uint64_t chunks = std::min(want, most);
     sh.chunk_rows = (S + chunks - 1) / chunks;
     sh.chunks = (uint32_t)((S + sh.chunk_rows - 1) / sh.chunk_rows);
     return sh;
@@ -697,7 +787,7 @@ uint32_t sub_slots(uint32_t C, uint32_t G) { return (C / G + kThreads - 1) / kTh
 
 // Upper bounds over every vector width, so that the size does not depend on
 // the pointers' alignment.
-constexpr uint64_t kRowsPerSm = 8;
+constexpr uint64_t kForwardPerSm = 6, kBackwardPerSm = 4;
 
 }  // namespace
 
@@ -706,13 +796,13 @@ size_t group_norm_scratch_bytes(uint64_t N, uint64_t S, uint32_t C, uint32_t G, 
     uint64_t rows = 0, chunks = 1;
     for (int V = 1; V <= 8; V <<= 1) {
         if ((C / G) % V) break;
-        if (rows_form(S, C / G, V)) rows = std::max(rows, rows_blocks(rows_shape(C, G, V), N, G, kRowsPerSm));
+        if (rows_form(S, C / G, V)) rows = std::max(rows, rows_blocks(rows_shape(C, G, V), N, G, kBackwardPerSm));
         chunks = std::max<uint64_t>(chunks, split_shape(N, S, C, G, V).chunks);
     }
     if (!backward && rows_form(S, C / G, 1)) return 0;  // whichever width is picked
     const uint64_t stats = 2 * align256(N * G * 4);
     if (!backward) return (size_t)(align256(N * chunks * G * sub_slots(C, G) * sizeof(Moments)) + stats);
-    return (size_t)(align256(std::max(rows, N * chunks) * 2 * C * 4) + align256(N * 2 * C * 4) + stats);
+    return (size_t)(align256(std::max(rows, N * chunks) * 2 * C * 4) + stats);
 }
 
 namespace {
@@ -749,11 +839,17 @@ void check_norm(const GroupNormArgs& a, void* scratch, size_t scratch_bytes, boo
 template <typename T, int V, int J>
 void rows_launch(const GroupNormArgs& a, float* partial, bool backward, cudaStream_t s) {
     const RowsShape sh = rows_shape(a.C, a.G, V);
-    const dim3 grid((unsigned)rows_blocks(sh, a.N, a.G, kRowsPerSm), (a.G + sh.GB - 1) / sh.GB);
+    const dim3 grid((unsigned)rows_blocks(sh, a.N, a.G, backward ? kBackwardPerSm : kForwardPerSm), (a.G + sh.GB - 1) / sh.GB);
     TCC_REQUIRE(grid.y <= 65535, "too many groups for one-row samples");
-    constexpr int U = V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1;
-    if (backward) rows_backward_kernel<T, V, J, U><<<grid, kThreads, 0, s>>>(a, sh, partial);
-    else rows_forward_kernel<T, V, J, U><<<grid, kThreads, 0, s>>>(a, sh);
+    const void* kernel = backward ? (const void*)rows_backward_kernel<T, V, J> : (const void*)rows_forward_kernel<T, V, J>;
+    // where nothing is copied ahead, room for the sums alone
+    const size_t smem = std::max<size_t>(backward ? sizeof(RowsRing<T, V, J, 2>) : sizeof(RowsRing<T, V, J, 1>),
+                                         backward ? 2 * kThreads * V * sizeof(float) : 0);
+    // per-device attribute: set on every call (cheap), the current device may change
+    if (smem > 48 * 1024)
+        TCC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (backward) rows_backward_kernel<T, V, J><<<grid, kThreads, smem, s>>>(a, sh, partial);
+    else rows_forward_kernel<T, V, J><<<grid, kThreads, smem, s>>>(a, sh);
     TCC_CUDA(cudaGetLastError());
     if (backward && partial) {
         param_grad_kernel<<<(2 * a.C + 31) / 32, 1024, 0, s>>>(partial, grid.x, a.C, a.dweight, a.dbias,
@@ -769,7 +865,7 @@ void rows_by_packs(const GroupNormArgs& a, float* partial, bool backward, cudaSt
     if (per_lane <= 1) rows_launch<T, V, 1>(a, partial, backward, s);
     else if (per_lane <= 2) rows_launch<T, V, 2>(a, partial, backward, s);
     else if (per_lane <= 4) rows_launch<T, V, 4>(a, partial, backward, s);
-    else rows_launch<T, V, 8>(a, partial, backward, s);
+    else if constexpr (V <= 4) rows_launch<T, V, 8>(a, partial, backward, s);
 }
 
 template <typename T, int V>
@@ -780,9 +876,10 @@ void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStrea
         return;
     }
     const SplitShape sh = split_shape(a.N, a.S, a.C, a.G, V);
-    TCC_REQUIRE(a.N * sh.chunks < (1ull << 31) && sh.cols <= 65535, "too many samples or groups for one call");
+    TCC_REQUIRE(a.N * sh.chunks < (1ull << 31) && a.N * a.G < (1ull << 31) && sh.cols <= 65535, "too many samples or groups for one call");
     const dim3 grid((unsigned)(a.N * sh.chunks), sh.cols);
-    const unsigned warps = ceil_div(a.N * a.G, kThreads / 32);
+    const unsigned groups = (unsigned)(a.N * a.G);
+    const bool many = sh.chunks * sh.SUB > 64;  // partial results of a group
     if (!backward) {
         Moments* partial = reinterpret_cast<Moments*>(scratch);
         float* mean = a.mean;
@@ -792,20 +889,19 @@ void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStrea
             rstd = mean + align256(a.N * a.G * 4) / 4;
         }
         split_moments_kernel<T, V><<<grid, kThreads, 0, s>>>(a, sh, partial);
-        split_stats_kernel<<<warps, kThreads, 0, s>>>(partial, a.N, a.G, sh.SUB, sh.chunks, a.eps, mean, rstd);
+        split_stats_kernel<<<groups, many ? kThreads : 32, 0, s>>>(partial, a.G, sh.SUB, sh.chunks, a.eps, mean, rstd);
         split_apply_kernel<T, V><<<grid, kThreads, 0, s>>>(a, sh, mean, rstd);
     } else {
         float* partial = reinterpret_cast<float*>(scratch);
-        float* sums = partial + align256(a.N * sh.chunks * 2 * a.C * 4) / 4;
-        float* group_sums = sums + align256(a.N * 2 * a.C * 4) / 4;
+        float* group_sums = partial + align256(a.N * sh.chunks * 2 * a.C * 4) / 4;
         split_sums_kernel<T, V><<<grid, kThreads, 0, s>>>(a, sh, partial);
-        split_fold_kernel<<<ceil_div(a.N * 2 * a.C, kThreads), kThreads, 0, s>>>(partial, a.N, a.C, sh.chunks, sums);
-        if (params)
-            param_grad_kernel<<<(2 * a.C + 31) / 32, 1024, 0, s>>>(sums, a.N, a.C, a.dweight, a.dbias, a.param_type);
         if (a.dx) {
-            split_groups_kernel<<<warps, kThreads, 0, s>>>(a, sums, group_sums);
+            split_groups_kernel<<<groups, dim3(32, many ? 32 : 4), 0, s>>>(a, partial, sh.chunks, group_sums);
             split_grad_kernel<T, V><<<grid, kThreads, 0, s>>>(a, sh, group_sums);
         }
+        if (params)
+            param_grad_kernel<<<(2 * a.C + 31) / 32, 1024, 0, s>>>(partial, a.N * sh.chunks, a.C, a.dweight, a.dbias,
+                                                                  a.param_type);
     }
     TCC_CUDA(cudaGetLastError());
 }

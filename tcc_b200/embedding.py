@@ -32,8 +32,6 @@ def _index(idx: torch.Tensor, device: torch.device):
 
 
 def _bad_flag(bad, device):
-    if bad is None:
-        return None
     if bad.dtype != torch.int32 or bad.device != device or bad.numel() < 1:
         raise ValueError("bad must be an int32 tensor of one element on the rows' device")
     return bad.data_ptr()
@@ -43,19 +41,26 @@ def _lookup(table, idx, scale, padding_idx, out_dtype, bad):
     code = type_code(table, "table")
     if table.dim() != 2:
         raise ValueError("the table must be 2-D")
-    width = table.shape[1]
-    if width > 1 and table.stride(1) != 1:
+    num_rows, width = table.shape
+    ld, col = table.stride()
+    if width > 1 and col != 1:
         raise ValueError("the table must have unit column stride")
-    ld = table.stride(0) if table.shape[0] > 1 else max(width, 1)
-    out_dtype = table.dtype if out_dtype is None else out_dtype
-    if out_dtype != table.dtype and out_dtype != torch.float32:
+    if num_rows < 2:
+        ld = max(width, 1)
+    if out_dtype is None or out_dtype == table.dtype:
+        out_dtype, out_code = table.dtype, code
+    elif out_dtype == torch.float32:
+        out_code = L.F32
+    else:
         raise TypeError("out_dtype must be the table's or float32")
-    idx, idx_code = _index(idx, table.device)
-    out = torch.empty((*idx.shape, width), dtype=out_dtype, device=table.device)
-    if out.numel():
-        launch(table.device, "tcc_embedding_forward", table.data_ptr(), code, ld, table.shape[0],
-               idx.data_ptr(), idx_code, idx.numel(), L.NO_PADDING if padding_idx is None else padding_idx,
-               scale, out.data_ptr(), TYPES[out_dtype], width, width, _bad_flag(bad, table.device))
+    device = table.device
+    idx, idx_code = _index(idx, device)
+    out = torch.empty((*idx.shape, width), dtype=out_dtype, device=device)
+    n = idx.numel()
+    if n and width:
+        launch(device, "tcc_embedding_forward", table.data_ptr(), code, ld, num_rows, idx.data_ptr(), idx_code, n,
+               L.NO_PADDING if padding_idx is None else padding_idx, scale, out.data_ptr(), out_code, width, width,
+               None if bad is None else _bad_flag(bad, device))
     return out
 
 
@@ -83,7 +88,7 @@ def embedding_backward(grad_out: torch.Tensor, idx: torch.Tensor, num_rows: int,
         hold, scratch = scratch_for(nbytes, device)
         launch(device, "tcc_embedding_backward", grad_out.data_ptr(), code, ld, idx.data_ptr(), idx_code, n,
                L.NO_PADDING if padding_idx is None else padding_idx, scale, out.data_ptr(), TYPES[dtype],
-               width, num_rows, width, scratch, nbytes, _bad_flag(bad, device))
+               width, num_rows, width, scratch, nbytes, None if bad is None else _bad_flag(bad, device))
     return out
 
 

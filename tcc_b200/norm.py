@@ -16,50 +16,63 @@ from . import _lib as L
 from ._args import launch, rows_of, scratch_for, type_code
 
 
+def _parameter(p, name: str, channels: int, x: torch.Tensor):
+    if p.dim() != 1 or p.shape[0] != channels:
+        raise ValueError(f"{name} must have shape ({channels},)")
+    if p.device != x.device:
+        raise ValueError(f"{name} must be on x's device")
+    return p if p.is_contiguous() else p.contiguous()
+
+
 def _parameters(weight, bias, channels: int, x: torch.Tensor):
     """(weight, bias, their type) contiguous; checks shape, type and device."""
     code = L.F32
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        code = type_code(p, name)
-        if p.shape != (channels,):
-            raise ValueError(f"{name} must have shape ({channels},)")
-        if p.device != x.device:
-            raise ValueError(f"{name} must be on x's device")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError("weight and bias must have one type")
-    return (None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), code)
+    if weight is not None:
+        code = type_code(weight, "weight")
+        weight = _parameter(weight, "weight", channels, x)
+    if bias is not None:
+        code = type_code(bias, "bias")
+        bias = _parameter(bias, "bias", channels, x)
+        if weight is not None and weight.dtype != bias.dtype:
+            raise TypeError("weight and bias must have one type")
+    return weight, bias, code
 
 
 def _sizes(x: torch.Tensor, num_groups: int):
-    if x.dim() < 2:
+    shape = x.shape
+    if len(shape) < 2:
         raise ValueError("x must be [N, ..., C]")
-    channels = x.shape[-1]
+    channels = shape[-1]
     if num_groups < 1 or channels < 1 or channels % num_groups:
         raise ValueError("num_groups must divide a positive number of channels")
-    return x.shape[0], math.prod(x.shape[1:-1]), channels
+    return shape[0], 1 if len(shape) == 2 else math.prod(shape[1:-1]), channels
 
 
 def _activation(act: str) -> int:
-    if act not in L.ACTIVATIONS:
+    code = L.ACTIVATIONS.get(act)
+    if code is None:
         raise ValueError(f"act must be one of {', '.join(L.ACTIVATIONS)}")
-    return L.ACTIVATIONS[act]
+    return code
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _empty(x):
+    """A contiguous tensor of x's shape, type and device."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _forward(x, num_groups, weight, bias, eps, act, stats):
     code, act = type_code(x, "x"), _activation(act)
     n, steps, channels = _sizes(x, num_groups)
     weight, bias, p_code = _parameters(weight, bias, channels, x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _empty(x)
     mean = rstd = None
     if stats:
         mean, rstd = torch.empty((2, n, num_groups), dtype=torch.float32, device=x.device).unbind(0)
-    if y.numel():
+    if n and steps:
         x, ld = rows_of(x, channels)
         nbytes = L.lib().tcc_group_norm_scratch_bytes(n, steps, channels, num_groups, 0)
         hold, scratch = scratch_for(nbytes, x.device)
@@ -92,7 +105,7 @@ def group_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
         if s.shape != (n, num_groups) or s.dtype != torch.float32 or s.device != x.device or not s.is_contiguous():
             raise ValueError(f"{name} must be a contiguous float32 [N, num_groups] tensor on x's device")
     weight, bias, p_code = _parameters(weight, bias, channels, x)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
+    dx = _empty(x) if need_dx else None
     dweight = None if weight is None else torch.empty_like(weight)
     dbias = None if bias is None else torch.empty_like(bias)
     x, ldx = rows_of(x, channels)
