@@ -217,6 +217,19 @@ struct RowsPlace {
     }
 };
 
+// wait_copies with a pass number that is a constant once the loop is unrolled.
+template <int D>
+__device__ __forceinline__ void wait_pass(uint32_t d) {
+    if (d == 0) wait_copies<D - 1>();
+    else if (d == 1) wait_copies<(D > 2 ? D - 2 : 0)>();
+    else if (d == 2) wait_copies<(D > 3 ? D - 3 : 0)>();
+    else if (d == 3) wait_copies<(D > 4 ? D - 4 : 0)>();
+    else if (d == 4) wait_copies<(D > 5 ? D - 5 : 0)>();
+    else if (d == 5) wait_copies<(D > 6 ? D - 6 : 0)>();
+    else if (d == 6) wait_copies<(D > 7 ? D - 7 : 0)>();
+    else wait_copies<0>();
+}
+
 // Ring of the packs of the next rows: D rows of J packs of A arrays.  A thread
 // copies and reads its own packs only.
 template <typename T, int V, int J, int A>
@@ -226,43 +239,48 @@ struct RowsRing {
     Pack<T, V> slot[D][A][J][kThreads];
 };
 
+// A CTA takes `passes` times RB neighbouring rows, at most what its ring holds:
+// it asks for all of them at once and is done, so reads and writes of many CTAs
+// mix (a persistent grid: 975 us at 2.4 M x 256 fp32, this one: see below).
+// mean and rstd are staged and leave in whole sectors (written from the lanes
+// that hold them they cost 70 us there).
 template <typename T, int V, int J>
-__global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormArgs a, const RowsShape sh) {
+__global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormArgs a, const RowsShape sh,
+                                                                uint32_t passes) {
     using Ring = RowsRing<T, V, J, 1>;
     extern __shared__ uint4 smem[];
     Ring& ring = *reinterpret_cast<Ring*>(smem);
+    float* stats = reinterpret_cast<float*>(smem + sizeof(Ring) / 16);  // [2][passes][RB][GB]
     const RowsPlace<V, J> p(a, sh);
     const float inv = 1.f / (float)(a.C / a.G);
-    const T* x = static_cast<const T*>(a.x);
-    T* y = static_cast<T*>(a.y);
-    const uint64_t stride = (uint64_t)gridDim.x * sh.RB, first = (uint64_t)blockIdx.x * sh.RB;
-    auto fetch = [&](uint64_t row0, uint32_t d) {
-        const uint64_t row = row0 + p.rb;
+    const uint64_t first = (uint64_t)blockIdx.x * passes * sh.RB;
+    const T* x = static_cast<const T*>(a.x) + (first + p.rb) * a.ldx;
+    T* y = static_cast<T*>(a.y) + (first + p.rb) * a.ldy;
+    auto live = [&](uint32_t d) { return first + (uint64_t)d * sh.RB + p.rb < a.N; };
+    if constexpr (Ring::kAsync) {
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-            if (p.ok[j] && row < a.N)
-                copy_pack_async<T, V>(&ring.slot[d][0][j][threadIdx.x], x + row * a.ldx + p.c[j]);
-        commit_copies();
-    };
-    if constexpr (Ring::kAsync)
-        for (uint32_t d = 0; d < Ring::D; ++d) fetch(first + d * stride, d);
-    uint32_t d = 0;
-#pragma unroll 1
-    for (uint64_t row0 = first; row0 < a.N; row0 += stride) {  // the same for the whole CTA
-        const uint64_t row = row0 + p.rb;
+        for (uint32_t d = 0; d < Ring::D; ++d) {
+            if (d < passes && live(d))
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+                    if (p.ok[j])
+                        copy_pack_async<T, V>(&ring.slot[d][0][j][threadIdx.x], x + (uint64_t)d * sh.RB * a.ldx + p.c[j]);
+            commit_copies();
+        }
+    }
+#pragma unroll
+    for (uint32_t d = 0; d < Ring::D; ++d) {
+        if (d >= passes) break;
+        const bool on = live(d);
         Vec<V> v[J];
-        if constexpr (Ring::kAsync) wait_copies<Ring::D - 1>();
+        if constexpr (Ring::kAsync) wait_pass<Ring::D>(d);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             v[j] = splat<V>(0.f);
-            if (p.ok[j] && row < a.N) {
+            if (p.ok[j] && on) {
                 if constexpr (Ring::kAsync) v[j] = widen<T, V>(load_pack<T, V>(ring.slot[d][0][j][threadIdx.x].v));
-                else v[j] = widen<T, V>(load_pack_cs<T, V>(x + row * a.ldx + p.c[j]));
+                else v[j] = widen<T, V>(load_pack_cs<T, V>(x + (uint64_t)d * sh.RB * a.ldx + p.c[j]));
             }
-        }
-        if constexpr (Ring::kAsync) {
-            fetch(row0 + Ring::D * stride, d);
-            d = d + 1 == Ring::D ? 0 : d + 1;
         }
         float s = 0.f, q = 0.f;
 #pragma unroll
@@ -274,16 +292,27 @@ __global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormA
             if (p.ok[j]) q += sum(mul(v[j], v[j]));
         }
         const float r = __frsqrt_rn(lane_sum(q, sh.L) * inv + a.eps);
-        if (row >= a.N) continue;
+        if (!on) continue;
         if (p.on && p.lane == 0 && a.mean) {
-            a.mean[row * a.G + p.g] = mean;
-            a.rstd[row * a.G + p.g] = r;
+            const uint32_t at = (d * sh.RB + p.rb) * sh.GB + (p.g - blockIdx.y * sh.GB);
+            stats[at] = mean;
+            stats[passes * sh.RB * sh.GB + at] = r;
         }
 #pragma unroll
         for (int j = 0; j < J; ++j)
             if (p.ok[j])
-                store_pack_cs<T, V>(y + row * a.ldy + p.c[j],
+                store_pack_cs<T, V>(y + (uint64_t)d * sh.RB * a.ldy + p.c[j],
                                     narrow<T, V>(activate<V>(a.act, fma(mul(v[j], splat<V>(r)), p.w[j], p.b[j]))));
+    }
+    if (!a.mean) return;
+    __syncthreads();
+    const uint32_t rows = (uint32_t)min((uint64_t)passes * sh.RB, a.N - first), g0 = blockIdx.y * sh.GB;
+    const uint32_t groups = min(sh.GB, a.G - g0);
+    for (uint32_t i = threadIdx.x; i < rows * groups; i += kThreads) {
+        const uint32_t row = i / groups, g = i - row * groups;
+        const uint64_t to = (first + row) * a.G + g0 + g;
+        a.mean[to] = stats[row * sh.GB + g];
+        a.rstd[to] = stats[passes * sh.RB * sh.GB + row * sh.GB + g];
     }
 }
 
@@ -413,20 +442,23 @@ __global__ void __launch_bounds__(kThreads) rows_backward_kernel(const GroupNorm
     }
 }
 
-// dweight, dbias [C] = column sums of partial [rows][2][C], in 64 bits.
+// dweight, dbias [C] = column sums of partial [rows][2][C], in 64 bits; a CTA
+// takes 8 columns (a sector of a row) by 128 rows of threads.
 __global__ void __launch_bounds__(1024) param_grad_kernel(const float* __restrict__ partial, uint64_t rows,
                                                           uint32_t C, void* dweight, void* dbias, int type) {
-    __shared__ double sm[32][33];
-    const uint32_t tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const uint64_t c = (uint64_t)blockIdx.x * 32 + tx;  // of 2 C
+    __shared__ double sm[32][8];
+    const uint32_t tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const uint64_t c = (uint64_t)blockIdx.x * 8 + tx;  // of 2 C
     double s = 0.0;
     if (c < 2ull * C) {
 #pragma unroll 4
-        for (uint64_t r = ty; r < rows; r += 32) s += (double)partial[r * 2 * C + c];
+        for (uint64_t r = ty; r < rows; r += 128) s += (double)partial[r * 2 * C + c];
     }
-    sm[ty][tx] = s;
+    s += __shfl_xor_sync(0xffffffffu, s, 8);
+    s += __shfl_xor_sync(0xffffffffu, s, 16);
+    if ((threadIdx.x & 31) < 8) sm[threadIdx.x >> 5][tx] = s;
     __syncthreads();
-    if (ty == 0 && c < 2ull * C) {
+    if (threadIdx.x < 8 && c < 2ull * C) {
         double t = 0.0;
         for (int i = 0; i < 32; ++i) t += sm[i][tx];
         void* out = c < C ? dweight : dbias;
@@ -498,45 +530,93 @@ __device__ __forceinline__ Moments merge(const Moments& a, const Moments& b) {
     return o;
 }
 
-constexpr int kBlockRows = 4;  // rows of a thread's block of values
+// Calls body(packs[B][A], how many of the B rows there are) for `count` rows of
+// A arrays, `inc` elements from one row to the next, B rows at a time; the next
+// D rows are on their way into the thread's part of `ring` ([D][A][kThreads])
+// meanwhile.  Registers hold B rows only, so that enough warps fit to hide the
+// exponentials and the memory (rows prefetched into registers: 128 registers,
+// 100 us in place of 56 for the sums of 232,965 x 256 bf16).
+template <typename T, int V, int A, int D, int B, typename Body>
+__device__ __forceinline__ void stream_rows(void* smem, const T* const (&from)[A], const int64_t (&inc)[A],
+                                            uint32_t count, Body&& body) {
+    constexpr bool kAsync = sizeof(Pack<T, V>) >= 4;
+    Pack<T, V>* ring = static_cast<Pack<T, V>*>(smem) + threadIdx.x;
+    const T* at[A];
+#pragma unroll
+    for (int i = 0; i < A; ++i) at[i] = from[i];
+    auto fetch = [&](uint32_t k) {
+        if (k < count)
+#pragma unroll
+            for (int i = 0; i < A; ++i) {
+                copy_pack_async<T, V>(ring + ((k & (D - 1)) * A + i) * kThreads, at[i]);
+                at[i] += inc[i];
+            }
+        commit_copies();
+    };
+    if constexpr (kAsync)
+        for (uint32_t k = 0; k < D; ++k) fetch(k);
+#pragma unroll 1
+    for (uint32_t k = 0; k < count; k += B) {
+        Pack<T, V> v[B][A];
+        if constexpr (kAsync) wait_copies<D - B>();
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+            if (k + u < count)
+#pragma unroll
+                for (int i = 0; i < A; ++i) {
+                    if constexpr (kAsync) {
+                        v[u][i] = load_pack<T, V>(ring[(((k + u) & (D - 1)) * A + i) * kThreads].v);
+                    } else {
+                        v[u][i] = load_pack<T, V>(at[i]);
+                        at[i] += inc[i];
+                    }
+                }
+        if constexpr (kAsync)
+#pragma unroll
+            for (int u = 0; u < B; ++u) fetch(k + D + u);
+        body(v, min((uint32_t)B, count - k));
+    }
+    if constexpr (kAsync) wait_copies<0>();
+}
+
+// Rows of this thread in its chunk.
+__device__ __forceinline__ uint32_t own_rows(const SplitPlace& p, const SplitShape& sh) {
+    const uint64_t first = p.row0 + p.rb;
+    return p.on && first < p.row1 ? (uint32_t)((p.row1 - 1 - first) / sh.RB) + 1 : 0;
+}
+
+constexpr int kBlockRows = 4;               // rows of a thread's block of values
+constexpr int kDepth1 = 8, kDepth2 = 4;     // rows ahead of one array, of two
+template <typename T, int V, int A>
+constexpr size_t ring_bytes() {
+    return (A == 1 ? kDepth1 : kDepth2) * A * kThreads * sizeof(Pack<T, V>);
+}
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) split_moments_kernel(const GroupNormArgs a, const SplitShape sh,
+__global__ void __launch_bounds__(kThreads, 3) split_moments_kernel(const GroupNormArgs a, const SplitShape sh,
                                                                  Moments* __restrict__ partial) {
+    extern __shared__ uint4 smem[];
     const SplitPlace p = split_place<V>(a, sh, false);
-    const T* x = static_cast<const T*>(a.x) + p.n * a.S * a.ldx + p.c;
+    const T* const from[1] = {static_cast<const T*>(a.x) + (p.n * a.S + p.row0 + p.rb) * a.ldx + p.c};
+    const int64_t inc[1] = {(int64_t)(sh.RB * a.ldx)};
     Moments m{0.f, 0.f, 0.f};
-    if (p.on) {
-        for (uint64_t r = p.row0 + p.rb; r < p.row1; r += (uint64_t)sh.RB * kBlockRows) {
-            Vec<V> v[kBlockRows];
-            float s = 0.f, q = 0.f;
-            int rows = 0;
+    stream_rows<T, V, 1, kDepth1, kBlockRows>(smem, from, inc, own_rows(p, sh), [&](const auto& pk, uint32_t rows) {
+        Vec<V> v[kBlockRows], t = splat<V>(0.f);
 #pragma unroll
-            for (int u = 0; u < kBlockRows; ++u) {
-                const uint64_t row = r + (uint64_t)u * sh.RB;
-                v[u] = splat<V>(0.f);
-                if (row < p.row1) {
-                    v[u] = widen<T, V>(load_pack<T, V>(x + row * a.ldx));
-                    ++rows;
-                }
-            }
-            Vec<V> t = v[0];
-#pragma unroll
-            for (int u = 1; u < kBlockRows; ++u) t = add(t, v[u]);
-            s = sum(t);
-            const float n = (float)(rows * V);
-            const float mean = __fdividef(s, n);
-            t = splat<V>(0.f);
-#pragma unroll
-            for (int u = 0; u < kBlockRows; ++u)
-                if (u < rows) {
-                    const Vec<V> e = add(v[u], splat<V>(-mean));
-                    t = fma(e, e, t);
-                }
-            q = sum(t);
-            m = merge(m, Moments{n, mean, q});
+        for (uint32_t u = 0; u < kBlockRows; ++u) {
+            v[u] = u < rows ? widen<T, V>(pk[u][0]) : splat<V>(0.f);
+            t = add(t, v[u]);
         }
-    }
+        const float n = (float)(rows * V), mean = __fdividef(sum(t), n);
+        t = splat<V>(0.f);
+#pragma unroll
+        for (uint32_t u = 0; u < kBlockRows; ++u)
+            if (u < rows) {
+                const Vec<V> e = add(v[u], splat<V>(-mean));
+                t = fma(e, e, t);
+            }
+        m = merge(m, Moments{n, mean, sum(t)});
+    });
     __shared__ Moments sm[kThreads];
     sm[threadIdx.x] = m;
     __syncthreads();
@@ -585,55 +665,52 @@ __global__ void split_stats_kernel(const Moments* __restrict__ partial, uint32_t
     }
 }
 
-// fn(row) for the thread's rows, from the chunk's end.
-template <typename Fn>
-__device__ __forceinline__ void rows_backwards(const SplitPlace& p, const SplitShape& sh, Fn&& fn) {
-    if (p.row0 + p.rb >= p.row1) return;
-    const uint64_t steps = (p.row1 - 1 - p.row0 - p.rb) / sh.RB;
-    int64_t r = (int64_t)(p.row0 + p.rb + steps * sh.RB);
-#pragma unroll 4
-    for (; r >= (int64_t)p.row0; r -= sh.RB) fn((uint64_t)r);
-}
-
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) split_apply_kernel(const GroupNormArgs a, const SplitShape sh,
                                                                const float* __restrict__ mean_,
                                                                const float* __restrict__ rstd_) {
+    extern __shared__ uint4 smem[];
     const SplitPlace p = split_place<V>(a, sh, true);
-    if (!p.on) return;
-    const T* x = static_cast<const T*>(a.x) + p.n * a.S * a.ldx + p.c;
-    T* y = static_cast<T*>(a.y) + p.n * a.S * a.ldy + p.c;
+    const uint32_t count = own_rows(p, sh);
+    if (!count) return;
+    const uint64_t last = p.n * a.S + p.row0 + p.rb + (uint64_t)(count - 1) * sh.RB;
+    const T* const from[1] = {static_cast<const T*>(a.x) + last * a.ldx + p.c};
+    const int64_t inc[1] = {-(int64_t)(sh.RB * a.ldx)};
+    T* y = static_cast<T*>(a.y) + last * a.ldy + p.c;
     const Vec<V> less = splat<V>(-mean_[p.n * a.G + p.g]), rstd = splat<V>(rstd_[p.n * a.G + p.g]);
     Vec<V> w, b;
     load_params<V>(a, p.c, true, w, b);
-    rows_backwards(p, sh, [&](uint64_t r) {
-        const Vec<V> h = mul(add(widen<T, V>(load_pack<T, V>(x + r * a.ldx)), less), rstd);
-        store_pack_cs<T, V>(y + r * a.ldy, narrow<T, V>(activate<V>(a.act, fma(h, w, b))));
+    stream_rows<T, V, 1, kDepth1, 1>(smem, from, inc, count, [&](const auto& pk, uint32_t) {
+        const Vec<V> h = mul(add(widen<T, V>(pk[0][0]), less), rstd);
+        store_pack_cs<T, V>(y, narrow<T, V>(activate<V>(a.act, fma(h, w, b))));
+        y -= sh.RB * a.ldy;
     });
 }
 
 // Per chunk and channel: sums of dz * h and of dz -> partial [N][chunks][2][C].
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) split_sums_kernel(const GroupNormArgs a, const SplitShape sh,
+__global__ void __launch_bounds__(kThreads, 3) split_sums_kernel(const GroupNormArgs a, const SplitShape sh,
                                                               float* __restrict__ partial) {
     const SplitPlace p = split_place<V>(a, sh, false);
+    extern __shared__ uint4 smem[];
     Vec<V> dw = splat<V>(0.f), db = dw;
-    if (p.on) {
-        const T* x = static_cast<const T*>(a.x) + p.n * a.S * a.ldx + p.c;
-        const T* dy = static_cast<const T*>(a.dy) + p.n * a.S * a.lddy + p.c;
+    if (const uint32_t count = own_rows(p, sh)) {
+        const uint64_t first = p.n * a.S + p.row0 + p.rb;
+        const T* const from[2] = {static_cast<const T*>(a.x) + first * a.ldx + p.c,
+                                  static_cast<const T*>(a.dy) + first * a.lddy + p.c};
+        const int64_t inc[2] = {(int64_t)(sh.RB * a.ldx), (int64_t)(sh.RB * a.lddy)};
         const Vec<V> less = splat<V>(-a.mean[p.n * a.G + p.g]), rstd = splat<V>(a.rstd[p.n * a.G + p.g]);
         Vec<V> w, b;
         load_params<V>(a, p.c, true, w, b);
-#pragma unroll 4
-        for (uint64_t r = p.row0 + p.rb; r < p.row1; r += sh.RB) {
-            const Pack<T, V> px = load_pack<T, V>(x + r * a.ldx), pd = load_pack<T, V>(dy + r * a.lddy);
-            const Vec<V> h = mul(add(widen<T, V>(px), less), rstd);
-            const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pd));
+        stream_rows<T, V, 2, kDepth2, 1>(smem, from, inc, count, [&](const auto& pk, uint32_t) {
+            const Vec<V> h = mul(add(widen<T, V>(pk[0][0]), less), rstd);
+            const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
             db = add(db, d);
             dw = fma(d, h, dw);
-        }
+        });
     }
-    __shared__ float sm[2][kThreads * V];
+    __syncthreads();
+    float(*sm)[kThreads * V] = reinterpret_cast<float(*)[kThreads * V]>(smem);  // [2], in the ring's place
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         sm[0][threadIdx.x * V + k] = dw.v[k];
@@ -656,65 +733,85 @@ __global__ void __launch_bounds__(kThreads) split_sums_kernel(const GroupNormArg
 }
 
 // group_sums [N][G][2]: a = sum of weight * (sum dz), b = sum of weight * (sum
-// dz * h), from the chunks' sums; a CTA per (sample, group), 32 channels at a
-// time by blockDim.y rows of threads over the chunks.
+// dz * h), from the chunks' sums; a CTA per (sample, group), `cw` channels at a
+// time (a power of two up to a warp) by blockDim.x / cw threads over the
+// chunks.  With one sample the channels' sums are the parameters' gradients.
 __global__ void split_groups_kernel(const GroupNormArgs a, const float* __restrict__ partial, uint32_t chunks,
-                                    float* __restrict__ group_sums) {
-    __shared__ double sm[2][32];
+                                    uint32_t cw, float* __restrict__ group_sums, bool params) {
+    __shared__ double sm[2][32][32];
     const uint64_t n = blockIdx.x / a.G;
     const uint32_t g = (uint32_t)(blockIdx.x - n * a.G), Cg = a.C / a.G;
-    double s = 0.0, q = 0.0;
-    for (uint32_t k = threadIdx.x; k < Cg; k += 32) {
-        const uint32_t c = g * Cg + k;
-        float tw = 0.f, tb = 0.f;
+    const uint32_t tx = threadIdx.x % cw, ty = threadIdx.x / cw, rows = blockDim.x / cw, warps = blockDim.x / 32;
+    double s = 0.0, q = 0.0;  // of the group; in the first cw threads
+    for (uint32_t k0 = 0; k0 < Cg; k0 += cw) {
+        const uint32_t c = g * Cg + k0 + tx;
+        const bool on = k0 + tx < Cg;
+        double tw = 0.0, tb = 0.0;
+        if (on) {
 #pragma unroll 4
-        for (uint32_t i = threadIdx.y; i < chunks; i += blockDim.y) {
-            const float* row = partial + (n * chunks + i) * 2 * a.C + c;
-            tw += row[0];
-            tb += row[a.C];
+            for (uint32_t i = ty; i < chunks; i += rows) {
+                const float* row = partial + (n * chunks + i) * 2 * a.C + c;
+                tw += (double)row[0];
+                tb += (double)row[a.C];
+            }
         }
-        const double w = a.weight ? (double)load_typed(a.weight, a.param_type, c) : 1.0;
-        q += w * tw;
-        s += w * tb;
-    }
-    for (int o = 16; o; o >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        q += __shfl_xor_sync(0xffffffffu, q, o);
-    }
-    if (threadIdx.x == 0) {
-        sm[0][threadIdx.y] = s;
-        sm[1][threadIdx.y] = q;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0 && threadIdx.y == 0) {
-        for (uint32_t i = 1; i < blockDim.y; ++i) {
-            s += sm[0][i];
-            q += sm[1][i];
+        for (uint32_t o = 16; o >= cw; o >>= 1) {  // the rows of threads in a warp
+            tw += __shfl_xor_sync(0xffffffffu, tw, o);
+            tb += __shfl_xor_sync(0xffffffffu, tb, o);
         }
-        group_sums[2 * blockIdx.x] = (float)s;
-        group_sums[2 * blockIdx.x + 1] = (float)q;
+        __syncthreads();
+        if ((threadIdx.x & 31) < cw) {
+            sm[0][threadIdx.x >> 5][tx] = tw;
+            sm[1][threadIdx.x >> 5][tx] = tb;
+        }
+        __syncthreads();
+        if (threadIdx.x < cw && on) {
+            for (uint32_t i = 1; i < warps; ++i) {
+                tw += sm[0][i][tx];
+                tb += sm[1][i][tx];
+            }
+            const double w = a.weight ? (double)load_typed(a.weight, a.param_type, c) : 1.0;
+            q += w * tw;
+            s += w * tb;
+            if (params && a.dweight) store_typed(a.dweight, a.param_type, c, (float)tw);
+            if (params && a.dbias) store_typed(a.dbias, a.param_type, c, (float)tb);
+        }
+    }
+    if (threadIdx.x < 32) {
+        for (int o = 16; o; o >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            q += __shfl_xor_sync(0xffffffffu, q, o);
+        }
+        if (threadIdx.x == 0) {
+            group_sums[2 * blockIdx.x] = (float)s;
+            group_sums[2 * blockIdx.x + 1] = (float)q;
+        }
     }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) split_grad_kernel(const GroupNormArgs a, const SplitShape sh,
+__global__ void __launch_bounds__(kThreads, 3) split_grad_kernel(const GroupNormArgs a, const SplitShape sh,
                                                               const float* __restrict__ group_sums) {
+    extern __shared__ uint4 smem[];
     const SplitPlace p = split_place<V>(a, sh, true);
-    if (!p.on) return;
-    const T* x = static_cast<const T*>(a.x) + p.n * a.S * a.ldx + p.c;
-    const T* dy = static_cast<const T*>(a.dy) + p.n * a.S * a.lddy + p.c;
-    T* dx = static_cast<T*>(a.dx) + p.n * a.S * a.lddx + p.c;
+    const uint32_t count = own_rows(p, sh);
+    if (!count) return;
+    const uint64_t last = p.n * a.S + p.row0 + p.rb + (uint64_t)(count - 1) * sh.RB;
+    const T* const from[2] = {static_cast<const T*>(a.x) + last * a.ldx + p.c,
+                              static_cast<const T*>(a.dy) + last * a.lddy + p.c};
+    const int64_t inc[2] = {-(int64_t)(sh.RB * a.ldx), -(int64_t)(sh.RB * a.lddy)};
+    T* dx = static_cast<T*>(a.dx) + last * a.lddx + p.c;
     const uint64_t i = p.n * a.G + p.g;
     const float inv = 1.f / ((float)a.S * (float)(a.C / a.G));
     const Vec<V> less = splat<V>(-a.mean[i]), rstd = splat<V>(a.rstd[i]);
     const Vec<V> s = splat<V>(-group_sums[2 * i] * inv), q = splat<V>(-group_sums[2 * i + 1] * inv);
     Vec<V> w, b;
     load_params<V>(a, p.c, true, w, b);
-    rows_backwards(p, sh, [&](uint64_t r) {
-        const Pack<T, V> px = load_pack<T, V>(x + r * a.ldx), pd = load_pack<T, V>(dy + r * a.lddy);
-        const Vec<V> h = mul(add(widen<T, V>(px), less), rstd);
-        const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pd));
-        store_pack_cs<T, V>(dx + r * a.lddx, narrow<T, V>(mul(rstd, fma(h, q, fma(d, w, s)))));
+    stream_rows<T, V, 2, kDepth2, 1>(smem, from, inc, count, [&](const auto& pk, uint32_t) {
+        const Vec<V> h = mul(add(widen<T, V>(pk[0][0]), less), rstd);
+        const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
+        store_pack_cs<T, V>(dx, narrow<T, V>(mul(rstd, fma(h, q, fma(d, w, s)))));
+        dx -= sh.RB * a.lddx;
     });
 }
 
@@ -751,10 +848,11 @@ RowsShape rows_shape(uint32_t C, uint32_t G, int V) {
     return sh;
 }
 
-// CTAs in x: as many as run at once (`per_sm`, which the ring's size allows).
-uint64_t rows_blocks(const RowsShape& sh, uint64_t N, uint32_t G, uint64_t per_sm) {
+// CTAs in x of the backward: four per SM, which run at once; each leaves one
+// row of sums for the parameters' gradients.
+uint64_t rows_blocks(const RowsShape& sh, uint64_t N, uint32_t G) {
     const uint64_t y = (G + sh.GB - 1) / sh.GB;
-    return std::max<uint64_t>(1, std::min((N + sh.RB - 1) / sh.RB, kSms * per_sm / std::min(kSms, y)));
+    return std::max<uint64_t>(1, std::min((N + sh.RB - 1) / sh.RB, kSms * 4 / std::min(kSms, y)));
 }
 
 // Chunks of a sample: eight CTAs per SM over all samples, which all run at
@@ -785,18 +883,16 @@ SplitShape split_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V) {
 
 uint32_t sub_slots(uint32_t C, uint32_t G) { return (C / G + kThreads - 1) / kThreads; }
 
-// Upper bounds over every vector width, so that the size does not depend on
-// the pointers' alignment.
-constexpr uint64_t kForwardPerSm = 6, kBackwardPerSm = 4;
-
 }  // namespace
 
+// Upper bounds over every vector width, so that the size does not depend on
+// the pointers' alignment.
 size_t group_norm_scratch_bytes(uint64_t N, uint64_t S, uint32_t C, uint32_t G, bool backward) {
     if (N == 0 || S == 0 || C == 0 || G == 0 || C % G) return 0;
     uint64_t rows = 0, chunks = 1;
     for (int V = 1; V <= 8; V <<= 1) {
         if ((C / G) % V) break;
-        if (rows_form(S, C / G, V)) rows = std::max(rows, rows_blocks(rows_shape(C, G, V), N, G, kBackwardPerSm));
+        if (rows_form(S, C / G, V)) rows = std::max(rows, rows_blocks(rows_shape(C, G, V), N, G));
         chunks = std::max<uint64_t>(chunks, split_shape(N, S, C, G, V).chunks);
     }
     if (!backward && rows_form(S, C / G, 1)) return 0;  // whichever width is picked
@@ -839,20 +935,35 @@ void check_norm(const GroupNormArgs& a, void* scratch, size_t scratch_bytes, boo
 template <typename T, int V, int J>
 void rows_launch(const GroupNormArgs& a, float* partial, bool backward, cudaStream_t s) {
     const RowsShape sh = rows_shape(a.C, a.G, V);
-    const dim3 grid((unsigned)rows_blocks(sh, a.N, a.G, backward ? kBackwardPerSm : kForwardPerSm), (a.G + sh.GB - 1) / sh.GB);
-    TCC_REQUIRE(grid.y <= 65535, "too many groups for one-row samples");
-    const void* kernel = backward ? (const void*)rows_backward_kernel<T, V, J> : (const void*)rows_forward_kernel<T, V, J>;
-    // where nothing is copied ahead, room for the sums alone
-    const size_t smem = std::max<size_t>(backward ? sizeof(RowsRing<T, V, J, 2>) : sizeof(RowsRing<T, V, J, 1>),
-                                         backward ? 2 * kThreads * V * sizeof(float) : 0);
-    // per-device attribute: set on every call (cheap), the current device may change
-    if (smem > 48 * 1024)
-        TCC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    if (backward) rows_backward_kernel<T, V, J><<<grid, kThreads, smem, s>>>(a, sh, partial);
-    else rows_forward_kernel<T, V, J><<<grid, kThreads, smem, s>>>(a, sh);
+    const uint32_t cols = (a.G + sh.GB - 1) / sh.GB;
+    TCC_REQUIRE(cols <= 65535, "too many groups for one-row samples");
+    dim3 grid(1, cols);
+    if (backward) {
+        using Ring = RowsRing<T, V, J, 2>;
+        grid.x = (unsigned)rows_blocks(sh, a.N, a.G);
+        // where nothing is copied ahead, room for the sums alone
+        const size_t smem = std::max<size_t>(Ring::kAsync ? sizeof(Ring) : 0, 2 * kThreads * V * sizeof(float));
+        // per-device attribute: set on every call (cheap), the current device may change
+        if (smem > 48 * 1024)
+            TCC_CUDA(cudaFuncSetAttribute(rows_backward_kernel<T, V, J>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)smem));
+        rows_backward_kernel<T, V, J><<<grid, kThreads, smem, s>>>(a, sh, partial);
+    } else {
+        using Ring = RowsRing<T, V, J, 1>;
+        // fewer rows a CTA where the ring's would leave SMs idle
+        const uint64_t row_passes = (a.N + sh.RB - 1) / sh.RB;
+        const uint32_t passes = (uint32_t)std::max<uint64_t>(
+            1, std::min<uint64_t>(Ring::D, row_passes * cols / (kSms * 4)));
+        grid.x = ceil_div(row_passes, passes);
+        const size_t smem = sizeof(Ring) + (a.mean ? 2 * passes * sh.RB * sh.GB * sizeof(float) : 0);
+        if (smem > 48 * 1024)
+            TCC_CUDA(cudaFuncSetAttribute(rows_forward_kernel<T, V, J>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)smem));
+        rows_forward_kernel<T, V, J><<<grid, kThreads, smem, s>>>(a, sh, passes);
+    }
     TCC_CUDA(cudaGetLastError());
     if (backward && partial) {
-        param_grad_kernel<<<(2 * a.C + 31) / 32, 1024, 0, s>>>(partial, grid.x, a.C, a.dweight, a.dbias,
+        param_grad_kernel<<<(2 * a.C + 7) / 8, 1024, 0, s>>>(partial, grid.x, a.C, a.dweight, a.dbias,
                                                               a.param_type);
         TCC_CUDA(cudaGetLastError());
     }
@@ -880,6 +991,7 @@ void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStrea
     const dim3 grid((unsigned)(a.N * sh.chunks), sh.cols);
     const unsigned groups = (unsigned)(a.N * a.G);
     const bool many = sh.chunks * sh.SUB > 64;  // partial results of a group
+    constexpr size_t ring1 = ring_bytes<T, V, 1>(), ring2 = ring_bytes<T, V, 2>();
     if (!backward) {
         Moments* partial = reinterpret_cast<Moments*>(scratch);
         float* mean = a.mean;
@@ -888,20 +1000,23 @@ void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStrea
             mean = reinterpret_cast<float*>(scratch + align256(a.N * sh.chunks * a.G * sh.SUB * sizeof(Moments)));
             rstd = mean + align256(a.N * a.G * 4) / 4;
         }
-        split_moments_kernel<T, V><<<grid, kThreads, 0, s>>>(a, sh, partial);
+        split_moments_kernel<T, V><<<grid, kThreads, ring1, s>>>(a, sh, partial);
         split_stats_kernel<<<groups, many ? kThreads : 32, 0, s>>>(partial, a.G, sh.SUB, sh.chunks, a.eps, mean, rstd);
-        split_apply_kernel<T, V><<<grid, kThreads, 0, s>>>(a, sh, mean, rstd);
+        split_apply_kernel<T, V><<<grid, kThreads, ring1, s>>>(a, sh, mean, rstd);
     } else {
         float* partial = reinterpret_cast<float*>(scratch);
         float* group_sums = partial + align256(a.N * sh.chunks * 2 * a.C * 4) / 4;
-        split_sums_kernel<T, V><<<grid, kThreads, 0, s>>>(a, sh, partial);
-        if (a.dx) {
-            split_groups_kernel<<<groups, dim3(32, many ? 32 : 4), 0, s>>>(a, partial, sh.chunks, group_sums);
-            split_grad_kernel<T, V><<<grid, kThreads, 0, s>>>(a, sh, group_sums);
+        split_sums_kernel<T, V><<<grid, kThreads, std::max(ring2, 2 * kThreads * V * sizeof(float)), s>>>(a, sh, partial);
+        const bool one = params && a.N == 1;  // one sample: its channels' sums are the parameters' gradients
+        if (a.dx || one) {
+            uint32_t cw = 1;
+            while (cw < 32 && cw < a.C / a.G) cw <<= 1;
+            split_groups_kernel<<<groups, many ? 1024 : 128, 0, s>>>(a, partial, sh.chunks, cw, group_sums, one);
         }
-        if (params)
-            param_grad_kernel<<<(2 * a.C + 31) / 32, 1024, 0, s>>>(partial, a.N * sh.chunks, a.C, a.dweight, a.dbias,
-                                                                  a.param_type);
+        if (a.dx) split_grad_kernel<T, V><<<grid, kThreads, ring2, s>>>(a, sh, group_sums);
+        if (params && !one)
+            param_grad_kernel<<<(2 * a.C + 7) / 8, 1024, 0, s>>>(partial, a.N * sh.chunks, a.C, a.dweight, a.dbias,
+                                                                a.param_type);
     }
     TCC_CUDA(cudaGetLastError());
 }
