@@ -19,8 +19,13 @@ namespace tcc {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kOneThreads = 1024;         // of the one CTA that clips few bytes
+constexpr uint64_t kOneBytes = 256 << 10;
 constexpr uint32_t kChunkBytes = 32768;  // of one tensor, for one CTA at a time
 constexpr uint32_t kMaxBlocks = 148 * 8;
+
+// Tensors of a launch over few of them, whose parameters are short, and of another.
+constexpr int kSmall = 32, kLarge = 480;
 
 // K tensors of one launch; chunk i of the launch belongs to the tensor t with
 // first[t] <= i < first[t + 1].
@@ -77,14 +82,15 @@ __device__ __forceinline__ double pack_squares(const Pack<T, V>& p) {
     return d;
 }
 
+template <int THREADS>
 __device__ __forceinline__ double block_sum(double v) {
-    __shared__ double ws[kThreads / 32];
+    __shared__ double ws[THREADS / 32];
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
     __syncthreads();
     double t = 0.0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) t += ws[i];
+    for (int i = 0; i < THREADS / 32; ++i) t += ws[i];
     __syncthreads();
     return t;
 }
@@ -95,7 +101,7 @@ __device__ __forceinline__ uint32_t head_of(const void* p, uint32_t n, uint32_t 
     return min(n, off ? (16 - off) / bytes : 0u);
 }
 
-template <typename T>
+template <typename T, int THREADS>
 __device__ __forceinline__ double span_squares(const Span& sp) {
     constexpr int V = 16 / sizeof(T);
     const T* p = static_cast<const T*>(sp.data);
@@ -103,11 +109,18 @@ __device__ __forceinline__ double span_squares(const Span& sp) {
     const uint32_t packs = (sp.n - head) / V, body = head + packs * V;
     double s = 0.0;
 #pragma unroll 4
-    for (uint32_t q = threadIdx.x; q < packs; q += kThreads)
+    for (uint32_t q = threadIdx.x; q < packs; q += THREADS)
         s += pack_squares<T, V>(load_pack<T, V>(p + head + (uint64_t)q * V));
     if (threadIdx.x < head) s += pack_squares<T, 1>(load_pack<T, 1>(p + threadIdx.x));
     if (body + threadIdx.x < sp.n) s += pack_squares<T, 1>(load_pack<T, 1>(p + body + threadIdx.x));
     return s;
+}
+
+template <int THREADS>
+__device__ __forceinline__ double squares_of(const Span& sp) {
+    if (sp.type == TCC_F32) return span_squares<float, THREADS>(sp);
+    if (sp.type == TCC_F16) return span_squares<__half, THREADS>(sp);
+    return span_squares<__nv_bfloat16, THREADS>(sp);
 }
 
 template <int K>
@@ -117,18 +130,16 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
     const uint32_t chunks = t.first[t.count];
     for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
         const Span sp = chunk_span<K>(t, c);
-        if (sp.type == TCC_F32) s += span_squares<float>(sp);
-        else if (sp.type == TCC_F16) s += span_squares<__half>(sp);
-        else s += span_squares<__nv_bfloat16>(sp);
+        s += squares_of<kThreads>(sp);
     }
-    s = block_sum(s);
+    s = block_sum<kThreads>(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = add ? partial[blockIdx.x] + s : s;
 }
 
 __device__ __forceinline__ float norm_of(const double* __restrict__ partial, uint32_t blocks) {
     double s = 0.0;
     for (uint32_t i = threadIdx.x; i < blocks; i += kThreads) s += partial[i];
-    return (float)sqrt(block_sum(s));
+    return (float)sqrt(block_sum<kThreads>(s));
 }
 
 __global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ partial, uint32_t blocks,
@@ -137,14 +148,14 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict
     if (threadIdx.x == 0) *norm = n;
 }
 
-template <typename T>
+template <typename T, int THREADS>
 __device__ __forceinline__ void span_scale(const Span& sp, float f) {
     constexpr int V = 16 / sizeof(T);
     T* p = static_cast<T*>(sp.data);
     const uint32_t head = head_of(p, sp.n, sizeof(T));
     const uint32_t packs = (sp.n - head) / V, body = head + packs * V;
 #pragma unroll 4
-    for (uint32_t q = threadIdx.x; q < packs; q += kThreads) {
+    for (uint32_t q = threadIdx.x; q < packs; q += THREADS) {
         Pack<T, V> v = load_pack<T, V>(p + head + (uint64_t)q * V);
 #pragma unroll
         for (int k = 0; k < V; ++k) v.v[k] = from_f32<T>(to_f32(v.v[k]) * f);
@@ -155,6 +166,13 @@ __device__ __forceinline__ void span_scale(const Span& sp, float f) {
         T* e = p + body + threadIdx.x;
         *e = from_f32<T>(to_f32(*e) * f);
     }
+}
+
+template <int THREADS>
+__device__ __forceinline__ void scale_by(const Span& sp, float f) {
+    if (sp.type == TCC_F32) span_scale<float, THREADS>(sp, f);
+    else if (sp.type == TCC_F16) span_scale<__half, THREADS>(sp, f);
+    else span_scale<__nv_bfloat16, THREADS>(sp, f);
 }
 
 // Scales in the reverse of the order in which the norm was read: what was read
@@ -172,10 +190,21 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
     const uint32_t chunks = t.first[t.count];
     for (uint32_t i = blockIdx.x; i < chunks; i += gridDim.x) {
         const Span sp = chunk_span<K>(t, chunks - 1 - i);
-        if (sp.type == TCC_F32) span_scale<float>(sp, f);
-        else if (sp.type == TCC_F16) span_scale<__half>(sp, f);
-        else span_scale<__nv_bfloat16>(sp, f);
+        scale_by<kThreads>(sp, f);
     }
+}
+
+// Norm and clipping of few bytes by one CTA: one launch in place of two, and
+// the second reading comes from the SM's own cache.
+__global__ void __launch_bounds__(kOneThreads) clip_one_kernel(const __grid_constant__ TensorTable<kSmall> t,
+                                                               float* norm_out, float max_norm, float eps) {
+    double s = 0.0;
+    const uint32_t chunks = t.first[t.count];
+    for (uint32_t c = 0; c < chunks; ++c) s += squares_of<kOneThreads>(chunk_span<kSmall>(t, c));
+    const float norm = (float)sqrt(block_sum<kOneThreads>(s)), f = max_norm / (norm + eps);
+    if (threadIdx.x == 0) *norm_out = norm;
+    if (f >= 1.f) return;
+    for (uint32_t c = 0; c < chunks; ++c) scale_by<kOneThreads>(chunk_span<kSmall>(t, c), f);
 }
 
 // Fills a table from the tensors at `at` on (empty ones are skipped); returns
@@ -221,10 +250,7 @@ void check_tensors(const tcc_tensor* t, uint32_t count, bool written) {
         TCC_REQUIRE(spans[i - 1].second <= spans[i].first, "two tensors share memory");
 }
 
-constexpr int kSmall = 32, kLarge = 480;
-
-// fn(table) for each launch's tensors; the small table keeps the parameters of
-// a launch over a few tensors short.
+// fn(table) for each launch's tensors.
 template <typename Fn>
 void each_launch(const tcc_tensor* t, uint32_t count, Fn&& fn) {
     if (count <= (uint32_t)kSmall) {
@@ -313,6 +339,15 @@ void clip_grad_norm(const tcc_tensor* t, uint32_t count, float max_norm, float e
     check_clip(max_norm, eps);
     TCC_REQUIRE(norm, "norm must not be NULL");
     double* partial = partials(scratch, scratch_bytes);
+    uint64_t bytes = 0;
+    for (uint32_t i = 0; i < count; ++i) bytes += t[i].n * type_bytes(t[i].type);
+    if (count <= (uint32_t)kSmall && bytes && bytes <= kOneBytes) {
+        TensorTable<kSmall> tab;
+        fill<kSmall>(t, count, 0, tab);
+        clip_one_kernel<<<1, kOneThreads, 0, s>>>(tab, norm, max_norm, eps);
+        TCC_CUDA(cudaGetLastError());
+        return;
+    }
     const uint32_t blocks = squares(t, count, partial, s);
     if (blocks == 0) {  // no elements: the norm is 0
         TCC_CUDA(cudaMemsetAsync(norm, 0, sizeof(float), s));
