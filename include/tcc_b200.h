@@ -351,6 +351,10 @@ typedef struct tcc_tensor {
     int32_t type;
     int32_t reserved;
 } tcc_tensor;
+/* tcc_clip_grad_norm takes a NULL scratch for at most this many bytes in at most
+ * this many tensors (one launch then does both). */
+#define TCC_CLIP_SMALL_BYTES (192u << 10)
+#define TCC_CLIP_SMALL_TENSORS 32
 size_t tcc_grad_norm_scratch_bytes(void);
 tcc_status tcc_grad_norm(const tcc_tensor* tensors, uint32_t count, float* norm, void* scratch,
                          size_t scratch_bytes, cudaStream_t stream);

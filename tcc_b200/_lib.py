@@ -111,6 +111,7 @@ F32, F16, BF16 = 0, 1, 2        # TCC_F32, TCC_F16, TCC_BF16
 I32, I64 = 0, 1                 # TCC_I32, TCC_I64
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}  # TCC_ACT_*
 NO_PADDING = -(1 << 63)         # TCC_NO_PADDING
+CLIP_SMALL_BYTES, CLIP_SMALL_TENSORS = 192 << 10, 32  # TCC_CLIP_SMALL_*
 
 
 class Tensor(C.Structure):

@@ -104,7 +104,8 @@ def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6, error_if_non
     if count == 0:
         return torch.zeros(())
     norm = torch.empty((), dtype=torch.float32, device=device)
-    nbytes = _scratch_bytes()
+    small = count <= L.CLIP_SMALL_TENSORS and sum(g.nbytes for g in grads) <= L.CLIP_SMALL_BYTES
+    nbytes = 0 if small else _scratch_bytes()
     hold, scratch = scratch_for(nbytes, device)
     launch(device, "tcc_clip_grad_norm", words.buffer_info()[0], count, max_norm, eps, norm.data_ptr(), scratch,
            nbytes)

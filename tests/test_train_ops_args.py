@@ -90,10 +90,11 @@ def test_clip_refusals(lib):
     assert clip_call([one, (P + 396, 10, L.F32)]) == 1 and b"share memory" in lib.tcc_last_error()
     assert clip_call([(P + 396, 10, L.F32), one]) == 1
     assert clip_call([one, one]) == 1
+    large = (P, 1 << 20, L.F32)
     for kw in (dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(eps=-1.0), dict(out=None), dict(scratch=None),
                dict(scratch=P + 8)):
-        assert clip_call([one], **kw) == 1, kw
-    assert clip_call([one], nbytes=8) == 6
+        assert clip_call([large], **kw) == 1, kw
+    assert clip_call([large], nbytes=8) == 6
     assert lib.tcc_clip_grad_norm(None, 2, 1.0, 1e-6, P, P, 1 << 20, None) == 1
     p, n, keep = table(one)
     assert lib.tcc_grad_norm(p, n, None, P, 1 << 20, None) == 1
