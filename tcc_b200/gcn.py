@@ -22,6 +22,7 @@ import torch
 
 from . import spmm_cnic
 from . import tiles as T
+from .norm import GroupNorm, group_norm
 
 CooData = namedtuple("CooData", ["f_row_indices", "f_col_indices",
                                  "s_row_indices", "s_col_indices"])
@@ -154,6 +155,16 @@ def relu_dropout(x: torch.Tensor, p: float, seed: int, training: bool = True) ->
     return ReluDropout.apply(x, p, seed)
 
 
+def hidden_activation(x: torch.Tensor, p: float, seed: int, training: bool = True,
+                      norm: GroupNorm | None = None) -> torch.Tensor:
+    """relu_dropout(norm(x)); without dropout the relu is part of the norm's pass."""
+    if norm is None:
+        return relu_dropout(x, p, seed, training)
+    if not training or p == 0.0:
+        return group_norm(x, norm.num_groups, norm.weight, norm.bias, norm.eps, "relu")
+    return relu_dropout(norm(x), p, seed)
+
+
 # ------------------------------------------------------------- TiledGraph --
 
 class TiledGraph:
@@ -230,11 +241,13 @@ class GCNConv(torch.nn.Module):
 
 
 class GCN(torch.nn.Module):
-    """Two-layer GCN of train/tcgnn_conv_release.py:196-268."""
+    """Two-layer GCN of train/tcgnn_conv_release.py:196-268; norm_groups > 0 puts a
+    group norm of every node's hidden features before the activation."""
 
-    def __init__(self, num_features, hidden_dim, num_classes, dropout=0.5, seed=0):
+    def __init__(self, num_features, hidden_dim, num_classes, dropout=0.5, seed=0, norm_groups=0):
         super().__init__()
         self.conv1 = GCNConv(num_features, hidden_dim, first_layer=True)
+        self.norm = GroupNorm(norm_groups, hidden_dim) if norm_groups else None
         self.conv_final = GCNConv(hidden_dim, num_classes)
         self.p = dropout
         self._seed = seed
@@ -243,6 +256,6 @@ class GCN(torch.nn.Module):
     def forward(self, graph: TiledGraph, x):
         # relu + dropout in one pass; a fresh dropout draw per call
         self._calls += 1
-        h = relu_dropout(self.conv1(graph, x), self.p, self._seed * 1_000_003 + self._calls,
-                         self.training)
+        h = hidden_activation(self.conv1(graph, x), self.p, self._seed * 1_000_003 + self._calls,
+                              self.training, self.norm)
         return self.conv_final(graph, h)

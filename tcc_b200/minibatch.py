@@ -16,6 +16,8 @@ module provides those inputs from a CSR on the GPU:
   "degree" split sends edges whose source has at least ``hub_degree`` edges
   in the block through the BCSC push pass and the rest through the BCSR pull
   pass (the two parts the reference's mixed op adds into one output);
+* ``embedding_rows`` -- the first block's input rows from a learned node
+  embedding, for graphs without node features;
 * ``sparse_inputs`` -- SparseMatrixSize / SparseMatrixData / CooData for a
   two-layer model (``s_*`` = first block, ``f_*`` = last block), plus the
   batch's hot/cold feature maps (``batch_feature_maps``).
@@ -30,6 +32,7 @@ import torch
 
 from . import gcn
 from . import tiles as T
+from .embedding import embedding
 
 
 # ------------------------------------------------------------- files --
@@ -203,3 +206,10 @@ def batch_feature_maps(store, input_ids: torch.Tensor):
     local source column) from a FeatureStore over all nodes."""
     idx = input_ids.to(torch.int64)
     return store.cache_search_map[idx].contiguous(), store.id_map[idx].contiguous()
+
+
+def embedding_rows(table: torch.Tensor, block: Block, scale: float = 1.0) -> torch.Tensor:
+    """Input rows [num_src, F] of a block from a learned node-embedding table (float32, as the
+    aggregation takes them, whatever the table's type; F a multiple of 4 for it), differentiable
+    in the table.  Source ids of -1 (a block filled up to a fixed size) give zero rows."""
+    return embedding(table, block.src_ids, scale, padding_idx=-1, out_dtype=torch.float32)

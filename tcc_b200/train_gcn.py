@@ -31,7 +31,8 @@ transforms first, Â·(H1·W2), so both of its SpMMs run 48 wide instead of 256
 (``transform_first``; None picks by width, ``--aggregate-first`` keeps the
 reference's order for every layer).  ``--save`` / ``--resume`` write and read a
 checkpoint of the weights, the Adam state and the epoch count (the reference
-saves none).
+saves none).  ``--norm-groups`` normalises the hidden features (group norm per
+node) and ``--clip-norm`` clips the summed gradients; the reference does neither.
 
 Run: ``python -m tcc_b200.train_gcn`` (1 GPU) or under torch.distributed.run.
 """
@@ -50,8 +51,10 @@ import torch.distributed as dist
 
 from . import graphs as G
 from . import tiles as T
+from .clip import clip_grad_norm_
 from .feature_store import FeatureStore
-from .gcn import relu_dropout
+from .gcn import hidden_activation
+from .norm import GroupNorm
 from .partition import DistGraph, balanced_bounds, nccl_options, tile_balanced_bounds
 
 
@@ -146,6 +149,10 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
     W1.requires_grad_(True)
     W2.requires_grad_(True)
     params = [W1, W2]
+    norm = None
+    if cfg.get("norm_groups"):
+        norm = GroupNorm(cfg["norm_groups"], cfg["hidden"], device=device)
+        params += [norm.weight, norm.bias]
     opt = torch.optim.Adam(params, lr=cfg["lr"])
     start_epoch = 0
     if cfg.get("resume"):
@@ -153,6 +160,8 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
         with torch.no_grad():
             W1.copy_(ck["W1"])
             W2.copy_(ck["W2"])
+            if norm is not None:
+                norm.load_state_dict(ck["norm"])
         opt.load_state_dict(ck["opt"])
         start_epoch = int(ck["epoch"])
     # cold rows: streamed into an HBM staging buffer once per epoch on a side
@@ -206,8 +215,8 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
                 ready.record(side)
         else:
             Z1 = _store_aggregate(R["tiles_g"], store, R["rs"])
-        # relu + dropout fused (one pass; the backward reads only H1)
-        H1 = relu_dropout(Z1 @ W1, cfg["dropout"], drop_seed + epoch_no[0])
+        # relu + dropout fused (one pass; the backward reads only H1), after the norm if there is one
+        H1 = hidden_activation(Z1 @ W1, cfg["dropout"], drop_seed + epoch_no[0], norm=norm)
         epoch_no[0] += 1
         if transform_first:
             P = torch.nn.functional.pad(H1 @ W2, (0, cls_pad - cfg["classes"]))
@@ -224,6 +233,8 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
         for p in params:
             p.grad.copy_(flat[off:off + p.numel()].view_as(p))
             off += p.numel()
+        if cfg.get("clip_norm") is not None:  # summed gradients: the same on every rank
+            clip_grad_norm_(params, cfg["clip_norm"])
         opt.step()
         lt = loss.detach().clone()
         if world > 1:
@@ -249,6 +260,7 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
         side.synchronize()
     if cfg.get("save") and rank == 0:  # weights are identical on every rank
         torch.save({"W1": W1.detach(), "W2": W2.detach(), "opt": opt.state_dict(),
+                    **({} if norm is None else {"norm": norm.state_dict()}),
                     "epoch": cfg["epochs"], "config": {k: v for k, v in cfg.items()
                                                        if k not in ("save", "resume")}},
                    cfg["save"])
@@ -296,6 +308,10 @@ def main(argv=None):
     p.add_argument("--partition", choices=["tiles", "nnz"], default="tiles",
                    help="N > 1: cut the rows into parts of equal pull work (tiles) or equal "
                         "nonzeros")
+    p.add_argument("--norm-groups", type=int, default=0,
+                   help="group norm of every node's hidden features, in this many groups (0: none)")
+    p.add_argument("--clip-norm", type=float, default=None,
+                   help="clip the gradients to this global norm before the optimiser's step")
     p.add_argument("--save", default=None, help="checkpoint path written at the end (rank 0)")
     p.add_argument("--resume", default=None, help="checkpoint to continue from")
     a = p.parse_args(argv)
@@ -313,6 +329,7 @@ def main(argv=None):
         cfg["save"], cfg["resume"] = a.save, a.resume
         cfg["cold_staging"] = not a.cold_zero_copy
         cfg["partition"] = a.partition
+        cfg["norm_groups"], cfg["clip_norm"] = a.norm_groups, a.clip_norm
         tf = {"transform": True, "aggregate": False}.get(a.order)
         r = train(cfg, device, world, rank, tf)
         if rank == 0:
@@ -333,6 +350,7 @@ def main(argv=None):
                                               else "zero-copy reads of pinned host memory"),
                            "halo_transport": r["transport"],
                            "partition": cfg["partition"] if world > 1 else None,
+                           "norm_groups": cfg["norm_groups"], "clip_norm": cfg["clip_norm"],
                            "halo_rows_total": int(r["halo_rows"]), "transform_first": r["transform_first"],
                            "order": "layer 1 from the hot/cold store, layer 2 over the row partition"}}),
                   flush=True)
