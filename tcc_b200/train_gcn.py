@@ -52,6 +52,7 @@ import torch.distributed as dist
 from . import graphs as G
 from . import tiles as T
 from .clip import clip_grad_norm_
+from .embedding import embedding
 from .feature_store import FeatureStore
 from .gcn import hidden_activation
 from .norm import GroupNorm
@@ -220,10 +221,12 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
         epoch_no[0] += 1
         if transform_first:
             P = torch.nn.functional.pad(H1 @ W2, (0, cls_pad - cfg["classes"]))
-            logits = _DistAggregate.apply(R["dg"], P)[:, :cfg["classes"]]
+            scores = _DistAggregate.apply(R["dg"], P)
         else:
-            logits = _DistAggregate.apply(R["dg"], H1) @ W2
-        loss = torch.nn.functional.cross_entropy(logits[R["lab_idx"]], R["lab_y"],
+            scores = _DistAggregate.apply(R["dg"], H1) @ W2
+        # the labelled rows first, then without the columns that fill them up
+        logits = embedding(scores, R["lab_idx"])[:, :cfg["classes"]]
+        loss = torch.nn.functional.cross_entropy(logits, R["lab_y"],
                                                  reduction="sum") / R["n_lab"]
         loss.backward()
         flat = torch.cat([p.grad.reshape(-1) for p in params])
