@@ -13,16 +13,21 @@
 // the difference of two large sums: moments of small blocks, each around its
 // own mean, are merged pairwise (Chan, Golub and LeVeque, 1979).
 //
-// Two forms:
+// Three forms:
 //  * rows  (S = 1, a group within a warp): every group of a row is reduced by
 //    a few lanes of one warp, x is read once; the next rows are on their way
 //    into a ring in shared memory meanwhile.
+//  * resident (a sample that fits the shared memory of at most eight SMs): a
+//    cluster of CTAs holds a sample, x (and dy) are read once, the CTAs exchange
+//    their moments or sums through distributed shared memory.
 //  * split (any other): the rows of a sample are cut into chunks, a CTA each;
 //    moments (or channel sums) per chunk, a merge over the chunks, and a
 //    second pass that normalises, walking each chunk from its end, so that what
 //    the first pass read last is still in L2.
 #include "elem.cuh"
 #include "train_ops.cuh"
+
+#include <cooperative_groups.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -686,32 +691,29 @@ constexpr size_t ring_bytes() {
     return (A == 1 ? kDepth1 : kDepth2) * A * kThreads * sizeof(Pack<T, V>);
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, 3) split_moments_kernel(const GroupNormArgs a, const SplitShape sh,
-                                                                 Moments* __restrict__ partial) {
-    extern __shared__ uint4 smem[];
-    const SplitPlace p = split_place<V>(a, sh, false);
-    const T* const from[1] = {static_cast<const T*>(a.x) + (p.n * a.S + p.row0 + p.rb) * a.ldx + p.c};
-    const int64_t inc[1] = {(int64_t)(sh.RB * a.ldx)};
-    Moments m{0.f, 0.f, 0.f};
-    stream_rows<T, V, 1, kDepth1, kBlockRows>(smem, from, inc, own_rows(p, sh), [&](const auto& pk, uint32_t rows) {
-        Vec<V> v[kBlockRows], t = splat<V>(0.f);
+// Moments of a thread's block of up to kBlockRows rows, around the block's own mean.
+template <typename T, int V, typename Packs>
+__device__ __forceinline__ Moments block_of(const Packs& pk, uint32_t rows) {
+    Vec<V> v[kBlockRows], t = splat<V>(0.f);
 #pragma unroll
-        for (uint32_t u = 0; u < kBlockRows; ++u) {
-            v[u] = u < rows ? widen<T, V>(pk[u][0]) : splat<V>(0.f);
-            t = add(t, v[u]);
+    for (uint32_t u = 0; u < kBlockRows; ++u) {
+        v[u] = u < rows ? widen<T, V>(pk[u][0]) : splat<V>(0.f);
+        t = add(t, v[u]);
+    }
+    const float n = (float)(rows * V), mean = __fdividef(sum(t), n);
+    t = splat<V>(0.f);
+#pragma unroll
+    for (uint32_t u = 0; u < kBlockRows; ++u)
+        if (u < rows) {
+            const Vec<V> e = add(v[u], splat<V>(-mean));
+            t = fma(e, e, t);
         }
-        const float n = (float)(rows * V), mean = __fdividef(sum(t), n);
-        t = splat<V>(0.f);
-#pragma unroll
-        for (uint32_t u = 0; u < kBlockRows; ++u)
-            if (u < rows) {
-                const Vec<V> e = add(v[u], splat<V>(-mean));
-                t = fma(e, e, t);
-            }
-        m = merge(m, Moments{n, mean, sum(t)});
-    });
-    __shared__ Moments sm[kThreads];
+    return Moments{n, mean, sum(t)};
+}
+
+// The threads' moments merged per group part: at sm[thread] of its first pack, row 0.
+__device__ __forceinline__ void block_moments(const SplitPlace& p, const SplitShape& sh, const Moments& m,
+                                              Moments* sm) {
     sm[threadIdx.x] = m;
     __syncthreads();
     for (uint32_t h = sh.RB; h > 1;) {  // over the rows of the block
@@ -728,6 +730,21 @@ __global__ void __launch_bounds__(kThreads, 3) split_moments_kernel(const GroupN
         h = half;
         __syncthreads();
     }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads, 3) split_moments_kernel(const GroupNormArgs a, const SplitShape sh,
+                                                                 Moments* __restrict__ partial) {
+    extern __shared__ uint4 smem[];
+    const SplitPlace p = split_place<V>(a, sh, false);
+    const T* const from[1] = {static_cast<const T*>(a.x) + (p.n * a.S + p.row0 + p.rb) * a.ldx + p.c};
+    const int64_t inc[1] = {(int64_t)(sh.RB * a.ldx)};
+    Moments m{0.f, 0.f, 0.f};
+    stream_rows<T, V, 1, kDepth1, kBlockRows>(smem, from, inc, own_rows(p, sh), [&](const auto& pk, uint32_t rows) {
+        m = merge(m, block_of<T, V>(pk, rows));
+    });
+    __shared__ Moments sm[kThreads];
+    block_moments(p, sh, m, sm);
     if (p.on && p.rb == 0 && p.gi == 0)
         partial[(p.n * sh.chunks + p.chunk) * ((uint64_t)a.G * sh.SUB) + p.slot] = sm[threadIdx.x];
 }
@@ -909,6 +926,183 @@ __global__ void __launch_bounds__(kThreads, 3) split_grad_kernel(const GroupNorm
     });
 }
 
+// --------------------------------------------------------- resident form --
+
+namespace cg = cooperative_groups;
+
+// A cluster of sh.chunks CTAs holds a sample, a chunk each; all of a row's
+// packs are in one block (sh.cols = 1).  A thread keeps its packs of its rows
+// at store[(k * A + array) * kThreads] and reads back only what it copied.
+constexpr uint32_t kMaxCluster = 8;
+
+template <typename T, int V, int A>
+__device__ __forceinline__ void fetch_resident(Pack<T, V>* store, const T* const (&from)[A],
+                                               const uint64_t (&step)[A], uint32_t count) {
+    for (uint32_t k = 0; k < count; ++k)
+#pragma unroll
+        for (int i = 0; i < A; ++i) {
+            const T* at = from[i] + k * step[i];
+            if constexpr (sizeof(Pack<T, V>) >= 4) copy_pack_async<T, V>(store + (k * A + i) * kThreads, at);
+            else store[(k * A + i) * kThreads] = load_pack<T, V>(at);
+        }
+    commit_copies();
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) resident_forward_kernel(const GroupNormArgs a, const SplitShape sh) {
+    extern __shared__ uint4 smem[];
+    __shared__ Moments sm[kThreads];
+    __shared__ Moments group[kThreads];  // of this CTA's chunk; G <= kThreads
+    __shared__ float2 stats[kThreads];   // mean and rstd of the sample's groups
+    cg::cluster_group cluster = cg::this_cluster();
+    const SplitPlace p = split_place<V>(a, sh, false);
+    const uint32_t count = own_rows(p, sh);
+    Pack<T, V>* store = reinterpret_cast<Pack<T, V>*>(smem) + threadIdx.x;
+    const uint64_t first = p.n * a.S + p.row0 + p.rb;
+    const T* const from[1] = {static_cast<const T*>(a.x) + first * a.ldx + p.c};
+    const uint64_t step[1] = {sh.RB * a.ldx};
+    fetch_resident<T, V, 1>(store, from, step, count);
+    Vec<V> w, b;
+    load_params<V>(a, p.c, p.on, w, b);
+    wait_copies<0>();
+    Moments m{0.f, 0.f, 0.f};
+    for (uint32_t k = 0; k < count; k += kBlockRows) {
+        Pack<T, V> pk[kBlockRows][1];
+        const uint32_t rows = min((uint32_t)kBlockRows, count - k);
+#pragma unroll
+        for (uint32_t u = 0; u < kBlockRows; ++u)
+            if (u < rows) pk[u][0] = load_pack<T, V>(store[(k + u) * kThreads].v);
+        m = merge(m, block_of<T, V>(pk, rows));
+    }
+    block_moments(p, sh, m, sm);
+    if (p.on && p.rb == 0 && p.gi == 0) group[p.g] = sm[threadIdx.x];
+    cluster.sync();
+    if (threadIdx.x < a.G) {
+        Moments t = *cluster.map_shared_rank(group + threadIdx.x, 0);
+        for (uint32_t r = 1; r < sh.chunks; ++r) t = merge(t, *cluster.map_shared_rank(group + threadIdx.x, r));
+        const float rstd = inverse_root(t.m2 / t.n + a.eps);
+        stats[threadIdx.x] = make_float2(t.mean, rstd);
+        if (a.mean && p.chunk == 0) {
+            a.mean[p.n * a.G + threadIdx.x] = t.mean;
+            a.rstd[p.n * a.G + threadIdx.x] = rstd;
+        }
+    }
+    cluster.sync();  // stats are written, and nobody reads this CTA's moments any more
+    if (!count) return;
+    T* y = static_cast<T*>(a.y) + first * a.ldy + p.c;
+    const Vec<V> less = splat<V>(-stats[p.g].x), rstd = splat<V>(stats[p.g].y);
+    for (uint32_t k = 0; k < count; ++k) {
+        const Vec<V> h = mul(add(widen<T, V>(load_pack<T, V>(store[k * kThreads].v)), less), rstd);
+        store_pack_cs<T, V>(y, narrow<T, V>(activate<V>(a.act, fma(h, w, b))));
+        y += sh.RB * a.ldy;
+    }
+}
+
+// A cluster takes every (grid / chunks)-th sample and keeps the sums for the
+// parameters' gradients: one row of partial [grid][2][C] per CTA, or NULL.
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) resident_backward_kernel(const GroupNormArgs a, const SplitShape sh,
+                                                                     float* __restrict__ partial) {
+    extern __shared__ uint4 smem[];
+    __shared__ float sums[2][kThreads * V];  // per thread, then per channel
+    __shared__ float2 group[kThreads];       // of this CTA's chunk
+    __shared__ float2 total[kThreads];       // of the sample
+    cg::cluster_group cluster = cg::this_cluster();
+    SplitPlace p = split_place<V>(a, sh, false);
+    const uint32_t count = own_rows(p, sh);
+    Pack<T, V>* store = reinterpret_cast<Pack<T, V>*>(smem) + threadIdx.x;
+    const uint64_t step[2] = {sh.RB * a.ldx, sh.RB * a.lddy};
+    const uint32_t Cg = a.C / a.G, lane = threadIdx.x & 31;
+    const float inv = 1.f / ((float)a.S * (float)Cg);
+    Vec<V> w, b, all_dw = splat<V>(0.f), all_db = all_dw;
+    load_params<V>(a, p.c, p.on, w, b);
+    // over the rows of threads: channel c at its first thread's place
+    auto over_rows = [&](const Vec<V>& dw, const Vec<V>& db, auto&& use) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            sums[0][threadIdx.x * V + k] = dw.v[k];
+            sums[1][threadIdx.x * V + k] = db.v[k];
+        }
+        __syncthreads();
+        if (p.on && p.rb == 0) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                float tw = 0.f, tb = 0.f;
+                for (uint32_t i = 0; i < sh.RB; ++i) {
+                    tw += sums[0][(threadIdx.x + i * sh.TX) * V + k];
+                    tb += sums[1][(threadIdx.x + i * sh.TX) * V + k];
+                }
+                use(k, tw, tb);
+            }
+        }
+    };
+    for (; p.n < a.N; p.n += gridDim.x / sh.chunks) {  // the same for the whole cluster
+        const uint64_t first = p.n * a.S + p.row0 + p.rb;
+        const T* const from[2] = {static_cast<const T*>(a.x) + first * a.ldx + p.c,
+                                  static_cast<const T*>(a.dy) + first * a.lddy + p.c};
+        fetch_resident<T, V, 2>(store, from, step, count);
+        const Vec<V> less = splat<V>(p.on ? -a.mean[p.n * a.G + p.g] : 0.f);
+        const Vec<V> rstd = splat<V>(p.on ? a.rstd[p.n * a.G + p.g] : 0.f);
+        auto row = [&](uint32_t k, Vec<V>& h, Vec<V>& d) {
+            h = mul(add(widen<T, V>(load_pack<T, V>(store[(2 * k) * kThreads].v)), less), rstd);
+            d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(load_pack<T, V>(store[(2 * k + 1) * kThreads].v)));
+        };
+        wait_copies<0>();
+        Vec<V> dw = splat<V>(0.f), db = dw;
+        for (uint32_t k = 0; k < count; ++k) {
+            Vec<V> h, d;
+            row(k, h, d);
+            db = add(db, d);
+            dw = fma(d, h, dw);
+        }
+        all_dw = add(all_dw, dw);
+        all_db = add(all_db, db);
+        if (!a.dx) continue;
+        over_rows(dw, db, [&](int k, float tw, float tb) {
+            sums[0][threadIdx.x * V + k] = tw * w.v[k];
+            sums[1][threadIdx.x * V + k] = tb * w.v[k];
+        });
+        __syncthreads();
+        for (uint32_t g = threadIdx.x >> 5; g < a.G; g += kThreads / 32) {
+            float q = 0.f, t = 0.f;
+            for (uint32_t k = lane; k < Cg; k += 32) {
+                q += sums[0][g * Cg + k];
+                t += sums[1][g * Cg + k];
+            }
+            q = lane_sum(q, 32);
+            t = lane_sum(t, 32);
+            if (lane == 0) group[g] = make_float2(t, q);
+        }
+        cluster.sync();
+        if (threadIdx.x < a.G) {
+            float2 t = make_float2(0.f, 0.f);
+            for (uint32_t i = 0; i < sh.chunks; ++i) {
+                const float2 o = *cluster.map_shared_rank(group + threadIdx.x, i);
+                t.x += o.x;
+                t.y += o.y;
+            }
+            total[threadIdx.x] = t;
+        }
+        cluster.sync();  // totals are written, and nobody reads this CTA's sums any more
+        if (!count) continue;
+        T* dx = static_cast<T*>(a.dx) + first * a.lddx + p.c;
+        const Vec<V> s = splat<V>(-total[p.g].x * inv), q = splat<V>(-total[p.g].y * inv);
+        for (uint32_t k = 0; k < count; ++k) {
+            Vec<V> h, d;
+            row(k, h, d);
+            store_pack_cs<T, V>(dx, narrow<T, V>(mul(rstd, fma(h, q, fma(d, w, s)))));
+            dx += sh.RB * a.lddx;
+        }
+    }
+    if (!partial) return;
+    __syncthreads();
+    float* out = partial + (uint64_t)blockIdx.x * 2 * a.C + p.c;
+    over_rows(all_dw, all_db, [&](int k, float tw, float tb) {
+        out[k] = tw;
+        out[a.C + k] = tb;
+    });
+}
+
 // ------------------------------------------------------------------ host --
 
 uint64_t align256(uint64_t b) { return (b + 255) / 256 * 256; }
@@ -977,24 +1171,61 @@ SplitShape split_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V) {
     return sh;
 }
 
-uint32_t sub_slots(uint32_t C, uint32_t G) { return (C / G + kThreads - 1) / kThreads; }
+// The resident form's cluster, or chunks = 0 where a sample does not fit: two
+// CTAs per SM; more CTAs than it needs while the GPU has room for them and a
+// thread has rows left to share.
+constexpr size_t kResidentBytes = 88 << 10;
+
+SplitShape resident_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V, uint32_t pack_bytes, int arrays) {
+    SplitShape sh{};
+    if (C / V > (uint32_t)kThreads || G > (uint32_t)kThreads || N >= (1ull << 27)) return sh;
+    SplitShape r;
+    r.PG = C / G / V;
+    r.GPB = G;
+    r.TX = C / V;
+    r.RB = kThreads / r.TX;
+    r.SUB = 1;
+    r.cols = 1;
+    for (uint32_t k = 1; k <= kMaxCluster; k <<= 1) {
+        r.chunk_rows = (S + k - 1) / k;
+        r.chunks = k;
+        const uint64_t deep = (r.chunk_rows + r.RB - 1) / r.RB;
+        if (deep * kThreads * pack_bytes * arrays > kResidentBytes) continue;
+        sh = r;
+        if (N * k >= 2 * kSms || deep <= 8) break;
+    }
+    return sh;
+}
+// Clusters of the backward: a cluster of one CTA goes on with another sample.
+uint64_t resident_grid(uint64_t N, uint32_t chunks) { return (chunks > 1 ? N : std::min(N, kSms * 8)) * chunks; }
+size_t resident_bytes(const SplitShape& sh, uint32_t pack_bytes, int arrays) {
+    return (sh.chunk_rows + sh.RB - 1) / sh.RB * kThreads * pack_bytes * arrays;
+}
 
 }  // namespace
 
-// Upper bounds over every vector width, so that the size does not depend on
-// the pointers' alignment.
+// The most that any vector width and element type would take, so that the
+// size depends neither on the type nor on the pointers' alignment.
 size_t group_norm_scratch_bytes(uint64_t N, uint64_t S, uint32_t C, uint32_t G, bool backward) {
     if (N == 0 || S == 0 || C == 0 || G == 0 || C % G) return 0;
-    uint64_t rows = 0, chunks = 1;
-    for (int V = 1; V <= 8; V <<= 1) {
-        if ((C / G) % V) break;
-        if (rows_form(S, C / G, V)) rows = std::max(rows, rows_blocks(rows_shape(C, G, V), N, G));
-        chunks = std::max<uint64_t>(chunks, split_shape(N, S, C, G, V).chunks);
-    }
-    if (!backward && rows_form(S, C / G, 1)) return 0;  // whichever width is picked
     const uint64_t stats = 2 * align256(N * G * 4);
-    if (!backward) return (size_t)(align256(N * chunks * G * sub_slots(C, G) * sizeof(Moments)) + stats);
-    return (size_t)(align256(std::max(rows, N * chunks) * 2 * C * 4) + stats);
+    uint64_t bytes = 0;
+    for (int V = 1; V <= 8 && (C / G) % V == 0; V <<= 1)
+        for (uint32_t es = 2; es <= 4 && es * V <= 16; es += 2) {
+            if (rows_form(S, C / G, V)) {
+                if (backward) bytes = std::max(bytes, rows_blocks(rows_shape(C, G, V), N, G) * 2 * C * 4);
+                continue;
+            }
+            const SplitShape held = resident_shape(N, S, C, G, V, es * V, backward ? 2 : 1);
+            if (held.chunks) {
+                if (backward) bytes = std::max(bytes, resident_grid(N, held.chunks) * 2 * C * 4);
+                continue;
+            }
+            const SplitShape sh = split_shape(N, S, C, G, V);
+            bytes = std::max(bytes, stats + (backward ? align256(N * sh.chunks * 2 * C * 4)
+                                                      : align256(N * sh.chunks * G * sh.SUB * sizeof(Moments))));
+        }
+    return (size_t)bytes;
 }
 
 namespace {
@@ -1076,10 +1307,45 @@ void rows_by_packs(const GroupNormArgs& a, float* partial, bool backward, cudaSt
 }
 
 template <typename T, int V>
+void resident_launch(const GroupNormArgs& a, const SplitShape& sh, float* partial, bool backward, cudaStream_t s) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(backward ? resident_grid(a.N, sh.chunks) : a.N * sh.chunks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = resident_bytes(sh, sizeof(Pack<T, V>), backward ? 2 : 1);
+    cfg.stream = s;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = sh.chunks;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    // per-device attribute: set on every call (cheap), the current device may change
+    if (backward) {
+        TCC_CUDA(cudaFuncSetAttribute(resident_backward_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)kResidentBytes));
+        TCC_CUDA(cudaLaunchKernelEx(&cfg, resident_backward_kernel<T, V>, a, sh, partial));
+        if (partial)
+            param_grad_kernel<<<(2 * a.C + 7) / 8, 1024, 0, s>>>(partial, cfg.gridDim.x, a.C, a.dweight, a.dbias,
+                                                                a.param_type);
+    } else {
+        TCC_CUDA(cudaFuncSetAttribute(resident_forward_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)kResidentBytes));
+        TCC_CUDA(cudaLaunchKernelEx(&cfg, resident_forward_kernel<T, V>, a, sh));
+    }
+    TCC_CUDA(cudaGetLastError());
+}
+
+template <typename T, int V>
 void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStream_t s) {
     const bool params = backward && (a.dweight || a.dbias);
     if (rows_form(a.S, a.C / a.G, V)) {
         rows_by_packs<T, V>(a, params ? reinterpret_cast<float*>(scratch) : nullptr, backward, s);
+        return;
+    }
+    const int arrays = backward ? 2 : 1;
+    const SplitShape held = resident_shape(a.N, a.S, a.C, a.G, V, sizeof(Pack<T, V>), arrays);
+    if (held.chunks) {
+        resident_launch<T, V>(a, held, params ? reinterpret_cast<float*>(scratch) : nullptr, backward, s);
         return;
     }
     const SplitShape sh = split_shape(a.N, a.S, a.C, a.G, V);

@@ -61,15 +61,20 @@ def test_group_norm_refusals(lib):
 
     both = (dict(type=5), dict(pt=-1), dict(act=4), dict(act=-1), dict(G=0), dict(C=0), dict(G=5), dict(x=None),
             dict(x=P + 2), dict(ldx=31), dict(N=1 << 31), dict(S=1 << 31), dict(w=P + 2), dict(b=P + 1),
-            dict(scratch=None), dict(scratch=P + 8), dict(C=(1 << 20) + 4, ldx=1 << 21, ldy=1 << 21))
+            dict(S=1 << 20, scratch=None), dict(S=1 << 20, scratch=P + 8), dict(C=(1 << 20) + 4, ldx=1 << 21, ldy=1 << 21))
     for bad in both + (dict(y=None), dict(ldy=31), dict(eps=-1.0), dict(mean=None), dict(rstd=None)):
         assert forward(**bad) == 1, bad
     for bad in both[:-1] + (dict(dy=None), dict(lddy=31), dict(lddx=31), dict(mean=None), dict(rstd=None),
                             dict(dw=P + 2), dict(db=P + 2)):
         assert backward(**bad) == 1, bad
-    assert forward(nbytes=16) == 6 and backward(nbytes=16) == 6
+    assert forward(S=1 << 20, nbytes=16) == 6 and backward(S=1 << 20, nbytes=16) == 6
     assert forward(N=0) == 0 and forward(S=0) == 0
-    assert lib.tcc_group_norm_scratch_bytes(1000, 1, 256, 8, 0) == 0  # rows by themselves, forward: none
+    # rows by themselves and samples that stay on chip, forward: none; backward: no more for more samples
+    assert lib.tcc_group_norm_scratch_bytes(1000, 1, 256, 8, 0) == 0
+    assert lib.tcc_group_norm_scratch_bytes(64, 517, 100, 10, 0) == 0
+    for steps in (1, 4):
+        few, many = (lib.tcc_group_norm_scratch_bytes(n, steps, 256, 8, 1) for n in (10_000, 10_000_000))
+        assert few == many < 8 << 20
 
 
 def test_clip_refusals(lib):
