@@ -14,9 +14,10 @@
 // own mean, are merged pairwise (Chan, Golub and LeVeque, 1979).
 //
 // Three forms:
-//  * rows  (S = 1, a group within a warp): every group of a row is reduced by
-//    a few lanes of one warp, x is read once; the next rows are on their way
-//    into a ring in shared memory meanwhile.
+//  * rows  (few rows a sample, S = 1 above all; a sample's group within a
+//    warp): every (sample, group) is reduced by a few lanes of one warp, x is
+//    read once; the next samples are on their way into a ring in shared memory
+//    meanwhile.
 //  * resident (a sample that fits the shared memory of at most eight SMs): a
 //    cluster of CTAs holds a sample, x (and dy) are read once, the CTAs exchange
 //    their moments or sums through distributed shared memory.
@@ -30,6 +31,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace tcc {
@@ -257,13 +259,20 @@ __device__ __forceinline__ float inverse_root(float x) {
 
 // ------------------------------------------------------------- rows form --
 
-// A slot is L lanes (a power of two) that hold one group of one row as J packs
-// each; a CTA's 256 / L slots are GB groups x RB rows.  A thread keeps its
-// group for the whole kernel: its parameters and their gradients stay in
-// registers.
+// A slot is L lanes (a power of two) that hold one group of one sample (of its
+// S rows) as J packs each; a CTA's 256 / L slots are GB groups x RB samples.  A
+// thread keeps its channels for the whole kernel: their parameters and the
+// parameters' gradients stay in registers.
 struct RowsShape {
-    uint32_t L, log_L, GB, RB, packs;  // packs: of one group
+    uint32_t L, log_L, GB, RB, PG, packs;  // packs of a group in a row, in a sample
+    // bytes from one pass to the next, computed here so that they are constants there
+    uint64_t x_step, y_step, dy_step, dx_step, stats_step;
 };
+
+template <typename T>
+__device__ __forceinline__ T* advance(T* p, uint64_t bytes) {
+    return reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(p) + bytes);
+}
 
 // Sum over the L lanes of a slot.
 __device__ __forceinline__ float lane_sum(float v, uint32_t L) {
@@ -275,12 +284,13 @@ __device__ __forceinline__ float lane_sum(float v, uint32_t L) {
     return v;
 }
 
-// The place of a thread: its slot's group and row, and its packs' channels.
+// The place of a thread: its slot's group and sample, its packs' rows and
+// channels in them.
 template <int V, int J>
 struct RowsPlace {
     uint32_t lane, g, rb;
     bool on, ok[J];
-    uint64_t c[J];
+    uint32_t row[J], c[J];
     Vec<V> w[J], b[J];
     __device__ __forceinline__ RowsPlace(const GroupNormArgs& a, const RowsShape& sh) {
         const uint32_t slot = threadIdx.x >> sh.log_L;
@@ -292,10 +302,12 @@ struct RowsPlace {
         for (int j = 0; j < J; ++j) {
             const uint32_t p = j * sh.L + lane;
             ok[j] = on && p < sh.packs;
-            c[j] = (uint64_t)g * (a.C / a.G) + (uint64_t)p * V;
+            row[j] = p / sh.PG;
+            c[j] = g * (a.C / a.G) + (p - row[j] * sh.PG) * V;
             load_params<V>(a, c[j], ok[j], w[j], b[j]);
         }
     }
+    __device__ __forceinline__ uint64_t at(int j, uint64_t ld) const { return row[j] * ld + c[j]; }
 };
 
 // wait_copies with a pass number that is a constant once the loop is unrolled.
@@ -333,12 +345,11 @@ __global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormA
     Ring& ring = *reinterpret_cast<Ring*>(smem);
     float* stats = reinterpret_cast<float*>(smem + sizeof(Ring) / 16);  // [2][passes][RB][GB]
     const RowsPlace<V, J> p(a, sh);
-    const float inv = 1.f / (float)(a.C / a.G);
+    const float inv = 1.f / ((float)a.S * (float)(a.C / a.G));
     const uint64_t first = (uint64_t)blockIdx.x * passes * sh.RB;
     const uint32_t rows = (uint32_t)min((uint64_t)passes * sh.RB, a.N - first);  // of the CTA
-    const T* x = static_cast<const T*>(a.x) + (first + p.rb) * a.ldx;
-    T* y = static_cast<T*>(a.y) + (first + p.rb) * a.ldy;
-    const uint64_t x_step = sh.RB * a.ldx, y_step = sh.RB * a.ldy;
+    const T* x = static_cast<const T*>(a.x) + (first + p.rb) * a.S * a.ldx;
+    T* y = static_cast<T*>(a.y) + (first + p.rb) * a.S * a.ldy;
     if constexpr (Ring::kAsync) {
         const T* at = x;
 #pragma unroll
@@ -346,9 +357,9 @@ __global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormA
             if (d * sh.RB + p.rb < rows)
 #pragma unroll
                 for (int j = 0; j < J; ++j)
-                    if (p.ok[j]) copy_pack_async<T, V>(&ring.slot[d][0][j][threadIdx.x], at + p.c[j]);
+                    if (p.ok[j]) copy_pack_async<T, V>(&ring.slot[d][0][j][threadIdx.x], at + p.at(j, a.ldx));
             commit_copies();
-            at += x_step;
+            at = advance(at, sh.x_step);
         }
     }
 #pragma unroll
@@ -362,10 +373,10 @@ __global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormA
             v[j] = splat<V>(0.f);
             if (p.ok[j] && on) {
                 if constexpr (Ring::kAsync) v[j] = widen<T, V>(load_pack<T, V>(ring.slot[d][0][j][threadIdx.x].v));
-                else v[j] = widen<T, V>(load_pack_cs<T, V>(x + p.c[j]));
+                else v[j] = widen<T, V>(load_pack_cs<T, V>(x + p.at(j, a.ldx)));
             }
         }
-        x += x_step;
+        x = advance(x, sh.x_step);
         float s = 0.f, q = 0.f;
 #pragma unroll
         for (int j = 0; j < J; ++j) s += sum(v[j]);
@@ -384,9 +395,9 @@ __global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormA
 #pragma unroll
         for (int j = 0; j < J; ++j)
             if (p.ok[j] && on)
-                store_pack_cs<T, V>(y + p.c[j],
+                store_pack_cs<T, V>(y + p.at(j, a.ldy),
                                     narrow<T, V>(activate<V>(a.act, fma(mul(v[j], splat<V>(r)), p.w[j], p.b[j]))));
-        y += y_step;
+        y = advance(y, sh.y_step);
     }
     if (!a.mean) return;
     __syncthreads();
@@ -401,7 +412,7 @@ __global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormA
 
 // Parameter gradients: a thread's sums over its rows (kept in two levels, so
 // that the rounding error does not grow with the number of rows), then over
-// the CTA's RB rows in shared memory; one partial row per CTA of the grid's x.
+// the CTA's RB samples in shared memory; S partial rows per CTA of the grid's x.
 template <typename T, int V, int J>
 __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1) rows_backward_kernel(const GroupNormArgs a, const RowsShape sh,
                                                                  float* __restrict__ partial) {
@@ -409,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
     extern __shared__ uint4 smem[];
     Ring& ring = *reinterpret_cast<Ring*>(smem);
     const RowsPlace<V, J> p(a, sh);
-    const float inv = 1.f / (float)(a.C / a.G);
+    const float inv = 1.f / ((float)a.S * (float)(a.C / a.G));
     const T* x = static_cast<const T*>(a.x);
     const T* dy = static_cast<const T*>(a.dy);
     T* dx = static_cast<T*>(a.dx);
@@ -420,24 +431,25 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
     // passes of the CTA, and of this thread (the last may end before its row)
     const uint32_t passes = first < a.N ? (uint32_t)((a.N - 1 - first) / stride) + 1 : 0;
     const uint32_t mine = p.on && first + p.rb < a.N ? (uint32_t)((a.N - 1 - first - p.rb) / stride) + 1 : 0;
-    const T* x_next = x + (first + p.rb) * a.ldx;
-    const T* dy_next = dy + (first + p.rb) * a.lddy;
-    T* dx_now = dx + (first + p.rb) * a.lddx;
-    const uint64_t x_step = stride * a.ldx, dy_step = stride * a.lddy, dx_step = stride * a.lddx;
+    // with one pack a lane the pointers hold its place already
+    auto from = [&](int j, uint64_t ld) { return J == 1 ? 0 : p.at(j, ld); };
+    auto start = [&](uint64_t ld) { return (first + p.rb) * a.S * ld + (J == 1 ? p.at(0, ld) : 0); };
+    const T* x_next = x + start(a.ldx);
+    const T* dy_next = dy + start(a.lddy);
+    T* dx_now = dx + start(a.lddx);
     const float* stats_next = a.mean + (first + p.rb) * a.G + p.g;
     const int64_t to_rstd = a.rstd - a.mean;
-    const uint64_t stats_step = stride * a.G;
     auto fetch = [&](uint32_t k, uint32_t d) {
         if (k < mine)
 #pragma unroll
             for (int j = 0; j < J; ++j)
                 if (p.ok[j]) {
-                    copy_pack_async<T, V>(&ring.slot[d][0][j][threadIdx.x], x_next + p.c[j]);
-                    copy_pack_async<T, V>(&ring.slot[d][1][j][threadIdx.x], dy_next + p.c[j]);
+                    copy_pack_async<T, V>(&ring.slot[d][0][j][threadIdx.x], x_next + from(j, a.ldx));
+                    copy_pack_async<T, V>(&ring.slot[d][1][j][threadIdx.x], dy_next + from(j, a.lddy));
                 }
         commit_copies();
-        x_next += x_step;
-        dy_next += dy_step;
+        x_next = advance(x_next, sh.x_step);
+        dy_next = advance(dy_next, sh.dy_step);
     };
     // the statistics of the next row, one row ahead
     float mean_next = 0.f, rstd_next = 0.f;
@@ -446,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
             mean_next = *stats_next;
             rstd_next = stats_next[to_rstd];
         }
-        stats_next += stats_step;
+        stats_next = advance(stats_next, sh.stats_step);
     };
     if constexpr (Ring::kAsync)
         for (uint32_t d = 0; d < Ring::D; ++d) fetch(d, d);
@@ -467,8 +479,8 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
                     h[j] = widen<T, V>(load_pack<T, V>(ring.slot[d][0][j][threadIdx.x].v));
                     g[j] = widen<T, V>(load_pack<T, V>(ring.slot[d][1][j][threadIdx.x].v));
                 } else {
-                    h[j] = widen<T, V>(load_pack_cs<T, V>(x_next + p.c[j]));
-                    g[j] = widen<T, V>(load_pack_cs<T, V>(dy_next + p.c[j]));
+                    h[j] = widen<T, V>(load_pack_cs<T, V>(x_next + from(j, a.ldx)));
+                    g[j] = widen<T, V>(load_pack_cs<T, V>(dy_next + from(j, a.lddy)));
                 }
                 h[j] = mul(add(h[j], splat<V>(-mean)), splat<V>(r));
             }
@@ -477,8 +489,8 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
             fetch(k + Ring::D, d);
             d = d + 1 == Ring::D ? 0 : d + 1;
         } else {
-            x_next += x_step;
-            dy_next += dy_step;
+            x_next = advance(x_next, sh.x_step);
+            dy_next = advance(dy_next, sh.dy_step);
         }
         float s = 0.f, q = 0.f;
 #pragma unroll
@@ -496,10 +508,10 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
 #pragma unroll
             for (int j = 0; j < J; ++j)
                 if (p.ok[j] && live)
-                    store_pack_cs<T, V>(dx_now + p.c[j],
+                    store_pack_cs<T, V>(dx_now + from(j, a.lddx),
                                         narrow<T, V>(mul(splat<V>(r), fma(h[j], splat<V>(-q),
                                                                           add(g[j], splat<V>(-s))))));
-            dx_now += dx_step;
+            dx_now = advance(dx_now, sh.dx_step);
         }
         if (++since == 32) {
             since = 0;
@@ -515,28 +527,49 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
     if constexpr (Ring::kAsync) wait_copies<0>();
     float* sm = reinterpret_cast<float*>(smem);  // [2][kThreads][V], in the ring's place
     static_assert(sizeof(Ring) >= 2 * kThreads * V * sizeof(float) || !Ring::kAsync, "sums fit");
+    // Where the lanes of a slot meet a channel again in other rows of a sample
+    // at a power of two apart, they add up first; else each row is left by itself.
+    const bool fold = a.S > 1 && sh.PG <= sh.L && (sh.PG & (sh.PG - 1)) == 0;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
+        dw[j] = add(dw2[j], dw[j]);
+        db[j] = add(db2[j], db[j]);
+    }
+    if (fold) {
+#pragma unroll
+        for (int j = 1; j < J; ++j) {
+            dw[0] = add(dw[0], dw[j]);
+            db[0] = add(db[0], db[j]);
+        }
+        for (uint32_t o = sh.PG; o < sh.L; o <<= 1) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                dw[0].v[k] += __shfl_xor_sync(0xffffffffu, dw[0].v[k], o);
+                db[0].v[k] += __shfl_xor_sync(0xffffffffu, db[0].v[k], o);
+            }
+        }
+    }
+    const uint32_t across = sh.GB * sh.L * V;  // values of a row of slots
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        if (fold && j) break;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            sm[threadIdx.x * V + k] = dw2[j].v[k] + dw[j].v[k];
-            sm[(kThreads + threadIdx.x) * V + k] = db2[j].v[k] + db[j].v[k];
+            sm[threadIdx.x * V + k] = dw[j].v[k];
+            sm[(kThreads + threadIdx.x) * V + k] = db[j].v[k];
         }
         __syncthreads();
-        if (p.rb == 0 && p.ok[j]) {
-            float* out = partial + (uint64_t)blockIdx.x * 2 * a.C;
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float tw = 0.f, tb = 0.f;
-                for (uint32_t i = 0; i < sh.RB; ++i) {
-                    const uint32_t t = (threadIdx.x + i * sh.GB * sh.L) * V + k;
-                    tw += sm[t];
-                    tb += sm[kThreads * V + t];
-                }
-                out[p.c[j] + k] = tw;
-                out[a.C + p.c[j] + k] = tb;
-            }
+        for (uint32_t i = threadIdx.x; i < 2 * across; i += kThreads) {
+            const uint32_t which = i >= across, e = i - which * across;
+            const uint32_t slot = e / V >> sh.log_L, lane = (e / V) & (sh.L - 1);
+            const uint32_t g = blockIdx.y * sh.GB + slot, pk = j * sh.L + lane, row = pk / sh.PG;
+            if (g >= a.G || pk >= (fold ? sh.PG : sh.packs)) continue;
+            float t = 0.f;
+#pragma unroll 4
+            for (uint32_t r = 0; r < sh.RB; ++r) t += sm[which * kThreads * V + r * across + e];
+            const uint64_t to = fold ? blockIdx.x : (uint64_t)blockIdx.x * a.S + row;
+            partial[(to * 2 + which) * a.C + g * (a.C / a.G) + (pk - row * sh.PG) * V + e % V] = t;
         }
     }
 }
@@ -613,6 +646,14 @@ __device__ __forceinline__ SplitPlace split_place(const GroupNormArgs& a, const 
     p.row0 = p.chunk * sh.chunk_rows;
     p.row1 = min(p.row0 + sh.chunk_rows, a.S);
     return p;
+}
+
+// First channel of the grid's block of columns.
+template <int V>
+__device__ __forceinline__ uint32_t block_channel(const SplitShape& sh) {
+    if (sh.SUB == 1) return blockIdx.y * sh.GPB * sh.PG * V;
+    const uint32_t g = blockIdx.y / sh.SUB;
+    return (g * sh.PG + (blockIdx.y - g * sh.SUB) * sh.TX) * V;
 }
 
 struct Moments {
@@ -828,18 +869,17 @@ __global__ void __launch_bounds__(kThreads, 3) split_sums_kernel(const GroupNorm
         sm[1][threadIdx.x * V + k] = db.v[k];
     }
     __syncthreads();
-    if (p.on && p.rb == 0) {
-        float* out = partial + (p.n * sh.chunks + p.chunk) * 2 * a.C + p.c;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            float tw = 0.f, tb = 0.f;
-            for (uint32_t i = 0; i < sh.RB; ++i) {
-                tw += sm[0][(threadIdx.x + i * sh.TX) * V + k];
-                tb += sm[1][(threadIdx.x + i * sh.TX) * V + k];
-            }
-            out[k] = tw;
-            out[a.C + k] = tb;
-        }
+    // channels of the block, then the rows of threads
+    const uint32_t across = sh.TX * V, c0 = block_channel<V>(sh);
+    const uint32_t c1 = min(c0 + across, sh.SUB == 1 ? a.C : (blockIdx.y / sh.SUB + 1) * (a.C / a.G));
+    float* out = partial + (p.n * sh.chunks + p.chunk) * 2 * a.C;
+    for (uint32_t i = threadIdx.x; i < 2 * across; i += kThreads) {
+        const uint32_t which = i >= across, e = i - which * across;
+        if (c0 + e >= c1) continue;
+        float t = 0.f;
+#pragma unroll 4
+        for (uint32_t r = 0; r < sh.RB; ++r) t += sm[which][r * across + e];
+        out[which * a.C + c0 + e] = t;
     }
 }
 
@@ -932,8 +972,14 @@ namespace cg = cooperative_groups;
 
 // A cluster of sh.chunks CTAs holds a sample, a chunk each; all of a row's
 // packs are in one block (sh.cols = 1).  A thread keeps its packs of its rows
-// at store[(k * A + array) * kThreads] and reads back only what it copied.
+// at store[(k * A + array) * kThreads] and reads back only what it copied.  The
+// store is followed by the threads' and the groups' sums.
 constexpr uint32_t kMaxCluster = 8;
+
+template <int V>
+__host__ __device__ __forceinline__ uint32_t resident_store(const SplitShape& sh, uint32_t pack_bytes, uint32_t arrays) {
+    return (uint32_t)((sh.chunk_rows + sh.RB - 1) / sh.RB) * kThreads * pack_bytes * arrays;
+}
 
 template <typename T, int V, int A>
 __device__ __forceinline__ void fetch_resident(Pack<T, V>* store, const T* const (&from)[A],
@@ -1004,9 +1050,10 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const GroupNormArgs a, const SplitShape sh,
                                                                      float* __restrict__ partial) {
     extern __shared__ uint4 smem[];
-    __shared__ float sums[2][kThreads * V];  // per thread, then per channel
-    __shared__ float2 group[kThreads];       // of this CTA's chunk
-    __shared__ float2 total[kThreads];       // of the sample
+    float(*sums)[kThreads * V] = reinterpret_cast<float(*)[kThreads * V]>(
+        reinterpret_cast<char*>(smem) + resident_store<V>(sh, sizeof(Pack<T, V>), 2));  // [2]: per thread, then channel
+    float2* group = reinterpret_cast<float2*>(sums + 2);  // [G]: of this CTA's chunk
+    float2* total = group + a.G;                          // [G]: of the sample
     cg::cluster_group cluster = cg::this_cluster();
     SplitPlace p = split_place<V>(a, sh, false);
     const uint32_t count = own_rows(p, sh);
@@ -1016,7 +1063,7 @@ __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const Group
     const float inv = 1.f / ((float)a.S * (float)Cg);
     Vec<V> w, b, all_dw = splat<V>(0.f), all_db = all_dw;
     load_params<V>(a, p.c, p.on, w, b);
-    // over the rows of threads: channel c at its first thread's place
+    // use(array, channel, sum over the rows of threads); TX * V = C
     auto over_rows = [&](const Vec<V>& dw, const Vec<V>& db, auto&& use) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -1024,16 +1071,12 @@ __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const Group
             sums[1][threadIdx.x * V + k] = db.v[k];
         }
         __syncthreads();
-        if (p.on && p.rb == 0) {
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float tw = 0.f, tb = 0.f;
-                for (uint32_t i = 0; i < sh.RB; ++i) {
-                    tw += sums[0][(threadIdx.x + i * sh.TX) * V + k];
-                    tb += sums[1][(threadIdx.x + i * sh.TX) * V + k];
-                }
-                use(k, tw, tb);
-            }
+        for (uint32_t i = threadIdx.x; i < 2 * a.C; i += kThreads) {
+            const uint32_t which = i >= a.C, c = i - which * a.C;
+            float t = 0.f;
+#pragma unroll 4
+            for (uint32_t r = 0; r < sh.RB; ++r) t += sums[which][r * a.C + c];
+            use(which, c, t);
         }
     };
     for (; p.n < a.N; p.n += gridDim.x / sh.chunks) {  // the same for the whole cluster
@@ -1058,9 +1101,9 @@ __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const Group
         all_dw = add(all_dw, dw);
         all_db = add(all_db, db);
         if (!a.dx) continue;
-        over_rows(dw, db, [&](int k, float tw, float tb) {
-            sums[0][threadIdx.x * V + k] = tw * w.v[k];
-            sums[1][threadIdx.x * V + k] = tb * w.v[k];
+        // row 0 of the sums becomes the channels' sums: each is read by the thread that writes it
+        over_rows(dw, db, [&](uint32_t which, uint32_t c, float t) {
+            sums[which][c] = t * (a.weight ? load_typed(a.weight, a.param_type, c) : 1.f);
         });
         __syncthreads();
         for (uint32_t g = threadIdx.x >> 5; g < a.G; g += kThreads / 32) {
@@ -1096,14 +1139,22 @@ __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const Group
     }
     if (!partial) return;
     __syncthreads();
-    float* out = partial + (uint64_t)blockIdx.x * 2 * a.C + p.c;
-    over_rows(all_dw, all_db, [&](int k, float tw, float tb) {
-        out[k] = tw;
-        out[a.C + k] = tb;
-    });
+    float* out = partial + (uint64_t)blockIdx.x * 2 * a.C;
+    over_rows(all_dw, all_db, [&](uint32_t which, uint32_t c, float t) { out[which * a.C + c] = t; });
 }
 
 // ------------------------------------------------------------------ host --
+
+// Lets a kernel use `bytes` of dynamic shared memory, once per device.
+template <typename Kernel>
+void allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    TCC_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return;
+    TCC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+}
 
 uint64_t align256(uint64_t b) { return (b + 255) / 256 * 256; }
 
@@ -1120,14 +1171,15 @@ int pick_width(const GroupNormArgs& a) {
     return rule.width();
 }
 
-// The rows form holds up to 8 packs and 32 values a lane.
+// The rows form: up to 8 packs and 32 values a lane, up to 32 rows.
 bool rows_form(uint64_t S, uint32_t Cg, int V) {
-    return S == 1 && Cg <= 32u * std::min(8u * (uint32_t)V, 32u);
+    return S <= 32 && S * Cg <= 32u * std::min(8u * (uint32_t)V, 32u);
 }
 
-RowsShape rows_shape(uint32_t C, uint32_t G, int V) {
-    RowsShape sh;
-    sh.packs = C / G / V;
+RowsShape rows_shape(uint64_t S, uint32_t C, uint32_t G, int V) {
+    RowsShape sh{};
+    sh.PG = C / G / V;
+    sh.packs = (uint32_t)S * sh.PG;
     sh.log_L = 0;
     while (sh.log_L < 5 && (1u << sh.log_L) < sh.packs) ++sh.log_L;
     sh.L = 1u << sh.log_L;
@@ -1139,7 +1191,8 @@ RowsShape rows_shape(uint32_t C, uint32_t G, int V) {
 
 // CTAs in x of the backward: four per SM, which is a whole number of waves (a
 // CTA's registers let four, two or one run at once); each leaves one row of
-// sums for the parameters' gradients.
+// sums for the parameters' gradients per row of a sample.
+bool rows_fold(const RowsShape& sh) { return sh.PG <= sh.L && (sh.PG & (sh.PG - 1)) == 0; }
 uint64_t rows_blocks(const RowsShape& sh, uint64_t N, uint32_t G) {
     const uint64_t y = (G + sh.GB - 1) / sh.GB;
     return std::max<uint64_t>(1, std::min((N + sh.RB - 1) / sh.RB, kSms * 4 / std::min(kSms, y)));
@@ -1172,13 +1225,20 @@ SplitShape split_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V) {
 }
 
 // The resident form's cluster, or chunks = 0 where a sample does not fit: two
-// CTAs per SM; more CTAs than it needs while the GPU has room for them and a
-// thread has rows left to share.
-constexpr size_t kResidentBytes = 88 << 10;
+// CTAs per SM; more CTAs than a sample needs only until every SM has one, and
+// while a thread has rows left to share.
+constexpr uint64_t kResidentBytes = 112 << 10;
 
-SplitShape resident_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V, uint32_t pack_bytes, int arrays) {
+uint64_t resident_bytes(const SplitShape& sh, int V, uint32_t G, uint32_t pack_bytes, uint32_t arrays) {
+    const uint64_t deep = (sh.chunk_rows + sh.RB - 1) / sh.RB;
+    // the forward's sums are in static shared memory, 8 KB
+    return deep * kThreads * pack_bytes * arrays + (arrays == 2 ? 2 * kThreads * V * 4 + 2 * G * 8 : 0);
+}
+
+SplitShape resident_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V, uint32_t pack_bytes,
+                          uint32_t arrays) {
     SplitShape sh{};
-    if (C / V > (uint32_t)kThreads || G > (uint32_t)kThreads || N >= (1ull << 27)) return sh;
+    if (C / V > (uint32_t)kThreads || N >= (1ull << 27)) return sh;
     SplitShape r;
     r.PG = C / G / V;
     r.GPB = G;
@@ -1189,18 +1249,17 @@ SplitShape resident_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V,
     for (uint32_t k = 1; k <= kMaxCluster; k <<= 1) {
         r.chunk_rows = (S + k - 1) / k;
         r.chunks = k;
-        const uint64_t deep = (r.chunk_rows + r.RB - 1) / r.RB;
-        if (deep * kThreads * pack_bytes * arrays > kResidentBytes) continue;
+        if (resident_bytes(r, V, G, pack_bytes, arrays) + (arrays == 1 ? 8 << 10 : 0) > kResidentBytes) continue;
+        // a sample alone on few SMs is slower than its chunks on all of them
+        // (1 x 4000 x 47 fp32: 17.7 against 9.9 us) unless its threads have little to do
+        if (N * k < kSms && r.chunk_rows > 16ull * r.RB) continue;
         sh = r;
-        if (N * k >= 2 * kSms || deep <= 8) break;
+        if (N * k >= kSms || r.chunk_rows <= 8ull * r.RB) break;
     }
     return sh;
 }
 // Clusters of the backward: a cluster of one CTA goes on with another sample.
 uint64_t resident_grid(uint64_t N, uint32_t chunks) { return (chunks > 1 ? N : std::min(N, kSms * 8)) * chunks; }
-size_t resident_bytes(const SplitShape& sh, uint32_t pack_bytes, int arrays) {
-    return (sh.chunk_rows + sh.RB - 1) / sh.RB * kThreads * pack_bytes * arrays;
-}
 
 }  // namespace
 
@@ -1213,7 +1272,7 @@ size_t group_norm_scratch_bytes(uint64_t N, uint64_t S, uint32_t C, uint32_t G, 
     for (int V = 1; V <= 8 && (C / G) % V == 0; V <<= 1)
         for (uint32_t es = 2; es <= 4 && es * V <= 16; es += 2) {
             if (rows_form(S, C / G, V)) {
-                if (backward) bytes = std::max(bytes, rows_blocks(rows_shape(C, G, V), N, G) * 2 * C * 4);
+                if (backward) bytes = std::max(bytes, rows_blocks(rows_shape(S, C, G, V), N, G) * S * 2 * C * 4);
                 continue;
             }
             const SplitShape held = resident_shape(N, S, C, G, V, es * V, backward ? 2 : 1);
@@ -1261,19 +1320,22 @@ void check_norm(const GroupNormArgs& a, void* scratch, size_t scratch_bytes, boo
 
 template <typename T, int V, int J>
 void rows_launch(const GroupNormArgs& a, float* partial, bool backward, cudaStream_t s) {
-    const RowsShape sh = rows_shape(a.C, a.G, V);
+    RowsShape sh = rows_shape(a.S, a.C, a.G, V);
     const uint32_t cols = (a.G + sh.GB - 1) / sh.GB;
-    TCC_REQUIRE(cols <= 65535, "too many groups for one-row samples");
+    TCC_REQUIRE(cols <= 65535, "too many groups for samples of few rows");
     dim3 grid(1, cols);
     if (backward) {
         using Ring = RowsRing<T, V, J, 2>;
         grid.x = (unsigned)rows_blocks(sh, a.N, a.G);
+        const uint64_t samples = (uint64_t)grid.x * sh.RB, bytes = samples * a.S * sizeof(T);
+        sh.x_step = bytes * a.ldx;
+        sh.dy_step = bytes * a.lddy;
+        sh.dx_step = bytes * a.lddx;
+        sh.stats_step = samples * a.G * sizeof(float);
         // where nothing is copied ahead, room for the sums alone
         const size_t smem = std::max<size_t>(Ring::kAsync ? sizeof(Ring) : 0, 2 * kThreads * V * sizeof(float));
-        // per-device attribute: set on every call (cheap), the current device may change
-        if (smem > 48 * 1024)
-            TCC_CUDA(cudaFuncSetAttribute(rows_backward_kernel<T, V, J>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)smem));
+        static std::atomic<uint64_t> done{0};
+        if (smem > 48 * 1024) allow_smem(rows_backward_kernel<T, V, J>, smem, done);
         rows_backward_kernel<T, V, J><<<grid, kThreads, smem, s>>>(a, sh, partial);
     } else {
         using Ring = RowsRing<T, V, J, 1>;
@@ -1282,15 +1344,17 @@ void rows_launch(const GroupNormArgs& a, float* partial, bool backward, cudaStre
         const uint32_t passes = (uint32_t)std::max<uint64_t>(
             1, std::min<uint64_t>(Ring::D, row_passes * cols / (kSms * 4)));
         grid.x = ceil_div(row_passes, passes);
+        sh.x_step = sh.RB * a.S * a.ldx * sizeof(T);
+        sh.y_step = sh.RB * a.S * a.ldy * sizeof(T);
         const size_t smem = sizeof(Ring) + (a.mean ? 2 * passes * sh.RB * sh.GB * sizeof(float) : 0);
-        if (smem > 48 * 1024)
-            TCC_CUDA(cudaFuncSetAttribute(rows_forward_kernel<T, V, J>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)smem));
+        static std::atomic<uint64_t> done{0};
+        // the statistics take at most 2 D floats a slot
+        if (smem > 48 * 1024) allow_smem(rows_forward_kernel<T, V, J>, sizeof(Ring) + 2 * Ring::D * kThreads * 4, done);
         rows_forward_kernel<T, V, J><<<grid, kThreads, smem, s>>>(a, sh, passes);
     }
     TCC_CUDA(cudaGetLastError());
     if (backward && partial) {
-        param_grad_kernel<<<(2 * a.C + 7) / 8, 1024, 0, s>>>(partial, grid.x, a.C, a.dweight, a.dbias,
+        param_grad_kernel<<<(2 * a.C + 7) / 8, 1024, 0, s>>>(partial, grid.x * (rows_fold(sh) ? 1 : a.S), a.C, a.dweight, a.dbias,
                                                               a.param_type);
         TCC_CUDA(cudaGetLastError());
     }
@@ -1298,7 +1362,7 @@ void rows_launch(const GroupNormArgs& a, float* partial, bool backward, cudaStre
 
 template <typename T, int V>
 void rows_by_packs(const GroupNormArgs& a, float* partial, bool backward, cudaStream_t s) {
-    const RowsShape sh = rows_shape(a.C, a.G, V);
+    const RowsShape sh = rows_shape(a.S, a.C, a.G, V);
     const uint32_t per_lane = (sh.packs + sh.L - 1) / sh.L;
     if (per_lane <= 1) rows_launch<T, V, 1>(a, partial, backward, s);
     else if (per_lane <= 2) rows_launch<T, V, 2>(a, partial, backward, s);
@@ -1311,7 +1375,7 @@ void resident_launch(const GroupNormArgs& a, const SplitShape& sh, float* partia
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(backward ? resident_grid(a.N, sh.chunks) : a.N * sh.chunks));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = resident_bytes(sh, sizeof(Pack<T, V>), backward ? 2 : 1);
+    cfg.dynamicSmemBytes = resident_bytes(sh, V, a.G, sizeof(Pack<T, V>), backward ? 2 : 1);
     cfg.stream = s;
     cudaLaunchAttribute cluster{};
     cluster.id = cudaLaunchAttributeClusterDimension;
@@ -1319,17 +1383,15 @@ void resident_launch(const GroupNormArgs& a, const SplitShape& sh, float* partia
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     cfg.attrs = &cluster;
     cfg.numAttrs = 1;
-    // per-device attribute: set on every call (cheap), the current device may change
+    static std::atomic<uint64_t> forward_done{0}, backward_done{0};
     if (backward) {
-        TCC_CUDA(cudaFuncSetAttribute(resident_backward_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)kResidentBytes));
+        allow_smem(resident_backward_kernel<T, V>, kResidentBytes, backward_done);
         TCC_CUDA(cudaLaunchKernelEx(&cfg, resident_backward_kernel<T, V>, a, sh, partial));
         if (partial)
             param_grad_kernel<<<(2 * a.C + 7) / 8, 1024, 0, s>>>(partial, cfg.gridDim.x, a.C, a.dweight, a.dbias,
                                                                 a.param_type);
     } else {
-        TCC_CUDA(cudaFuncSetAttribute(resident_forward_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)kResidentBytes));
+        allow_smem(resident_forward_kernel<T, V>, kResidentBytes, forward_done);
         TCC_CUDA(cudaLaunchKernelEx(&cfg, resident_forward_kernel<T, V>, a, sh));
     }
     TCC_CUDA(cudaGetLastError());
@@ -1342,7 +1404,7 @@ void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStrea
         rows_by_packs<T, V>(a, params ? reinterpret_cast<float*>(scratch) : nullptr, backward, s);
         return;
     }
-    const int arrays = backward ? 2 : 1;
+    const uint32_t arrays = backward ? 2 : 1;
     const SplitShape held = resident_shape(a.N, a.S, a.C, a.G, V, sizeof(Pack<T, V>), arrays);
     if (held.chunks) {
         resident_launch<T, V>(a, held, params ? reinterpret_cast<float*>(scratch) : nullptr, backward, s);

@@ -8,6 +8,7 @@ a variance.  The reference's models have no normalisation
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -48,6 +49,11 @@ def _sizes(x: torch.Tensor, num_groups: int):
     return shape[0], 1 if len(shape) == 2 else math.prod(shape[1:-1]), channels
 
 
+def _statistics(s, name: str, n: int, num_groups: int, x: torch.Tensor) -> None:
+    if s.shape != (n, num_groups) or s.dtype != torch.float32 or s.device != x.device or not s.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 [N, num_groups] tensor on x's device")
+
+
 def _activation(act: str) -> int:
     code = L.ACTIVATIONS.get(act)
     if code is None:
@@ -64,6 +70,11 @@ def _empty(x):
     return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(n: int, steps: int, channels: int, num_groups: int, backward: int) -> int:
+    return L.lib().tcc_group_norm_scratch_bytes(n, steps, channels, num_groups, backward)
+
+
 def _forward(x, num_groups, weight, bias, eps, act, stats):
     code, act = type_code(x, "x"), _activation(act)
     n, steps, channels = _sizes(x, num_groups)
@@ -74,7 +85,7 @@ def _forward(x, num_groups, weight, bias, eps, act, stats):
         mean, rstd = torch.empty((2, n, num_groups), dtype=torch.float32, device=x.device).unbind(0)
     if n and steps:
         x, ld = rows_of(x, channels)
-        nbytes = L.lib().tcc_group_norm_scratch_bytes(n, steps, channels, num_groups, 0)
+        nbytes = _scratch_bytes(n, steps, channels, num_groups, 0)
         hold, scratch = scratch_for(nbytes, x.device)
         launch(x.device, "tcc_group_norm_forward", x.data_ptr(), code, ld, _ptr(weight), _ptr(bias), p_code,
                y.data_ptr(), channels, _ptr(mean), _ptr(rstd), n, steps, channels, num_groups, eps, act,
@@ -101,16 +112,18 @@ def group_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     n, steps, channels = _sizes(x, num_groups)
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
         raise ValueError("dy must have x's shape, type and device")
-    for name, s in (("mean", mean), ("rstd", rstd)):
-        if s.shape != (n, num_groups) or s.dtype != torch.float32 or s.device != x.device or not s.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous float32 [N, num_groups] tensor on x's device")
+    _statistics(mean, "mean", n, num_groups, x)
+    _statistics(rstd, "rstd", n, num_groups, x)
     weight, bias, p_code = _parameters(weight, bias, channels, x)
     dx = _empty(x) if need_dx else None
-    dweight = None if weight is None else torch.empty_like(weight)
-    dbias = None if bias is None else torch.empty_like(bias)
+    if weight is not None and bias is not None:  # one allocation for both
+        dweight, dbias = torch.empty((2, channels), dtype=weight.dtype, device=x.device).unbind(0)
+    else:
+        dweight = None if weight is None else torch.empty_like(weight)
+        dbias = None if bias is None else torch.empty_like(bias)
     x, ldx = rows_of(x, channels)
     dy, lddy = rows_of(dy, channels)
-    nbytes = L.lib().tcc_group_norm_scratch_bytes(n, steps, channels, num_groups, 1)
+    nbytes = _scratch_bytes(n, steps, channels, num_groups, 1)
     hold, scratch = scratch_for(nbytes, x.device)
     launch(x.device, "tcc_group_norm_backward", dy.data_ptr(), lddy, x.data_ptr(), ldx, code, _ptr(weight),
            _ptr(bias), p_code, mean.data_ptr(), rstd.data_ptr(), _ptr(dx), channels, _ptr(dweight),
