@@ -25,62 +25,79 @@ __device__ __forceinline__ int64_t load_index(const void* idx, int type, uint64_
 // ---------------------------------------------------------------- lookup --
 
 constexpr int kLookupThreads = 256;
-constexpr int kLookupUnroll = 8;
+constexpr uint32_t kLookupAhead = 8;
+constexpr uint32_t kLookupRows = 1024;  // of a CTA, at most
 constexpr uint32_t kZeroRow = 0xFFFFFFFFu;  // of padding and of bad indices
 
-// A team of 8, 16 or 32 lanes copies whole rows, a pack a lane; it holds the
-// rows of `lanes` indices at a time, one a lane, and keeps kLookupUnroll of them
-// (or of their parts, if wide) in flight.  The index is read once per row, not
-// per pack, and nothing is divided in the loop.
+// A team of 8, 16 or 32 lanes copies `per` whole rows, a pack a lane, row by row
+// and part by part; the next kLookupAhead parts are on their way into the lane's
+// part of a ring in shared memory.  A CTA reads its indices once, before.
 template <typename TT, typename TO, int V>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(
     const TT* __restrict__ table, uint32_t table_stride, uint32_t num_rows, const void* __restrict__ idx,
     int idx_type, uint32_t n, int64_t padding, float scale, TO* __restrict__ out, uint32_t out_stride,
     uint32_t packs, uint32_t lanes, uint32_t per, uint32_t* __restrict__ bad) {
-    const uint32_t lane = threadIdx.x % lanes;
-    const uint64_t team = (uint64_t)blockIdx.x * (kLookupThreads / lanes) + threadIdx.x / lanes;
-    const uint32_t e0 = (uint32_t)min(team * per, (uint64_t)n), e1 = min(e0 + per, n);
-#pragma unroll 1
-    for (uint32_t b = 0; b < per; b += lanes) {  // the same for the whole CTA
-        const uint32_t at = e0 + b;
-        uint32_t mine = kZeroRow;
-        if (b + lane < per && at + lane < e1) {
-            const int64_t id = load_index(idx, idx_type, at + lane);
-            if (id != padding) {
-                if (id >= 0 && id < (int64_t)num_rows) mine = (uint32_t)id;
-                else if (bad) atomicExch(bad, 1u);
+    constexpr bool kAsync = sizeof(Pack<TT, V>) >= 4;
+    __shared__ Pack<TT, V> ring[kLookupAhead][kLookupThreads];
+    __shared__ uint32_t ids[kLookupRows];
+    const uint32_t teams = kLookupThreads / lanes, first = blockIdx.x * teams * per;
+    const uint32_t rows = min(teams * per, n - first);
+    for (uint32_t i = threadIdx.x; i < rows; i += kLookupThreads) {
+        const int64_t id = load_index(idx, idx_type, first + i);
+        uint32_t row = kZeroRow;
+        if (id != padding) {
+            if (id >= 0 && id < (int64_t)num_rows) row = (uint32_t)id;
+            else if (bad) atomicExch(bad, 1u);
+        }
+        ids[i] = row;
+    }
+    __syncthreads();
+    const uint32_t lane = threadIdx.x % lanes, team = threadIdx.x / lanes;
+    const uint32_t r0 = min(team * per, rows), r1 = min(r0 + per, rows);
+    auto source = [&](uint32_t row, uint32_t c) {
+        return reinterpret_cast<const TT*>(reinterpret_cast<const char*>(table) + (uint64_t)row * table_stride) + c * V;
+    };
+    uint32_t fetch_row = r0, fetch_c = lane, put = 0;
+    auto fetch = [&] {
+        if (fetch_row < r1) {
+            const uint32_t row = ids[fetch_row];
+            if (fetch_c < packs && row != kZeroRow)
+                copy_pack_async<TT, V>(&ring[put][threadIdx.x], source(row, fetch_c));
+            fetch_c += lanes;
+            if (fetch_c - lane >= packs) {
+                fetch_c = lane;
+                ++fetch_row;
             }
         }
-        const uint32_t rows = e1 > at ? min(min(lanes, per - b), e1 - at) : 0;
+        commit_copies();
+        put = (put + 1) % kLookupAhead;
+    };
+    if constexpr (kAsync)
+        for (uint32_t k = 0; k < kLookupAhead; ++k) fetch();
+    uint32_t take = 0;
 #pragma unroll 1
-        for (uint32_t j = 0; j < lanes && __any_sync(0xffffffffu, j < rows); j += kLookupUnroll) {
+    for (uint32_t r = r0; r < r1; ++r) {
+        const uint32_t row = ids[r];
+        TO* to = reinterpret_cast<TO*>(reinterpret_cast<char*>(out) + (uint64_t)(first + r) * out_stride);
 #pragma unroll 1
-            for (uint32_t c0 = 0; c0 < packs; c0 += lanes) {
-                const uint32_t c = c0 + lane;
-                const TT* from = table + (uint64_t)c * V;
-                char* to = reinterpret_cast<char*>(out + (uint64_t)c * V) + (uint64_t)(at + j) * out_stride;
-                Pack<TT, V> val[kLookupUnroll];
-                uint32_t real = 0;  // bit u: row u is one of the table's
-#pragma unroll
-                for (int u = 0; u < kLookupUnroll; ++u) {
-                    const uint32_t row = __shfl_sync(0xffffffffu, mine, j + u, lanes);
-                    if (row != kZeroRow) real |= 1u << u;
-                    if (j + u < rows && c < packs && row != kZeroRow)
-                        val[u] = load_pack_nc<TT, V>(reinterpret_cast<const TT*>(
-                            reinterpret_cast<const char*>(from) + (uint64_t)row * table_stride));
-                }
-#pragma unroll
-                for (int u = 0; u < kLookupUnroll; ++u) {
-                    if (j + u >= rows || c >= packs) continue;
-                    Pack<TO, V> o;
-#pragma unroll
-                    for (int k = 0; k < V; ++k)
-                        o.v[k] = from_f32<TO>(real >> u & 1u ? to_f32(val[u].v[k]) * scale : 0.f);
-                    store_pack_cs<TO, V>(reinterpret_cast<TO*>(to + (uint64_t)u * out_stride), o);
-                }
+        for (uint32_t c = lane; c - lane < packs; c += lanes) {
+            Pack<TT, V> v;
+            if constexpr (kAsync) {
+                wait_copies<kLookupAhead - 1>();
+                v = load_pack<TT, V>(ring[take][threadIdx.x].v);
+                take = (take + 1) % kLookupAhead;
+                fetch();
+            } else if (c < packs && row != kZeroRow) {
+                v = load_pack_nc<TT, V>(source(row, c));
             }
+            if (c >= packs) continue;
+            Pack<TO, V> o;
+#pragma unroll
+            for (int k = 0; k < V; ++k) o.v[k] = from_f32<TO>(row != kZeroRow ? to_f32(v.v[k]) * scale : 0.f);
+            store_pack_cs<TO, V>(to + c * V, o);
         }
     }
+    if constexpr (kAsync) wait_copies<0>();
 }
 
 // Teams of at least as many lanes as rows in flight: narrower packs for
@@ -95,10 +112,10 @@ void launch_lookup(const EmbeddingArgs& a, cudaStream_t s) {
     const uint32_t packs = a.F / V;
     uint32_t lanes = 8;
     while (lanes < 32 && lanes < packs) lanes <<= 1;
-    // a team takes as many rows as it has lanes, fewer where that would leave SMs idle
+    // 32 rows a team, fewer where that would leave less than eight CTAs per SM
     const uint32_t teams = kLookupThreads / lanes;
-    uint32_t per = lanes;
-    while (per > 1 && a.n / per < 148ull * 4 * teams) per >>= 1;
+    uint32_t per = kLookupRows / (kLookupThreads / 8);
+    while (per > 1 && a.n / per < 148ull * 8 * teams) per >>= 1;
     lookup_kernel<TT, TO, V><<<ceil_div(a.n, (uint64_t)per * teams), kLookupThreads, 0, s>>>(
         static_cast<const TT*>(a.table), (uint32_t)(a.ldt * sizeof(TT)), (uint32_t)a.num_rows, a.idx, a.idx_type,
         (uint32_t)a.n, a.padding, a.scale, static_cast<TO*>(a.rows), (uint32_t)(a.ldr * sizeof(TO)), packs, lanes,
