@@ -175,6 +175,10 @@ __device__ __forceinline__ void span_scale(const Span& sp, float f) {
     }
 }
 
+// A factor of 1 changes no value, nor does any factor change zeros alone; a NaN
+// norm spreads, as it should.
+__device__ __forceinline__ bool must_scale(float norm, float factor) { return !(factor >= 1.f) && norm != 0.f; }
+
 template <int THREADS>
 __device__ __forceinline__ void scale_by(const Span& sp, float f) {
     if (sp.type == TCC_F32) span_scale<float, THREADS>(sp, f);
@@ -191,9 +195,8 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
                                                          float eps) {
     const float norm = partial ? norm_of(partial, blocks) : *norm_in;
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
-    // a factor of exactly 1 changes no value; a NaN norm spreads, as it should
     const float f = max_norm / (norm + eps);
-    if (f >= 1.f) return;
+    if (!must_scale(norm, f)) return;
     const uint32_t chunks = t.first[t.count];
     for (uint32_t i = blockIdx.x; i < chunks; i += gridDim.x) {
         const Span sp = chunk_span<K>(t, chunks - 1 - i);
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(kOneThreads) clip_one_kernel(const __grid_cons
         s += squares_of<kTeam>(chunk_span<kSmall>(t, c));
     const float norm = (float)sqrt(block_sum<kOneThreads>(s)), f = max_norm / (norm + eps);
     if (threadIdx.x == 0) *norm_out = norm;
-    if (f >= 1.f) return;
+    if (!must_scale(norm, f)) return;
     for (uint32_t c = threadIdx.x / kTeam; c < chunks; c += kOneThreads / kTeam)
         scale_by<kTeam>(chunk_span<kSmall>(t, c), f);
 }

@@ -8,7 +8,20 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 namespace tcc {
+
+// Lets a kernel use `bytes` of dynamic shared memory, once per device.
+template <typename Kernel>
+void allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    TCC_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return;
+    TCC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+}
 
 inline bool valid_type(int t) { return t == TCC_F32 || t == TCC_F16 || t == TCC_BF16; }
 inline uint32_t type_bytes(int t) { return t == TCC_F32 ? 4u : 2u; }
@@ -91,12 +104,12 @@ __device__ __forceinline__ void store_pack_cs(T* p, const Pack<T, V>& v) {
 }
 
 // Asynchronous copies global -> shared of one pack (4 bytes at least); a
-// thread waits for its own.
-template <typename T, int V>
+// thread waits for its own.  L1: 16-byte copies go through the L1 cache too.
+template <typename T, int V, bool L1 = false>
 __device__ __forceinline__ void copy_pack_async(Pack<T, V>* smem, const T* global) {
     constexpr int bytes = sizeof(T) * V;
     const uint32_t to = (uint32_t)__cvta_generic_to_shared(smem);
-    if constexpr (bytes == 16)
+    if constexpr (bytes == 16 && !L1)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(global) : "memory");
     else if constexpr (bytes >= 4)
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(global), "n"(bytes) : "memory");

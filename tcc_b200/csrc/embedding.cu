@@ -9,11 +9,15 @@
 #include "primitives.cuh"
 #include "train_ops.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 namespace tcc {
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr uint32_t kMaxWidth = 1u << 20;
 
@@ -25,7 +29,11 @@ __device__ __forceinline__ int64_t load_index(const void* idx, int type, uint64_
 // ---------------------------------------------------------------- lookup --
 
 constexpr int kLookupThreads = 256;
-constexpr uint32_t kLookupAhead = 8;
+// Four parts ahead, through L1, so that a row that many indices share is not
+// fetched from one place of L2 each time: 2 M lookups of one row of 400 bytes
+// take 169 us in place of 2141 past L1, power-law ones 273 either way.  Eight
+// ahead leave L1 too little room (314 us).
+constexpr uint32_t kLookupAhead = 4;
 constexpr uint32_t kLookupRows = 1024;  // of a CTA, at most
 constexpr uint32_t kZeroRow = 0xFFFFFFFFu;  // of padding and of bad indices
 
@@ -62,7 +70,7 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(
         if (fetch_row < r1) {
             const uint32_t row = ids[fetch_row];
             if (fetch_c < packs && row != kZeroRow)
-                copy_pack_async<TT, V>(&ring[put][threadIdx.x], source(row, fetch_c));
+                copy_pack_async<TT, V, true>(&ring[put][threadIdx.x], source(row, fetch_c));
             fetch_c += lanes;
             if (fetch_c - lane >= packs) {
                 fetch_c = lane;
@@ -372,14 +380,20 @@ struct ZeroRows {
 
 template <typename W>
 __device__ __forceinline__ void zero_rows_by(const uint8_t* touched, uint32_t r0, uint32_t r1, const ZeroRows& z) {
-    const uint32_t words = z.bytes / (uint32_t)sizeof(W);
-    uint32_t lanes = 1;
-    while (lanes < 32 && lanes < words) lanes <<= 1;
-    const uint32_t lane = threadIdx.x % lanes;
-    for (uint32_t r = r0 + threadIdx.x / lanes; r < r1; r += blockDim.x / lanes) {
-        if (touched[r - r0]) continue;
-        W* row = reinterpret_cast<W*>(z.base + (uint64_t)r * z.stride);
-        for (uint32_t c = lane; c < words; c += lanes) __stcs(row + c, W{});
+    // the range's words in order, whatever a row's length: neighbouring threads, neighbouring words
+    const uint32_t words = z.bytes / (uint32_t)sizeof(W), rows_on = blockDim.x / words;
+    const uint32_t on = blockDim.x - rows_on * words;
+    uint32_t r = threadIdx.x / words, c = threadIdx.x - r * words;
+    char* at = z.base + (uint64_t)r0 * z.stride;
+#pragma unroll 4
+    while (r < r1 - r0) {
+        if (!touched[r]) __stcs(reinterpret_cast<W*>(at + r * z.stride) + c, W{});
+        r += rows_on;
+        c += on;
+        if (c >= words) {
+            c -= words;
+            ++r;
+        }
     }
 }
 
@@ -400,7 +414,7 @@ ZeroRows rows_to_zero(const EmbeddingArgs& a) {
 
 // ------------------------------------------------------------ owner form --
 
-constexpr uint32_t kOwnerMax = 2048;       // indices
+constexpr uint32_t kOwnerMax = 1024;       // indices; 1,000 of one row take 38 us, which the sorted form takes at any
 constexpr uint32_t kOwnerRows = 8192;      // table rows of a CTA, at most
 constexpr int kOwnerEach = kOwnerMax / kThreads;
 
@@ -488,13 +502,13 @@ template <typename TG, typename TT, int V>
 void launch_owner(const EmbeddingArgs& a, cudaStream_t s) {
     const TeamShape sh = team_shape(a.F / V);
     const uint32_t num_rows = (uint32_t)a.num_rows;
-    // four CTAs per SM, or what a CTA can own at most
-    const uint32_t rows = std::min(kOwnerRows, std::max(1u, ceil_div(num_rows, 148 * 4)));
+    // four CTAs per SM, of at most 64 rows each or else sixteen per SM
+    const uint32_t rows =
+        std::min(kOwnerRows, std::max(ceil_div(num_rows, 148 * 16), std::min(64u, ceil_div(num_rows, 148 * 4))));
     const dim3 grid(ceil_div(num_rows, rows), sh.blocks);
     const size_t smem = sizeof(Ring<TG, V>) + (kOwnerMax + 2) * sizeof(Entry) + (rows + 15) / 16 * 16;
-    // per-device attribute: set on every call (cheap), the current device may change
-    TCC_CUDA(cudaFuncSetAttribute(grad_owner_kernel<TG, TT, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  sizeof(Ring<TG, V>) + (kOwnerMax + 2) * sizeof(Entry) + kOwnerRows));
+    static std::atomic<uint64_t> done{0};
+    allow_smem(grad_owner_kernel<TG, TT, V>, sizeof(Ring<TG, V>) + (kOwnerMax + 2) * sizeof(Entry) + kOwnerRows, done);
     grad_owner_kernel<TG, TT, V><<<grid, kThreads, smem, s>>>(
         static_cast<const TG*>(a.rows), (uint32_t)(a.ldr * sizeof(TG)), a.idx, a.idx_type, (uint32_t)a.n,
         a.padding, a.scale, static_cast<TT*>(a.table), a.ldt, num_rows, rows, sh, rows_to_zero(a), a.bad);
@@ -680,10 +694,133 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const Sourc
         if (base + k * 32 < n) out[start[k] + cnt[place[k] >> 16] + (place[k] & 0xFFFFu)] = e[k];
 }
 
+// The whole sort by one cluster of CTAs for up to kClusterMax entries: each CTA
+// holds `each` of them, ranks them by digit, and writes them to their places in
+// the CTAs' shared memory.  One launch in place of seven: 62 us of host time
+// for 2,049 indices otherwise, the kernels' own times far below it.
+constexpr uint32_t kCluster = 8;
+constexpr int kHeldEach = 16;  // entries of a thread
+constexpr uint32_t kHeld = kSortThreads * kHeldEach;
+constexpr uint32_t kClusterMax = kCluster * kHeld;
+
+size_t cluster_smem(uint32_t each, uint32_t digits) {
+    return 2 * (size_t)each * sizeof(Entry) + (size_t)kSortWarps * digits * 2 + (size_t)digits * 12;
+}
+
+__global__ void __launch_bounds__(kSortThreads) cluster_sort_kernel(const IndexSource src, uint32_t n, uint32_t each,
+                                                                    int passes, int bits, Entry* __restrict__ out) {
+    extern __shared__ uint4 smem[];
+    __shared__ uint32_t warp_sums[kSortWarps];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t digits = 1u << bits, rank_cta = cluster.block_rank();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Entry* held = reinterpret_cast<Entry*>(smem);  // [2][each]
+    uint16_t* all = reinterpret_cast<uint16_t*>(held + 2 * each);             // [kSortWarps][digits]
+    uint32_t* hist = reinterpret_cast<uint32_t*>(all + kSortWarps * digits);  // [digits]: of this CTA
+    uint32_t* total = hist + digits;  // [digits]: of the cluster
+    uint32_t* start = total + digits;  // [digits]: where this CTA's first entry of a digit goes
+    uint16_t* cnt = all + warp * digits;
+    const uint32_t first = min(rank_cta * each, n), count = min(each, n - first);
+    // a warp ranks `steps` times 32 neighbouring entries
+    const uint32_t steps = (each + kSortThreads - 1) / kSortThreads, base = warp * steps * 32 + lane;
+    Entry e[kHeldEach];
+#pragma unroll
+    for (int k = 0; k < kHeldEach; ++k) {
+        const uint32_t i = base + k * 32;
+        e[k] = ~0ull;
+        if (k < (int)steps && i < count) {
+            e[k] = src.load(first + i);
+            src.note(first + i, e[k]);
+        }
+    }
+#pragma unroll 1
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * bits;
+        for (uint32_t i = threadIdx.x; i < kSortWarps * digits / 8; i += kSortThreads)
+            reinterpret_cast<uint4*>(all)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        uint32_t place[kHeldEach];
+#pragma unroll
+        for (int k = 0; k < kHeldEach; ++k) {
+            if (k >= (int)steps) break;
+            const bool in = base + k * 32 < count;
+            const uint32_t d = in ? (row_of(e[k]) >> shift) & (digits - 1) : kMaxDigits;
+            const unsigned peers = same_digit(d, in, digits);
+            const uint32_t rank = __popc(peers & lanemask_lt());
+            const uint32_t seen = in ? cnt[d] : 0;
+            __syncwarp();
+            if (in && rank == 0) cnt[d] = (uint16_t)(seen + __popc(peers));
+            __syncwarp();
+            place[k] = d << 16 | (seen + rank);
+        }
+        __syncthreads();
+        for (uint32_t d = threadIdx.x; d < digits / 2; d += kSortThreads) {
+            uint32_t* col = reinterpret_cast<uint32_t*>(all) + d;
+            uint32_t run = 0;
+#pragma unroll
+            for (int w = 0; w < kSortWarps; ++w) {
+                const uint32_t c = col[w * (digits / 2)];
+                col[w * (digits / 2)] = run;
+                run += c;
+            }
+            hist[2 * d] = run & 0xFFFFu;
+            hist[2 * d + 1] = run >> 16;
+        }
+        cluster.sync();  // every CTA's counts are there
+        for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) {
+            uint32_t c[kCluster], before = 0, sum = 0;
+#pragma unroll
+            for (uint32_t r = 0; r < kCluster; ++r) c[r] = *cluster.map_shared_rank(hist + d, r);
+#pragma unroll
+            for (uint32_t r = 0; r < kCluster; ++r) {
+                if (r < rank_cta) before += c[r];
+                sum += c[r];
+            }
+            total[d] = sum;
+            start[d] = before;
+        }
+        __syncthreads();
+        // exclusive sums of the totals: a thread takes neighbouring digits
+        const uint32_t per = (digits + kSortThreads - 1) / kSortThreads, d0 = threadIdx.x * per;
+        uint32_t mine = 0;
+        for (uint32_t i = 0; i < per && d0 + i < digits; ++i) mine += total[d0 + i];
+        uint32_t inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= (uint32_t)o) inc += t;
+        }
+        if (lane == 31) warp_sums[warp] = inc;
+        __syncthreads();
+        uint32_t below = inc - mine;
+        for (uint32_t w = 0; w < warp; ++w) below += warp_sums[w];
+        for (uint32_t i = 0; i < per && d0 + i < digits; ++i) {
+            start[d0 + i] += below;
+            below += total[d0 + i];
+        }
+        __syncthreads();
+        Entry* next = held + (pass & 1) * each;
+#pragma unroll
+        for (int k = 0; k < kHeldEach; ++k)
+            if (k < (int)steps && base + k * 32 < count) {
+                const uint32_t d = place[k] >> 16, to = start[d] + cnt[d] + (place[k] & 0xFFFFu);
+                const uint32_t cta = to / each;
+                *cluster.map_shared_rank(next + (to - cta * each), cta) = e[k];
+            }
+        cluster.sync();  // every entry is in its place, and nobody reads the counts any more
+#pragma unroll
+        for (int k = 0; k < kHeldEach; ++k)
+            if (k < (int)steps && base + k * 32 < count) e[k] = next[base + k * 32];
+    }
+#pragma unroll
+    for (int k = 0; k < kHeldEach; ++k)
+        if (k < (int)steps && base + k * 32 < count) out[first + base + k * 32] = e[k];
+}
+
 // The rows of a table range that have no entry become zero; the range's
 // entries are found by search, and rows looked up in them one by one where
 // they are too many to walk (a hub's).
-constexpr uint32_t kFillRows = 1024;
+constexpr uint32_t kFillRows = 1024;  // at most
 constexpr uint32_t kFillWalk = 16384;
 
 __device__ __forceinline__ uint32_t first_of(const Entry* entries, uint32_t lo, uint32_t hi, uint32_t row) {
@@ -716,7 +853,8 @@ __device__ __forceinline__ void fill_range(const Entry* __restrict__ entries, ui
 
 // CTAs [0, fills) of the grid's x fill; of the others i takes range i of the entries.
 struct SortedShape {
-    uint32_t per, range, sums, fills;  // entries of a team, of a CTA; CTAs
+    uint32_t per, range, sums;  // entries of a team, of a CTA; CTAs
+    uint32_t fill_rows, fills;  // table rows of a CTA that fills; CTAs
 };
 
 template <typename TG, typename TT, int V>
@@ -729,9 +867,9 @@ __global__ void __launch_bounds__(kThreads) grad_sorted_kernel(
         __shared__ uint32_t bounds[2];
         static_assert(kFillRows <= sizeof(Ring<TG, V>), "flags fit");
         // the CTAs of the other columns take their share of the rows
-        const uint32_t share = (kFillRows + gridDim.y - 1) / gridDim.y;
-        const uint32_t r0 = blockIdx.x * kFillRows + min(blockIdx.y * share, kFillRows);
-        const uint32_t r1 = min(min(r0 + share, (blockIdx.x + 1) * kFillRows), num_rows);
+        const uint32_t share = (so.fill_rows + gridDim.y - 1) / gridDim.y;
+        const uint32_t r0 = blockIdx.x * so.fill_rows + min(blockIdx.y * share, so.fill_rows);
+        const uint32_t r1 = min(min(r0 + share, (blockIdx.x + 1) * so.fill_rows), num_rows);
         if (r0 < r1) fill_range(entries, n, r0, r1, zero, reinterpret_cast<uint8_t*>(smem), bounds);
         return;
     }
@@ -830,7 +968,9 @@ SortedShape sorted_shape(uint64_t n, uint64_t num_rows, const TeamShape& sh) {
     so.per = (uint32_t)std::min<uint64_t>(kRangeMax / sh.teams, std::max<uint64_t>(16, per));
     so.range = so.per * sh.teams;
     so.sums = ceil_div(n, so.range);
-    so.fills = ceil_div(num_rows, kFillRows);
+    // about four such CTAs per SM, so that a small table's rows are spread too
+    so.fill_rows = (uint32_t)std::min<uint64_t>(kFillRows, std::max<uint64_t>(16, num_rows / (148 * 4)));
+    so.fills = ceil_div(num_rows, so.fill_rows);
     return so;
 }
 
@@ -868,21 +1008,33 @@ GradScratch lay_out(uint64_t n, uint64_t num_rows, uint32_t F, char* base) {
     return g;
 }
 
-template <typename TG, typename TT, int V>
-void launch_sorted(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
-    const uint32_t n = (uint32_t)a.n, num_rows = (uint32_t)a.num_rows;
-    const GradScratch g = lay_out(n, num_rows, a.F, scratch);
-    const SortPlan p = sort_plan(n, num_rows);
-    const TeamShape sh = team_shape(a.F / V);
-    const SortedShape so = sorted_shape(n, num_rows, sh);
+const Entry* sort_by_cluster(const IndexSource& src, uint32_t n, const SortPlan& p, const GradScratch& g,
+                             cudaStream_t s) {
+    const uint32_t each = (n + kCluster - 1) / kCluster;
+    static std::atomic<uint64_t> done{0};
+    allow_smem(cluster_sort_kernel, cluster_smem(kHeld, kMaxDigits), done);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kCluster);
+    cfg.blockDim = dim3(kSortThreads);
+    cfg.dynamicSmemBytes = cluster_smem(each, p.digits);
+    cfg.stream = s;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = kCluster;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    TCC_CUDA(cudaLaunchKernelEx(&cfg, cluster_sort_kernel, src, n, each, p.passes, p.bits, g.a));
+    return g.a;
+}
+
+const Entry* sort_by_tiles(const IndexSource& src, uint32_t n, const SortPlan& p, const GradScratch& g,
+                           cudaStream_t s) {
     TCC_CUDA(cudaMemsetAsync(g.totals, 0, g.total_bytes, s));
-    const IndexSource from_idx{a.idx, a.idx_type, a.padding, num_rows, a.bad};
     const size_t smem = (size_t)kSortWarps * p.digits * sizeof(uint16_t);
-    // per-device attribute: set on every call (cheap), the current device may change
-    TCC_CUDA(cudaFuncSetAttribute(digit_scatter_kernel<IndexSource>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  kSortWarps * kMaxDigits * sizeof(uint16_t)));
-    TCC_CUDA(cudaFuncSetAttribute(digit_scatter_kernel<EntrySource>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  kSortWarps * kMaxDigits * sizeof(uint16_t)));
+    static std::atomic<uint64_t> first_done{0}, next_done{0};
+    allow_smem(digit_scatter_kernel<IndexSource>, kSortWarps * kMaxDigits * sizeof(uint16_t), first_done);
+    allow_smem(digit_scatter_kernel<EntrySource>, kSortWarps * kMaxDigits * sizeof(uint16_t), next_done);
     Entry* in = g.b;
     Entry* out = g.a;
     for (int pass = 0; pass < p.passes; ++pass) {
@@ -890,19 +1042,32 @@ void launch_sorted(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
         uint32_t* totals = g.totals + (size_t)pass * p.digits;
         const EntrySource from_entries{in};
         if (pass == 0)
-            digit_counts_kernel<<<p.tiles, kSortThreads, 0, s>>>(from_idx, n, shift, p.digits, g.counts, totals);
+            digit_counts_kernel<<<p.tiles, kSortThreads, 0, s>>>(src, n, shift, p.digits, g.counts, totals);
         else
             digit_counts_kernel<<<p.tiles, kSortThreads, 0, s>>>(from_entries, n, shift, p.digits, g.counts, totals);
         digit_offsets_kernel<<<ceil_div(p.digits, 32), 1024, 0, s>>>(g.counts, p.tiles, p.digits, totals);
         if (pass == 0)
-            digit_scatter_kernel<<<p.tiles, kSortThreads, smem, s>>>(from_idx, n, shift, p.digits, g.counts, out);
+            digit_scatter_kernel<<<p.tiles, kSortThreads, smem, s>>>(src, n, shift, p.digits, g.counts, out);
         else
             digit_scatter_kernel<<<p.tiles, kSortThreads, smem, s>>>(from_entries, n, shift, p.digits, g.counts, out);
         std::swap(in, out);
     }
+    TCC_CUDA(cudaGetLastError());
+    return in;
+}
+
+template <typename TG, typename TT, int V>
+void launch_sorted(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
+    const uint32_t n = (uint32_t)a.n, num_rows = (uint32_t)a.num_rows;
+    const GradScratch g = lay_out(n, num_rows, a.F, scratch);
+    const SortPlan p = sort_plan(n, num_rows);
+    const TeamShape sh = team_shape(a.F / V);
+    const SortedShape so = sorted_shape(n, num_rows, sh);
+    const IndexSource from_idx{a.idx, a.idx_type, a.padding, num_rows, a.bad};
+    const Entry* in = n <= kClusterMax ? sort_by_cluster(from_idx, n, p, g, s) : sort_by_tiles(from_idx, n, p, g, s);
+    static std::atomic<uint64_t> sums_done{0};
     const size_t sum_smem = sizeof(Ring<TG, V>) + (so.range + 2) * sizeof(Entry);
-    TCC_CUDA(cudaFuncSetAttribute(grad_sorted_kernel<TG, TT, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  sizeof(Ring<TG, V>) + (kRangeMax + 2) * sizeof(Entry)));
+    allow_smem(grad_sorted_kernel<TG, TT, V>, sizeof(Ring<TG, V>) + (kRangeMax + 2) * sizeof(Entry), sums_done);
     grad_sorted_kernel<TG, TT, V><<<dim3(so.fills + so.sums, sh.blocks), kThreads, sum_smem, s>>>(
         static_cast<const TG*>(a.rows), (uint32_t)(a.ldr * sizeof(TG)), in, n, a.scale, static_cast<TT*>(a.table),
         a.ldt, num_rows, sh, so, rows_to_zero(a), g.heads, g.tails, g.borders);

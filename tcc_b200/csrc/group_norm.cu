@@ -31,7 +31,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 namespace tcc {
@@ -1145,17 +1144,6 @@ __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const Group
 
 // ------------------------------------------------------------------ host --
 
-// Lets a kernel use `bytes` of dynamic shared memory, once per device.
-template <typename Kernel>
-void allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
-    int dev = 0;
-    TCC_CUDA(cudaGetDevice(&dev));
-    const uint64_t bit = 1ull << (dev & 63);
-    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return;
-    TCC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    if (dev < 64) done.fetch_or(bit, std::memory_order_release);
-}
-
 uint64_t align256(uint64_t b) { return (b + 255) / 256 * 256; }
 
 int pick_width(const GroupNormArgs& a) {
@@ -1258,8 +1246,8 @@ SplitShape resident_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V,
     }
     return sh;
 }
-// Clusters of the backward: a cluster of one CTA goes on with another sample.
-uint64_t resident_grid(uint64_t N, uint32_t chunks) { return (chunks > 1 ? N : std::min(N, kSms * 8)) * chunks; }
+// CTAs of the backward: a cluster goes on with another sample.
+uint64_t resident_grid(uint64_t N, uint32_t chunks) { return std::min(N, kSms * 8 / chunks) * chunks; }
 
 }  // namespace
 

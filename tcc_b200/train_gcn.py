@@ -161,6 +161,8 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
         with torch.no_grad():
             W1.copy_(ck["W1"])
             W2.copy_(ck["W2"])
+            if (norm is not None) != ("norm" in ck):
+                raise ValueError("the checkpoint and this run differ in whether they normalise (--norm-groups)")
             if norm is not None:
                 norm.load_state_dict(ck["norm"])
         opt.load_state_dict(ck["opt"])

@@ -194,3 +194,17 @@ def test_offsets_past_32_bits(gpu):
     p.grad[0], p.grad[1 << 31], p.grad[n - 1] = 3.0, 4.0, 12.0
     assert float(K.clip_grad_norm_(p, 6.5)) == 13.0
     assert [float(p.grad[i]) for i in (0, 1 << 31, n - 1)] == [1.5, 2.0, 6.0]
+
+
+@pytest.mark.parametrize("shapes", [[(50,)], [(300, 300), (7,)]])
+def test_zero_gradients(gpu, shapes):
+    for max_norm, eps in ((1.0, 1e-6), (0.0, 1e-6), (0.0, 0.0), (1.0, 0.0)):
+        ps = _params(shapes, (F32,), 1, scale=0.0)
+        assert float(K.clip_grad_norm_(ps, max_norm, eps=eps)) == 0.0
+        assert not any(p.grad.any() or p.grad.isnan().any() for p in ps)
+
+
+def test_limit_of_the_one_launch_form(gpu):
+    """One byte range and one tensor more than what one launch takes."""
+    for shapes in ([(49152,)], [(49152,), (1,)], [(1536,)] * 32, [(1489,)] * 33):
+        _check_clip(_params(shapes, (F32,), 11), 1.0)

@@ -20,6 +20,7 @@ import math
 import pytest
 import torch
 
+from tcc_b200 import _lib as L
 from tcc_b200 import norm as N
 
 pytestmark = pytest.mark.gpu
@@ -310,3 +311,59 @@ def test_offsets_past_32_bits(gpu):
     del dx
     whole = N.group_norm(x.view(1, rows, c), 8)
     assert torch.equal(whole[0, rows - 1], whole[0, 0]) and bool((whole[0, ::70001] == whole[0, 0]).all())
+
+
+def _call(name, *args):
+    L.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("shape,groups", [((500, 1, 64), 8), ((300, 5, 24), 6), ((7, 130, 40), 4), ((2, 6000, 64), 8)])
+def test_outputs_in_the_place_of_inputs(gpu, shape, groups):
+    """The C calls with y = x and dx = dy (every form), and with rows further apart than C."""
+    n, steps, c = shape
+    for pad in (0, 8):
+        x, w, b, dy = _inputs((n, steps, c + pad), F32, F32, 14)
+        o = Oracle(x[..., :c].contiguous(), groups, w[:c], b[:c], 1e-5, "silu")
+        mean, rstd = torch.empty((2, n, groups), device="cuda").unbind(0)
+        size = L.lib().tcc_group_norm_scratch_bytes(n, steps, c, groups, 1)
+        size = max(size, L.lib().tcc_group_norm_scratch_bytes(n, steps, c, groups, 0), 256)
+        scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+        y, dx, beside = x.clone(), dy.clone(), [t[..., c:].clone() for t in (x, dy)]
+        _call("tcc_group_norm_forward", y.data_ptr(), L.F32, c + pad, w.data_ptr(), b.data_ptr(), L.F32, y.data_ptr(),
+              c + pad, mean.data_ptr(), rstd.data_ptr(), n, steps, c, groups, 1e-5, 2, scratch.data_ptr(), size)
+        o.check_forward(y[..., :c].contiguous(), mean, rstd)
+        dw, db = torch.empty_like(w[:c]), torch.empty_like(b[:c])
+        _call("tcc_group_norm_backward", dx.data_ptr(), c + pad, x.data_ptr(), c + pad, L.F32, w.data_ptr(),
+              b.data_ptr(), L.F32, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), c + pad, dw.data_ptr(),
+              db.data_ptr(), n, steps, c, groups, 2, scratch.data_ptr(), size)
+        o.check_backward(dy[..., :c].contiguous(), dx[..., :c].contiguous(), dw, db)
+        assert torch.equal(y[..., c:], beside[0]) and torch.equal(dx[..., c:], beside[1])
+
+
+@pytest.mark.parametrize("shape,groups", [((500, 1, 64), 8), ((7, 130, 40), 4), ((2, 6000, 64), 8)])
+def test_parts_of_the_backward(gpu, shape, groups):
+    """Only dx, only one parameter's gradient: the same bits as all at once."""
+    n, steps, c = shape
+    x, w, b, dy = _inputs(shape, F32, F32, 15)
+    _, mean, rstd = N.group_norm_forward(x, groups, w, b, act="gelu")
+    dx, dw, db = N.group_norm_backward(dy, x, mean, rstd, groups, w, b, act="gelu")
+    none_dx, dw2, db2 = N.group_norm_backward(dy, x, mean, rstd, groups, w, b, act="gelu", need_dx=False)
+    assert none_dx is None and torch.equal(dw, dw2) and torch.equal(db, db2)
+    size = L.lib().tcc_group_norm_scratch_bytes(n, steps, c, groups, 1)
+    scratch = torch.empty(max(size, 256), dtype=torch.uint8, device="cuda")
+    for want in ((dx, None, None), (None, dw, None), (dx, None, db)):
+        got = [None if t is None else torch.empty_like(t) for t in want]
+        ptr = [None if t is None else t.data_ptr() for t in got]
+        _call("tcc_group_norm_backward", dy.data_ptr(), c, x.data_ptr(), c, L.F32, w.data_ptr(), b.data_ptr(), L.F32,
+              mean.data_ptr(), rstd.data_ptr(), ptr[0], c, ptr[1], ptr[2], n, steps, c, groups, 3, scratch.data_ptr(),
+              size)
+        for t, v in zip(got, want):
+            assert t is None or torch.equal(t, v)
+
+
+@pytest.mark.parametrize("n,steps,c,groups", [(5000, 4, 64, 8), (3000, 40, 24, 3), (40, 2000, 64, 8), (1200, 1, 2048, 1)])
+def test_many_samples(gpu, n, steps, c, groups):
+    """More samples than CTAs run at once, in every form."""
+    shape = (n, c) if steps == 1 else (n, steps, c)
+    x, w, b, dy = _inputs(shape, F32, F32, 16)
+    _both(x, groups, w, b, dy, "silu")
