@@ -525,7 +525,7 @@ constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kTileEach = 8;
 constexpr uint32_t kTile = kSortThreads * kTileEach;  // entries of a tile
-constexpr int kMaxDigitBits = 11;
+constexpr int kMinDigitBits = 8, kMaxDigitBits = 11;
 constexpr uint32_t kMaxDigits = 1u << kMaxDigitBits;
 
 struct IndexSource {  // pass 0: the indices themselves; rows without a gradient sort last
@@ -628,24 +628,24 @@ __global__ void __launch_bounds__(1024) digit_offsets_kernel(uint32_t* __restric
 
 // Lanes of the warp with the same digit: a vote for each of its bits (the
 // warp's own match instruction took longer: 20 us in place of 14 per pass at 1 M).
-__device__ __forceinline__ unsigned same_digit(uint32_t d, bool in, uint32_t digits) {
+template <int BITS>
+__device__ __forceinline__ unsigned same_digit(uint32_t d, bool in) {
     unsigned same = __ballot_sync(0xffffffffu, in);
 #pragma unroll
-    for (uint32_t bit = 1; bit < kMaxDigits; bit <<= 1) {
-        if (bit >= digits) break;
-        const unsigned set = __ballot_sync(0xffffffffu, d & bit);
-        same &= d & bit ? set : ~set;
+    for (int bit = 0; bit < BITS; ++bit) {
+        const unsigned set = __ballot_sync(0xffffffffu, d >> bit & 1u);
+        same &= d >> bit & 1u ? set : ~set;
     }
     return same;
 }
 
 // Stable: warp w ranks the tile's entries [w * 256, (w + 1) * 256) against its
 // own digit counts; a prefix over the warps puts them in order.
-template <typename Source>
+template <typename Source, int BITS>
 __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const Source src, uint32_t n, int shift,
-                                                                     uint32_t digits,
                                                                      const uint32_t* __restrict__ offsets,
                                                                      Entry* __restrict__ out) {
+    constexpr uint32_t digits = 1u << BITS;
     extern __shared__ uint4 smem[];
     uint16_t* all = reinterpret_cast<uint16_t*>(smem);  // [kSortWarps][digits]
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const Sourc
     for (int k = 0; k < kTileEach; ++k) {
         const bool in = base + k * 32 < n;
         const uint32_t d = in ? (row_of(e[k]) >> shift) & (digits - 1) : kMaxDigits;
-        const unsigned peers = same_digit(d, in, digits);
+        const unsigned peers = same_digit<BITS>(d, in);
         const uint32_t rank = __popc(peers & lanemask_lt());
         const uint32_t seen = in ? cnt[d] : 0;
         __syncwarp();
@@ -707,12 +707,14 @@ size_t cluster_smem(uint32_t each, uint32_t digits) {
     return 2 * (size_t)each * sizeof(Entry) + (size_t)kSortWarps * digits * 2 + (size_t)digits * 12;
 }
 
+template <int BITS>
 __global__ void __launch_bounds__(kSortThreads) cluster_sort_kernel(const IndexSource src, uint32_t n, uint32_t each,
-                                                                    int passes, int bits, Entry* __restrict__ out) {
+                                                                    int passes, Entry* __restrict__ out) {
     extern __shared__ uint4 smem[];
     __shared__ uint32_t warp_sums[kSortWarps];
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t digits = 1u << bits, rank_cta = cluster.block_rank();
+    constexpr uint32_t digits = 1u << BITS;
+    const uint32_t rank_cta = cluster.block_rank();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Entry* held = reinterpret_cast<Entry*>(smem);  // [2][each]
     uint16_t* all = reinterpret_cast<uint16_t*>(held + 2 * each);             // [kSortWarps][digits]
@@ -735,7 +737,7 @@ __global__ void __launch_bounds__(kSortThreads) cluster_sort_kernel(const IndexS
     }
 #pragma unroll 1
     for (int pass = 0; pass < passes; ++pass) {
-        const int shift = pass * bits;
+        const int shift = pass * BITS;
         for (uint32_t i = threadIdx.x; i < kSortWarps * digits / 8; i += kSortThreads)
             reinterpret_cast<uint4*>(all)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
@@ -745,7 +747,7 @@ __global__ void __launch_bounds__(kSortThreads) cluster_sort_kernel(const IndexS
             if (k >= (int)steps) break;
             const bool in = base + k * 32 < count;
             const uint32_t d = in ? (row_of(e[k]) >> shift) & (digits - 1) : kMaxDigits;
-            const unsigned peers = same_digit(d, in, digits);
+            const unsigned peers = same_digit<BITS>(d, in);
             const uint32_t rank = __popc(peers & lanemask_lt());
             const uint32_t seen = in ? cnt[d] : 0;
             __syncwarp();
@@ -799,6 +801,15 @@ __global__ void __launch_bounds__(kSortThreads) cluster_sort_kernel(const IndexS
             below += total[d0 + i];
         }
         __syncthreads();
+        if (pass + 1 == passes) {
+#pragma unroll
+            for (int k = 0; k < kHeldEach; ++k)
+                if (k < (int)steps && base + k * 32 < count) {
+                    const uint32_t d = place[k] >> 16;
+                    out[start[d] + cnt[d] + (place[k] & 0xFFFFu)] = e[k];
+                }
+            break;
+        }
         Entry* next = held + (pass & 1) * each;
 #pragma unroll
         for (int k = 0; k < kHeldEach; ++k)
@@ -812,9 +823,7 @@ __global__ void __launch_bounds__(kSortThreads) cluster_sort_kernel(const IndexS
         for (int k = 0; k < kHeldEach; ++k)
             if (k < (int)steps && base + k * 32 < count) e[k] = next[base + k * 32];
     }
-#pragma unroll
-    for (int k = 0; k < kHeldEach; ++k)
-        if (k < (int)steps && base + k * 32 < count) out[first + base + k * 32] = e[k];
+    cluster.sync();  // no CTA's counts go while another reads them
 }
 
 // The rows of a table range that have no entry become zero; the range's
@@ -953,7 +962,7 @@ SortPlan sort_plan(uint64_t n, uint64_t num_rows) {
     SortPlan p;
     const int total = std::max(1, bits_for(num_rows + 1));
     p.passes = (total + kMaxDigitBits - 1) / kMaxDigitBits;
-    p.bits = std::max(3, (total + p.passes - 1) / p.passes);  // whole 16-byte words of counts
+    p.bits = std::max(kMinDigitBits, (total + p.passes - 1) / p.passes);
     p.digits = 1u << p.bits;
     p.tiles = ceil_div(n, kTile);
     return p;
@@ -1008,11 +1017,12 @@ GradScratch lay_out(uint64_t n, uint64_t num_rows, uint32_t F, char* base) {
     return g;
 }
 
+template <int BITS>
 const Entry* sort_by_cluster(const IndexSource& src, uint32_t n, const SortPlan& p, const GradScratch& g,
                              cudaStream_t s) {
     const uint32_t each = (n + kCluster - 1) / kCluster;
     static std::atomic<uint64_t> done{0};
-    allow_smem(cluster_sort_kernel, cluster_smem(kHeld, kMaxDigits), done);
+    allow_smem(cluster_sort_kernel<BITS>, cluster_smem(kHeld, p.digits), done);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kCluster);
     cfg.blockDim = dim3(kSortThreads);
@@ -1024,21 +1034,22 @@ const Entry* sort_by_cluster(const IndexSource& src, uint32_t n, const SortPlan&
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     cfg.attrs = &cluster;
     cfg.numAttrs = 1;
-    TCC_CUDA(cudaLaunchKernelEx(&cfg, cluster_sort_kernel, src, n, each, p.passes, p.bits, g.a));
+    TCC_CUDA(cudaLaunchKernelEx(&cfg, cluster_sort_kernel<BITS>, src, n, each, p.passes, g.a));
     return g.a;
 }
 
+template <int BITS>
 const Entry* sort_by_tiles(const IndexSource& src, uint32_t n, const SortPlan& p, const GradScratch& g,
                            cudaStream_t s) {
     TCC_CUDA(cudaMemsetAsync(g.totals, 0, g.total_bytes, s));
     const size_t smem = (size_t)kSortWarps * p.digits * sizeof(uint16_t);
     static std::atomic<uint64_t> first_done{0}, next_done{0};
-    allow_smem(digit_scatter_kernel<IndexSource>, kSortWarps * kMaxDigits * sizeof(uint16_t), first_done);
-    allow_smem(digit_scatter_kernel<EntrySource>, kSortWarps * kMaxDigits * sizeof(uint16_t), next_done);
+    allow_smem(digit_scatter_kernel<IndexSource, BITS>, smem, first_done);
+    allow_smem(digit_scatter_kernel<EntrySource, BITS>, smem, next_done);
     Entry* in = g.b;
     Entry* out = g.a;
     for (int pass = 0; pass < p.passes; ++pass) {
-        const int shift = pass * p.bits;
+        const int shift = pass * BITS;
         uint32_t* totals = g.totals + (size_t)pass * p.digits;
         const EntrySource from_entries{in};
         if (pass == 0)
@@ -1047,13 +1058,19 @@ const Entry* sort_by_tiles(const IndexSource& src, uint32_t n, const SortPlan& p
             digit_counts_kernel<<<p.tiles, kSortThreads, 0, s>>>(from_entries, n, shift, p.digits, g.counts, totals);
         digit_offsets_kernel<<<ceil_div(p.digits, 32), 1024, 0, s>>>(g.counts, p.tiles, p.digits, totals);
         if (pass == 0)
-            digit_scatter_kernel<<<p.tiles, kSortThreads, smem, s>>>(src, n, shift, p.digits, g.counts, out);
+            digit_scatter_kernel<IndexSource, BITS><<<p.tiles, kSortThreads, smem, s>>>(src, n, shift, g.counts, out);
         else
-            digit_scatter_kernel<<<p.tiles, kSortThreads, smem, s>>>(from_entries, n, shift, p.digits, g.counts, out);
+            digit_scatter_kernel<EntrySource, BITS>
+                <<<p.tiles, kSortThreads, smem, s>>>(from_entries, n, shift, g.counts, out);
         std::swap(in, out);
     }
     TCC_CUDA(cudaGetLastError());
     return in;
+}
+
+template <int BITS>
+const Entry* sort_entries(const IndexSource& src, uint32_t n, const SortPlan& p, const GradScratch& g, cudaStream_t s) {
+    return n <= kClusterMax ? sort_by_cluster<BITS>(src, n, p, g, s) : sort_by_tiles<BITS>(src, n, p, g, s);
 }
 
 template <typename TG, typename TT, int V>
@@ -1064,7 +1081,10 @@ void launch_sorted(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
     const TeamShape sh = team_shape(a.F / V);
     const SortedShape so = sorted_shape(n, num_rows, sh);
     const IndexSource from_idx{a.idx, a.idx_type, a.padding, num_rows, a.bad};
-    const Entry* in = n <= kClusterMax ? sort_by_cluster(from_idx, n, p, g, s) : sort_by_tiles(from_idx, n, p, g, s);
+    const Entry* in = p.bits == 8    ? sort_entries<8>(from_idx, n, p, g, s)
+                      : p.bits == 9  ? sort_entries<9>(from_idx, n, p, g, s)
+                      : p.bits == 10 ? sort_entries<10>(from_idx, n, p, g, s)
+                                     : sort_entries<11>(from_idx, n, p, g, s);
     static std::atomic<uint64_t> sums_done{0};
     const size_t sum_smem = sizeof(Ring<TG, V>) + (so.range + 2) * sizeof(Entry);
     allow_smem(grad_sorted_kernel<TG, TT, V>, sizeof(Ring<TG, V>) + (kRangeMax + 2) * sizeof(Entry), sums_done);
