@@ -192,7 +192,8 @@ struct Border {
 // A lane's packs of the next kUnroll rows lie in a ring in shared memory, which
 // asynchronous copies fill while earlier rows are added; a lane reads back only
 // what it copied itself.  (Rows held in registers instead took 64 to 200
-// registers a thread: 199 us for the sums of 1 M x 128 in place of 130.)
+// registers a thread: 199 us for the sums of 1 M x 128 alone, in place of 182
+// with the zeroing of the other rows beside them.)
 template <typename TG, int V>
 struct Ring {
     Pack<TG, V> slot[kUnroll][kThreads];
@@ -414,7 +415,9 @@ ZeroRows rows_to_zero(const EmbeddingArgs& a) {
 
 // ------------------------------------------------------------ owner form --
 
-constexpr uint32_t kOwnerMax = 1024;       // indices; 1,000 of one row take 38 us, which the sorted form takes at any
+// Indices of the owner form, at most: 1,000 spread ones take 7 us, in the sorted
+// form 20; but 2,000 of one row are one CTA's work, 73 us, there 28.
+constexpr uint32_t kOwnerMax = 1024;
 constexpr uint32_t kOwnerRows = 8192;      // table rows of a CTA, at most
 constexpr int kOwnerEach = kOwnerMax / kThreads;
 
@@ -627,7 +630,7 @@ __global__ void __launch_bounds__(1024) digit_offsets_kernel(uint32_t* __restric
 }
 
 // Lanes of the warp with the same digit: a vote for each of its bits (the
-// warp's own match instruction took longer: 20 us in place of 14 per pass at 1 M).
+// warp's own match instruction took 17 us in place of 15 for a pass over 1 M).
 template <int BITS>
 __device__ __forceinline__ unsigned same_digit(uint32_t d, bool in) {
     unsigned same = __ballot_sync(0xffffffffu, in);
@@ -696,8 +699,10 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const Sourc
 
 // The whole sort by one cluster of CTAs for up to kClusterMax entries: each CTA
 // holds `each` of them, ranks them by digit, and writes them to their places in
-// the CTAs' shared memory.  One launch in place of seven: 62 us of host time
-// for 2,049 indices otherwise, the kernels' own times far below it.
+// the CTAs' shared memory.  One launch in place of seven: the gradient of 2,049
+// indices takes 24 us in place of 62, most of it the host's; at 65,536 the sort
+// is bound by what eight SMs can do (42 us for two passes of 11 bits) and the
+// tiles of the larger form are as fast.
 constexpr uint32_t kCluster = 8;
 constexpr int kHeldEach = 16;  // entries of a thread
 constexpr uint32_t kHeld = kSortThreads * kHeldEach;
