@@ -80,8 +80,9 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(
         commit_copies();
         put = (put + 1) % kLookupAhead;
     };
+    // a slot is filled again one part after it was read, when its values are in use already
     if constexpr (kAsync)
-        for (uint32_t k = 0; k < kLookupAhead; ++k) fetch();
+        for (uint32_t k = 0; k + 1 < kLookupAhead; ++k) fetch();
     uint32_t take = 0;
 #pragma unroll 1
     for (uint32_t r = r0; r < r1; ++r) {
@@ -91,10 +92,10 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(
         for (uint32_t c = lane; c - lane < packs; c += lanes) {
             Pack<TT, V> v;
             if constexpr (kAsync) {
+                fetch();
                 wait_copies<kLookupAhead - 1>();
                 v = load_pack<TT, V>(ring[take][threadIdx.x].v);
                 take = (take + 1) % kLookupAhead;
-                fetch();
             } else if (c < packs && row != kZeroRow) {
                 v = load_pack_nc<TT, V>(source(row, c));
             }
@@ -286,12 +287,13 @@ struct RunSums {
                     copy_pack_async<TG, V>(&ring->slot[(i - e0) % kUnroll][threadIdx.x], source(ent[i]));
                 commit_copies();
             };
-            for (uint32_t u = 0; u < kUnroll; ++u) fetch(e0 + u);
+            // a slot is filled again one row after it was read, when its values are in use already
+            for (uint32_t u = 0; u + 1 < kUnroll; ++u) fetch(e0 + u);
 #pragma unroll 1
             for (uint32_t i = e0; i < e1; ++i) {
+                fetch(i + kUnroll - 1);
                 wait_copies<kUnroll - 1>();
                 consume(i, (i - e0) % kUnroll);
-                fetch(i + kUnroll);
             }
             wait_copies<0>();
         } else {
@@ -988,9 +990,13 @@ SortedShape sorted_shape(uint64_t n, uint64_t num_rows, const TeamShape& sh) {
     return so;
 }
 
-// Ranges whatever the vector width: a range is never below 16 entries of the
-// eight teams that full warps give.
-uint64_t max_sums(uint64_t n) { return n / (16 * (kThreads / 32)) + 1; }
+// Ranges of any vector width.
+uint64_t max_sums(uint64_t n, uint64_t num_rows, uint32_t F) {
+    uint64_t most = 1;
+    for (uint32_t width = 1; width <= 8 && F % width == 0; width <<= 1)
+        most = std::max<uint64_t>(most, sorted_shape(n, num_rows, team_shape(F / width)).sums);
+    return most;
+}
 
 struct GradScratch {
     Entry *a, *b;
@@ -1004,6 +1010,7 @@ struct GradScratch {
 GradScratch lay_out(uint64_t n, uint64_t num_rows, uint32_t F, char* base) {
     GradScratch g;
     const SortPlan p = sort_plan(n, num_rows);
+    const uint64_t sums = max_sums(n, num_rows, F);
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
         char* q = base + at;
@@ -1015,9 +1022,9 @@ GradScratch lay_out(uint64_t n, uint64_t num_rows, uint32_t F, char* base) {
     g.counts = reinterpret_cast<uint32_t*>(take((uint64_t)p.tiles * p.digits * 4));
     g.total_bytes = (size_t)p.passes * p.digits * 4;
     g.totals = reinterpret_cast<uint32_t*>(take(g.total_bytes));
-    g.heads = reinterpret_cast<float*>(take(max_sums(n) * F * 4));
-    g.tails = reinterpret_cast<float*>(take(max_sums(n) * F * 4));
-    g.borders = reinterpret_cast<Border*>(take(max_sums(n) * sizeof(Border)));
+    g.heads = reinterpret_cast<float*>(take(sums * F * 4));
+    g.tails = reinterpret_cast<float*>(take(sums * F * 4));
+    g.borders = reinterpret_cast<Border*>(take(sums * sizeof(Border)));
     g.bytes = at;
     return g;
 }

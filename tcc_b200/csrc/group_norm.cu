@@ -462,17 +462,22 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
         }
         stats_next = advance(stats_next, sh.stats_step);
     };
+    // a slot is filled again one row after it was read, when its values are in use already
     if constexpr (Ring::kAsync)
-        for (uint32_t d = 0; d < Ring::D; ++d) fetch(d, d);
+        for (uint32_t d = 0; d + 1 < Ring::D; ++d) fetch(d, d);
     fetch_stats(0);
-    uint32_t d = 0, since = 0;
+    uint32_t d = 0, put = Ring::D - 1, since = 0;
 #pragma unroll 1
     for (uint32_t k = 0; k < passes; ++k) {
         const bool live = k < mine;
         const float mean = mean_next, r = rstd_next;
         fetch_stats(k + 1);
         Vec<V> h[J], g[J];
-        if constexpr (Ring::kAsync) wait_copies<Ring::D - 1>();
+        if constexpr (Ring::kAsync) {
+            fetch(k + Ring::D - 1, put);
+            put = put + 1 == Ring::D ? 0 : put + 1;
+            wait_copies<Ring::D - 1>();
+        }
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             h[j] = g[j] = splat<V>(0.f);
@@ -488,7 +493,6 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
             }
         }
         if constexpr (Ring::kAsync) {
-            fetch(k + Ring::D, d);
             d = d + 1 == Ring::D ? 0 : d + 1;
         } else {
             x_next = advance(x_next, sh.x_step);
@@ -697,12 +701,17 @@ __device__ __forceinline__ void stream_rows(void* smem, const T* const (&from)[A
             }
         commit_copies();
     };
+    // a slot is filled again one step after it was read, when its values are in use already
     if constexpr (kAsync)
-        for (uint32_t k = 0; k < D; ++k) fetch(k);
+        for (uint32_t k = 0; k < D - B; ++k) fetch(k);
 #pragma unroll 1
     for (uint32_t k = 0; k < count; k += B) {
         Pack<T, V> v[B][A];
-        if constexpr (kAsync) wait_copies<D - B>();
+        if constexpr (kAsync) {
+#pragma unroll
+            for (int u = 0; u < B; ++u) fetch(k + D - B + u);
+            wait_copies<D - B>();
+        }
 #pragma unroll
         for (int u = 0; u < B; ++u)
             if (k + u < count)
@@ -715,9 +724,6 @@ __device__ __forceinline__ void stream_rows(void* smem, const T* const (&from)[A
                         at[i] += inc[i];
                     }
                 }
-        if constexpr (kAsync)
-#pragma unroll
-            for (int u = 0; u < B; ++u) fetch(k + D + u);
         body(v, min((uint32_t)B, count - k));
     }
     if constexpr (kAsync) wait_copies<0>();

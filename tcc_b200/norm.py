@@ -116,11 +116,8 @@ def group_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     _statistics(rstd, "rstd", n, num_groups, x)
     weight, bias, p_code = _parameters(weight, bias, channels, x)
     dx = _empty(x) if need_dx else None
-    if weight is not None and bias is not None:  # one allocation for both
-        dweight, dbias = torch.empty((2, channels), dtype=weight.dtype, device=x.device).unbind(0)
-    else:
-        dweight = None if weight is None else torch.empty_like(weight)
-        dbias = None if bias is None else torch.empty_like(bias)
+    dweight = None if weight is None else torch.empty_like(weight)
+    dbias = None if bias is None else torch.empty_like(bias)
     x, ldx = rows_of(x, channels)
     dy, lddy = rows_of(dy, channels)
     nbytes = _scratch_bytes(n, steps, channels, num_groups, 1)
