@@ -162,3 +162,44 @@ def test_functional_chain_in_a_captured_graph(gpu):
         got = [o.clone() for o in outs] + [p.grad.clone()]
         want = list(chain()) + [p.grad]
         assert all(torch.equal(a, v) for a, v in zip(got, want))  # every order of sums is fixed
+
+
+COLD = """
+import torch
+from tcc_b200 import clip, embedding, norm
+dev = "cuda"
+idx = torch.randint(3000, (80000,), device=dev)
+g = torch.randn(80000, 64, device=dev)
+xs = [torch.randn(*s, device=dev) for s in ((2, 9000, 64), (500, 64), (5, 300, 64))]
+w = torch.ones(64, device=dev)
+p = torch.zeros(300000, device=dev)
+p.grad = torch.randn(300000, device=dev)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    d = [embedding.embedding_backward(g[:n], idx[:n], 3000) for n in (500, 5000, 80000)]
+    e = embedding.embedding(d[2], idx)
+    y = [norm.group_norm_forward(x, 8, w, w, act="gelu") for x in xs]
+    dx = [norm.group_norm_backward(x, x, m, r, 8, w, w, act="gelu") for x, (_, m, r) in zip(xs, y)]
+    total = clip.clip_grad_norm_([p], 1.0)
+graph.replay()
+torch.cuda.synchronize()
+for n, t in zip((500, 5000, 80000), d):
+    assert torch.equal(t, embedding.embedding_backward(g[:n], idx[:n], 3000))
+assert torch.equal(e, embedding.embedding(d[2], idx))
+for x, (o, m, r), t in zip(xs, y, dx):
+    assert torch.equal(o, norm.group_norm(x, 8, w, w, act="gelu"))
+    assert all(torch.equal(a, b) for a, b in zip(t, norm.group_norm_backward(x, x, m, r, 8, w, w, act="gelu")))
+assert abs(float(clip.grad_norm([p.grad])) - 1.0) < 1e-5 and float(total) > 1.0
+print("done")
+"""
+
+
+def test_captured_before_any_other_call(gpu):
+    """A process whose first calls of every form are captured into a graph."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", COLD], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]

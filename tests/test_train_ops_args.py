@@ -128,3 +128,49 @@ def test_python_refusals():
     with pytest.raises(TypeError):
         clip.grad_norm([t.double()])
     assert float(clip.grad_norm([])) == 0.0
+
+
+def test_calls_run_on_the_tensors_device(monkeypatch):
+    """With another device current, the call runs inside a guard for the tensors' device,
+    on that device's current stream; no guard where it is current (fakes, no GPU)."""
+    from tcc_b200 import _args
+    log = []
+
+    class Guard:
+        def __init__(self, device):
+            log.append(("guard", device.index))
+
+        def __enter__(self):
+            log.append("in")
+
+        def __exit__(self, *exc):
+            log.append("out")
+
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(_args, "_current_device", lambda: 0)
+    monkeypatch.setattr(_args, "_raw_stream", lambda index: 100 + index)
+    monkeypatch.setitem(_args._bound, "fake", lambda *args: log.append(args) or 0)
+    _args.launch(torch.device("cuda", 1), "fake", 7)
+    assert log == [("guard", 1), "in", (7, 101), "out"]
+    log.clear()
+    _args.launch(torch.device("cuda", 0), "fake", 8)
+    assert log == [(8, 100)]
+    monkeypatch.setitem(_args._bound, "fake", lambda *args: 1)
+    with pytest.raises(L.TccError):
+        _args.launch(torch.device("cuda", 1), "fake")
+
+
+def test_rows_of_strides():
+    from tcc_b200._args import rows_of
+    t = torch.zeros(6, 5, 8)
+    assert rows_of(t, 8) == (t, 8)
+    part = t[..., 2:6]
+    same, ld = rows_of(part, 4)
+    assert same is part and ld == 8
+    for other in (t.transpose(0, 1)[..., :4], t[:, ::2, :4][..., ::2], torch.zeros(4).expand(3, 5, 4), t[:, :3, :4]):
+        copy, ld = rows_of(other, other.shape[-1])
+        assert copy.is_contiguous() and ld == other.shape[-1] and torch.equal(copy, other)
+    one = t[:1, :1, ::2]  # a single row: only its values' stride counts
+    copy, ld = rows_of(t[:1, 1:2, :4], 4)
+    assert ld == 4
+    assert rows_of(one, 4)[0].is_contiguous()
