@@ -27,22 +27,25 @@ def _dense(t: torch.Tensor) -> bool:
 
 
 def _table(tensors):
-    """(tcc_tensor array of the tensors, its length, their device)."""
-    device, words = None, []
+    """(tcc_tensor array of the tensors, its length, their device, their bytes)."""
+    index, words, nbytes = None, [], 0
     for t in tensors:
         code = TYPES.get(t.dtype)
         if code is None:
             raise TypeError(f"gradients must be float32, float16 or bfloat16, not {t.dtype}")
-        if t.layout is not torch.strided or not t.is_cuda:
+        where = t.get_device()
+        if where < 0 or t.layout is not torch.strided:
             raise ValueError("gradients must be dense CUDA tensors")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError("gradients must be on one device")
+        if where != index:
+            if index is not None:
+                raise ValueError("gradients must be on one device")
+            index = where
         if not (t.is_contiguous() or _dense(t)):
             raise ValueError("a gradient's elements must fill one block of memory (no gaps, no broadcast)")
-        words += (t.data_ptr(), t.numel(), code)  # data, n, type and reserved
-    return array("Q", words), len(words) // 3, device
+        n = t.numel()
+        nbytes += n << 2 if code == L.F32 else n << 1
+        words += (t.data_ptr(), n, code)  # data, n, type and reserved
+    return array("Q", words), len(words) // 3, None if index is None else torch.device("cuda", index), nbytes
 
 
 @functools.cache
@@ -56,13 +59,16 @@ def _list(tensors) -> list:
 
 def _written(tensors) -> None:
     """The tensors were changed in place: a graph that saved one notices."""
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:  # inference tensors have no version
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm of all elements of the tensors (one, or an iterable), a float32 scalar on
     their device; 64-bit sums in a fixed order.  Without tensors a CPU zero."""
-    words, count, device = _table(_list(tensors))
+    words, count, device, _ = _table(_list(tensors))
     if count == 0:
         return torch.zeros(())
     norm = torch.empty((), dtype=torch.float32, device=device)
@@ -77,7 +83,7 @@ def clip_grads_with_norm_(tensors, max_norm: float, total_norm: torch.Tensor, ep
     total_norm: a float32 scalar on their device (e.g. combined over the ranks that each
     hold a part of the parameters: the root of the sum of their squared norms)."""
     tensors = _list(tensors)
-    words, count, device = _table(tensors)
+    words, count, device, _ = _table(tensors)
     if count == 0:
         return
     if total_norm.dtype != torch.float32 or total_norm.numel() != 1 or total_norm.device != device:
@@ -100,11 +106,11 @@ def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6, error_if_non
         if grads:
             clip_grads_with_norm_(grads, max_norm, norm, eps)
         return norm
-    words, count, device = _table(grads)
+    words, count, device, total = _table(grads)
     if count == 0:
         return torch.zeros(())
     norm = torch.empty((), dtype=torch.float32, device=device)
-    small = count <= L.CLIP_SMALL_TENSORS and sum(g.nbytes for g in grads) <= L.CLIP_SMALL_BYTES
+    small = count <= L.CLIP_SMALL_TENSORS and total <= L.CLIP_SMALL_BYTES
     nbytes = 0 if small else _scratch_bytes()
     hold, scratch = scratch_for(nbytes, device)
     launch(device, "tcc_clip_grad_norm", words.buffer_info()[0], count, max_norm, eps, norm.data_ptr(), scratch,

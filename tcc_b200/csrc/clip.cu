@@ -29,8 +29,9 @@ constexpr int kOneThreads = 1024, kTeam = 128;
 constexpr uint32_t kOneChunkBytes = 8192;
 constexpr uint32_t kMaxBlocks = 148 * 8;
 
-// Tensors of a launch over few of them, whose parameters are short, and of another.
-constexpr int kSmall = TCC_CLIP_SMALL_TENSORS, kLarge = 480;
+// Tensors of a launch: over few of them its parameters are short (0.7, 2.7 and
+// 10 KB).
+constexpr int kSmall = TCC_CLIP_SMALL_TENSORS, kMiddle = 128, kLarge = 480;
 
 // K tensors of one launch; chunk i of the launch belongs to the tensor t with
 // first[t] <= i < first[t + 1].
@@ -265,21 +266,19 @@ void check_tensors(const tcc_tensor* t, uint32_t count, bool written) {
 }
 
 // fn(table) for each launch's tensors.
+template <int K, typename Fn>
+void each_launch_of(const tcc_tensor* t, uint32_t count, Fn&& fn) {
+    TensorTable<K> tab;
+    for (uint32_t at = 0; at < count;) {
+        at = fill<K>(t, count, at, tab);
+        if (tab.count) fn(tab);
+    }
+}
 template <typename Fn>
 void each_launch(const tcc_tensor* t, uint32_t count, Fn&& fn) {
-    if (count <= (uint32_t)kSmall) {
-        TensorTable<kSmall> tab;
-        for (uint32_t at = 0; at < count;) {
-            at = fill<kSmall>(t, count, at, tab);
-            if (tab.count) fn(tab);
-        }
-    } else {
-        TensorTable<kLarge> tab;
-        for (uint32_t at = 0; at < count;) {
-            at = fill<kLarge>(t, count, at, tab);
-            if (tab.count) fn(tab);
-        }
-    }
+    if (count <= (uint32_t)kSmall) each_launch_of<kSmall>(t, count, fn);
+    else if (count <= (uint32_t)kMiddle) each_launch_of<kMiddle>(t, count, fn);
+    else each_launch_of<kLarge>(t, count, fn);
 }
 
 template <int K>

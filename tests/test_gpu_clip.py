@@ -58,7 +58,7 @@ def test_sizes_and_types(gpu, dtypes, shapes):
 
 
 # one table of tensors to a launch, the next size of table, several launches
-@pytest.mark.parametrize("count", [32, 33, 480, 481, 1500])
+@pytest.mark.parametrize("count", [32, 33, 128, 129, 480, 481, 1500])
 def test_many_tensors(gpu, count):
     shapes = [((i * 37) % 211,) for i in range(count)]
     _check_clip(_params(shapes, (F32, BF16), count), 2.0)
@@ -208,3 +208,11 @@ def test_limit_of_the_one_launch_form(gpu):
     """One byte range and one tensor more than what one launch takes."""
     for shapes in ([(49152,)], [(49152,), (1,)], [(1536,)] * 32, [(1489,)] * 33):
         _check_clip(_params(shapes, (F32,), 11), 1.0)
+
+
+def test_inference_tensors(gpu):
+    with torch.inference_mode():
+        g = torch.full((100,), 2.0, device="cuda")
+    total = torch.full((), 20.0, device="cuda")
+    K.clip_grads_with_norm_([g], 5.0, total)
+    assert bool(((g - 0.5).abs() < 1e-6).all())
