@@ -1,5 +1,5 @@
 // train_ops.cuh -- host interface of the training operators beside the
-// aggregation: embedding.cu, group_norm.cu, clip.cu.
+// aggregation: embedding.cu, group_norm.cu(h), clip.cu.
 #pragma once
 
 #include "common.cuh"
