@@ -415,6 +415,21 @@ ZeroRows rows_to_zero(const EmbeddingArgs& a) {
     return z;
 }
 
+// Words of the table's gradient that become zero beside a kernel of the sort,
+// which leaves the memory idle: CTAs of its own, after the kernel's.
+struct EarlyZero {
+    uint4* at;
+    uint64_t words;
+    uint32_t ctas;
+};
+
+__device__ __forceinline__ void zero_words(const EarlyZero& z, uint32_t cta) {
+    const uint64_t step = (uint64_t)z.ctas * blockDim.x;
+#pragma unroll 4
+    for (uint64_t i = (uint64_t)cta * blockDim.x + threadIdx.x; i < z.words; i += step)
+        __stcs(z.at + i, make_uint4(0, 0, 0, 0));
+}
+
 // ------------------------------------------------------------ owner form --
 
 // Indices of the owner form, at most: 1,000 spread ones take 7 us, in the sorted
@@ -716,7 +731,9 @@ size_t cluster_smem(uint32_t each, uint32_t digits) {
 
 template <int BITS>
 __global__ void __launch_bounds__(kSortThreads) cluster_sort_kernel(const IndexSource src, uint32_t n, uint32_t each,
-                                                                    int passes, Entry* __restrict__ out) {
+                                                                    int passes, Entry* __restrict__ out,
+                                                                    const EarlyZero zero) {
+    if (blockIdx.x >= kCluster) return zero_words(zero, blockIdx.x - kCluster);  // whole clusters
     extern __shared__ uint4 smem[];
     __shared__ uint32_t warp_sums[kSortWarps];
     cg::cluster_group cluster = cg::this_cluster();
@@ -871,6 +888,7 @@ __device__ __forceinline__ void fill_range(const Entry* __restrict__ entries, ui
 struct SortedShape {
     uint32_t per, range, sums;  // entries of a team, of a CTA; CTAs
     uint32_t fill_rows, fills;  // table rows of a CTA that fills; CTAs
+    uint32_t zeroed;            // rows that are zero already
 };
 
 template <typename TG, typename TT, int V>
@@ -884,8 +902,9 @@ __global__ void __launch_bounds__(kThreads) grad_sorted_kernel(
         static_assert(kFillRows <= sizeof(Ring<TG, V>), "flags fit");
         // the CTAs of the other columns take their share of the rows
         const uint32_t share = (so.fill_rows + gridDim.y - 1) / gridDim.y;
-        const uint32_t r0 = blockIdx.x * so.fill_rows + min(blockIdx.y * share, so.fill_rows);
-        const uint32_t r1 = min(min(r0 + share, (blockIdx.x + 1) * so.fill_rows), num_rows);
+        const uint32_t f0 = so.zeroed + blockIdx.x * so.fill_rows;
+        const uint32_t r0 = f0 + min(blockIdx.y * share, so.fill_rows);
+        const uint32_t r1 = min(min(r0 + share, f0 + so.fill_rows), num_rows);
         if (r0 < r1) fill_range(entries, n, r0, r1, zero, reinterpret_cast<uint8_t*>(smem), bounds);
         return;
     }
@@ -978,7 +997,7 @@ SortPlan sort_plan(uint64_t n, uint64_t num_rows) {
 // Entries of a team: about 16 CTAs per SM over the whole list (ranges long
 // enough that few runs cross), at least 16; of a CTA at most 1024.
 constexpr uint32_t kRangeMax = 1024;
-SortedShape sorted_shape(uint64_t n, uint64_t num_rows, const TeamShape& sh) {
+SortedShape sorted_shape(uint64_t n, uint64_t num_rows, const TeamShape& sh, uint64_t zeroed = 0) {
     SortedShape so;
     const uint64_t per = (n / (148 * 16) + sh.teams - 1) / sh.teams;
     so.per = (uint32_t)std::min<uint64_t>(kRangeMax / sh.teams, std::max<uint64_t>(16, per));
@@ -986,7 +1005,8 @@ SortedShape sorted_shape(uint64_t n, uint64_t num_rows, const TeamShape& sh) {
     so.sums = ceil_div(n, so.range);
     // about four such CTAs per SM, so that a small table's rows are spread too
     so.fill_rows = (uint32_t)std::min<uint64_t>(kFillRows, std::max<uint64_t>(16, num_rows / (148 * 4)));
-    so.fills = ceil_div(num_rows, so.fill_rows);
+    so.fills = ceil_div(num_rows - zeroed, so.fill_rows);
+    so.zeroed = (uint32_t)zeroed;
     return so;
 }
 
@@ -1029,14 +1049,27 @@ GradScratch lay_out(uint64_t n, uint64_t num_rows, uint32_t F, char* base) {
     return g;
 }
 
+// Rows that become zero beside the cluster's sort, which leaves most SMs idle:
+// about what is written in its time (more delays the sums: all 537 MB of 1 M x 128
+// first take 167 us for 65,536 indices, none 161, these 136; for 2,049 157, 132
+// and 107).  Beside the tiles' kernels the stores slow the sort by more than they
+// save (1 M indices: 277 to 300 us in place of 261).
+uint64_t early_rows(const EmbeddingArgs& a) {
+    if (a.n > kClusterMax || a.ldt != a.F || (uintptr_t)a.table % 16) return 0;
+    const uint64_t most = 80000000 + 2000 * a.n;
+    return std::min<uint64_t>(a.num_rows, most / (a.F * type_bytes(a.table_type))) & ~7ull;  // of whole words
+}
+
 template <int BITS>
 const Entry* sort_by_cluster(const IndexSource& src, uint32_t n, const SortPlan& p, const GradScratch& g,
-                             cudaStream_t s) {
+                             EarlyZero zero, cudaStream_t s) {
     const uint32_t each = (n + kCluster - 1) / kCluster;
     static std::atomic<uint64_t> done{0};
     allow_smem(cluster_sort_kernel<BITS>, cluster_smem(kHeld, p.digits), done);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(kCluster);
+    // two CTAs per SM beside the sort's, and only as many as find work
+    zero.ctas = (uint32_t)std::min<uint64_t>(33, (zero.words + 8191) / 8192) * kCluster;
+    cfg.gridDim = dim3(kCluster + zero.ctas);
     cfg.blockDim = dim3(kSortThreads);
     cfg.dynamicSmemBytes = cluster_smem(each, p.digits);
     cfg.stream = s;
@@ -1046,7 +1079,7 @@ const Entry* sort_by_cluster(const IndexSource& src, uint32_t n, const SortPlan&
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     cfg.attrs = &cluster;
     cfg.numAttrs = 1;
-    TCC_CUDA(cudaLaunchKernelEx(&cfg, cluster_sort_kernel<BITS>, src, n, each, p.passes, g.a));
+    TCC_CUDA(cudaLaunchKernelEx(&cfg, cluster_sort_kernel<BITS>, src, n, each, p.passes, g.a, zero));
     return g.a;
 }
 
@@ -1081,8 +1114,9 @@ const Entry* sort_by_tiles(const IndexSource& src, uint32_t n, const SortPlan& p
 }
 
 template <int BITS>
-const Entry* sort_entries(const IndexSource& src, uint32_t n, const SortPlan& p, const GradScratch& g, cudaStream_t s) {
-    return n <= kClusterMax ? sort_by_cluster<BITS>(src, n, p, g, s) : sort_by_tiles<BITS>(src, n, p, g, s);
+const Entry* sort_entries(const IndexSource& src, uint32_t n, const SortPlan& p, const GradScratch& g,
+                          const EarlyZero& zero, cudaStream_t s) {
+    return n <= kClusterMax ? sort_by_cluster<BITS>(src, n, p, g, zero, s) : sort_by_tiles<BITS>(src, n, p, g, s);
 }
 
 template <typename TG, typename TT, int V>
@@ -1091,12 +1125,14 @@ void launch_sorted(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
     const GradScratch g = lay_out(n, num_rows, a.F, scratch);
     const SortPlan p = sort_plan(n, num_rows);
     const TeamShape sh = team_shape(a.F / V);
-    const SortedShape so = sorted_shape(n, num_rows, sh);
+    const uint64_t early = early_rows(a), row = a.F * type_bytes(a.table_type);
+    const EarlyZero zero{static_cast<uint4*>(a.table), early * row / 16, 0};
+    const SortedShape so = sorted_shape(n, num_rows, sh, early);
     const IndexSource from_idx{a.idx, a.idx_type, a.padding, num_rows, a.bad};
-    const Entry* in = p.bits == 8    ? sort_entries<8>(from_idx, n, p, g, s)
-                      : p.bits == 9  ? sort_entries<9>(from_idx, n, p, g, s)
-                      : p.bits == 10 ? sort_entries<10>(from_idx, n, p, g, s)
-                                     : sort_entries<11>(from_idx, n, p, g, s);
+    const Entry* in = p.bits == 8    ? sort_entries<8>(from_idx, n, p, g, zero, s)
+                      : p.bits == 9  ? sort_entries<9>(from_idx, n, p, g, zero, s)
+                      : p.bits == 10 ? sort_entries<10>(from_idx, n, p, g, zero, s)
+                                     : sort_entries<11>(from_idx, n, p, g, zero, s);
     static std::atomic<uint64_t> sums_done{0};
     const size_t sum_smem = sizeof(Ring<TG, V>) + (so.range + 2) * sizeof(Entry);
     allow_smem(grad_sorted_kernel<TG, TT, V>, sizeof(Ring<TG, V>) + (kRangeMax + 2) * sizeof(Entry), sums_done);

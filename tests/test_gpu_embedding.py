@@ -174,6 +174,25 @@ def test_gradient_leaves_columns_beyond_the_width(gpu):
         assert bool((out[:, 10:] == 7.0).all())
 
 
+@pytest.mark.parametrize("rows,width,dtype", [(300007, 100, F32), (13, 3, BF16), (60001, 5, F16), (1, 1, F32)])
+@pytest.mark.parametrize("n", [1025, 9001, 65537])
+def test_gradient_covers_every_row_and_no_more(gpu, rows, width, dtype, n):
+    """Rows without an index are written wherever the zeroing beside the sort ends; what lies behind the table stays."""
+    gen = _gen(rows + n)
+    idx = torch.randint(rows, (n,), generator=gen, device="cuda")
+    grad = torch.randn((n, width), generator=gen, device="cuda").to(dtype)
+    out = torch.full((rows * width + 8,), float("nan"), device="cuda", dtype=dtype)
+    out[rows * width:] = 7.0
+    nbytes = L.lib().tcc_embedding_backward_scratch_bytes(n, rows, width)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    code = {F32: L.F32, F16: L.F16, BF16: L.BF16}[dtype]
+    L.call("tcc_embedding_backward", grad.data_ptr(), code, width, idx.data_ptr(), L.I64, n, L.NO_PADDING, 1.0,
+           out.data_ptr(), code, width, rows, width, scratch.data_ptr(), nbytes, None,
+           torch.cuda.current_stream().cuda_stream)
+    _check_grad(out[:rows * width].view(rows, width), grad, idx, 1.0, None)
+    assert bool((out[rows * width:] == 7.0).all())
+
+
 def test_empty(gpu):
     table = torch.randn((5, 4), device="cuda")
     none = torch.empty(0, dtype=torch.int64, device="cuda")
