@@ -132,7 +132,8 @@ __device__ __forceinline__ double squares_of(const Span& sp) {
 
 template <int K>
 __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ TensorTable<K> t,
-                                                           double* __restrict__ partial, bool add) {
+                                                           double* partial, bool add) {
+    after_previous();
     double s = 0.0;
     const uint32_t chunks = t.first[t.count];
     for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
@@ -143,14 +144,14 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
     if (threadIdx.x == 0) partial[blockIdx.x] = add ? partial[blockIdx.x] + s : s;
 }
 
-__device__ __forceinline__ float norm_of(const double* __restrict__ partial, uint32_t blocks) {
+__device__ __forceinline__ float norm_of(const double* partial, uint32_t blocks) {
     double s = 0.0;
     for (uint32_t i = threadIdx.x; i < blocks; i += kThreads) s += partial[i];
     return (float)sqrt(block_sum<kThreads>(s));
 }
 
-__global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ partial, uint32_t blocks,
-                                                        float* __restrict__ norm) {
+__global__ void __launch_bounds__(kThreads) norm_kernel(const double* partial, uint32_t blocks, float* norm) {
+    after_previous();
     const float n = norm_of(partial, blocks);
     if (threadIdx.x == 0) *norm = n;
 }
@@ -191,9 +192,10 @@ __device__ __forceinline__ void scale_by(const Span& sp, float f) {
 // last is still in L2.  partial == NULL: the norm is read from norm_in.
 template <int K>
 __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ TensorTable<K> t,
-                                                         const double* __restrict__ partial, uint32_t blocks,
+                                                         const double* partial, uint32_t blocks,
                                                          const float* norm_in, float* norm_out, float max_norm,
                                                          float eps) {
+    after_previous();
     const float norm = partial ? norm_of(partial, blocks) : *norm_in;
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
     const float f = max_norm / (norm + eps);
@@ -283,8 +285,12 @@ void each_launch(const tcc_tensor* t, uint32_t count, Fn&& fn) {
 
 template <int K>
 void launch_squares(const TensorTable<K>& tab, double* partial, unsigned blocks, bool add, cudaStream_t s) {
-    squares_kernel<K><<<blocks, kThreads, 0, s>>>(tab, partial, add);
-    TCC_CUDA(cudaGetLastError());
+    if (add) {
+        launch_after(squares_kernel<K>, blocks, kThreads, 0, s, tab, partial, add);
+    } else {
+        squares_kernel<K><<<blocks, kThreads, 0, s>>>(tab, partial, add);
+        TCC_CUDA(cudaGetLastError());
+    }
 }
 
 // Partial sums of every tensor; returns how many there are.
@@ -310,12 +316,17 @@ double* partials(void* scratch, size_t scratch_bytes) {
     return static_cast<double*>(scratch);
 }
 
+template <int K>
+void scale_after(const TensorTable<K>& tab, unsigned grid, const double* partial, uint32_t blocks,
+                 const float* norm_in, float* norm_out, float max_norm, float eps, cudaStream_t s) {
+    launch_after(scale_kernel<K>, grid, kThreads, 0, s, tab, partial, blocks, norm_in, norm_out, max_norm, eps);
+}
+
 void scale(const tcc_tensor* t, uint32_t count, const double* partial, uint32_t blocks, const float* norm_in,
            float* norm_out, float max_norm, float eps, cudaStream_t s) {
     each_launch(t, count, [&](const auto& tab) {
         const unsigned grid = std::min(tab.first[tab.count], kMaxBlocks);
-        scale_kernel<<<grid, kThreads, 0, s>>>(tab, partial, blocks, norm_in, norm_out, max_norm, eps);
-        TCC_CUDA(cudaGetLastError());
+        scale_after(tab, grid, partial, blocks, norm_in, norm_out, max_norm, eps, s);
     });
 }
 
@@ -334,8 +345,7 @@ void grad_norm(const tcc_tensor* t, uint32_t count, float* norm, void* scratch, 
     TCC_REQUIRE(norm, "norm must not be NULL");
     double* partial = partials(scratch, scratch_bytes);
     const uint32_t blocks = squares(t, count, partial, s);
-    norm_kernel<<<1, kThreads, 0, s>>>(partial, blocks, norm);
-    TCC_CUDA(cudaGetLastError());
+    launch_after(norm_kernel, 1, kThreads, 0, s, partial, blocks, norm);
 }
 
 void clip_grads_with_norm(const tcc_tensor* t, uint32_t count, const float* norm, float max_norm, float eps,

@@ -121,6 +121,30 @@ __device__ __forceinline__ void wait_copies() {
     asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 
+// Kernels of one call that follow each other: launch_after lets the next one's
+// CTAs take their places once the previous kernel's have all begun, and
+// after_previous, first in each such kernel, holds them until that kernel is
+// through and what it wrote can be seen.  What it wrote is read by plain loads
+// (no __restrict__, no __ldg), which the compiler moves past no such wait.
+__device__ __forceinline__ void after_previous() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... P, typename... A>
+void launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    TCC_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+}
+
 // The widest V (of 8, 4, 2, 1; V * bytes <= 16) that divides every count in
 // `counts` and keeps every pointer aligned to V elements of its own size.
 struct VecRule {

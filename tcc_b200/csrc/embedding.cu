@@ -549,6 +549,7 @@ constexpr int kMinDigitBits = 8, kMaxDigitBits = 11;
 constexpr uint32_t kMaxDigits = 1u << kMaxDigitBits;
 
 struct IndexSource {  // pass 0: the indices themselves; rows without a gradient sort last
+    static constexpr bool kGiven = true;  // before the call's first kernel
     const void* idx;
     int type;
     int64_t padding;
@@ -565,6 +566,7 @@ struct IndexSource {  // pass 0: the indices themselves; rows without a gradient
 };
 
 struct EntrySource {
+    static constexpr bool kGiven = false;
     const Entry* entries;
     __device__ __forceinline__ Entry load(uint32_t i) const { return entries[i]; }
     __device__ __forceinline__ void note(uint32_t, Entry) const {}
@@ -575,6 +577,7 @@ template <typename Source>
 __global__ void __launch_bounds__(kSortThreads) digit_counts_kernel(const Source src, uint32_t n, int shift,
                                                                     uint32_t digits, uint32_t* __restrict__ counts,
                                                                     uint32_t* __restrict__ totals) {
+    after_previous();
     __shared__ uint32_t hist[kMaxDigits];
     for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) hist[d] = 0;
     const uint32_t base = blockIdx.x * kTile + threadIdx.x;
@@ -598,8 +601,9 @@ __global__ void __launch_bounds__(kSortThreads) digit_counts_kernel(const Source
 
 // counts -> where a tile's first entry of each digit goes.  A CTA takes 32
 // digits; 32 rows of threads share the tiles.
-__global__ void __launch_bounds__(1024) digit_offsets_kernel(uint32_t* __restrict__ counts, uint32_t tiles,
-                                                             uint32_t digits, const uint32_t* __restrict__ totals) {
+__global__ void __launch_bounds__(1024) digit_offsets_kernel(uint32_t* counts, uint32_t tiles, uint32_t digits,
+                                                             const uint32_t* totals) {
+    after_previous();
     __shared__ uint32_t part[32][33];
     __shared__ uint32_t below[32];
     const uint32_t lane = threadIdx.x & 31, row = threadIdx.x >> 5;
@@ -663,8 +667,8 @@ __device__ __forceinline__ unsigned same_digit(uint32_t d, bool in) {
 // own digit counts; a prefix over the warps puts them in order.
 template <typename Source, int BITS>
 __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const Source src, uint32_t n, int shift,
-                                                                     const uint32_t* __restrict__ offsets,
-                                                                     Entry* __restrict__ out) {
+                                                                     const uint32_t* offsets, Entry* out) {
+    if constexpr (!Source::kGiven) after_previous();
     constexpr uint32_t digits = 1u << BITS;
     extern __shared__ uint4 smem[];
     uint16_t* all = reinterpret_cast<uint16_t*>(smem);  // [kSortWarps][digits]
@@ -704,10 +708,11 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const Sourc
             run += c;
         }
     }
+    if constexpr (Source::kGiven) after_previous();  // the ranks took the indices alone
     const uint32_t* offset = offsets + (uint64_t)blockIdx.x * digits;
     uint32_t start[kTileEach];
 #pragma unroll
-    for (int k = 0; k < kTileEach; ++k) start[k] = base + k * 32 < n ? __ldg(offset + (place[k] >> 16)) : 0;
+    for (int k = 0; k < kTileEach; ++k) start[k] = base + k * 32 < n ? offset[place[k] >> 16] : 0;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kTileEach; ++k)
@@ -733,6 +738,7 @@ template <int BITS>
 __global__ void __launch_bounds__(kSortThreads) cluster_sort_kernel(const IndexSource src, uint32_t n, uint32_t each,
                                                                     int passes, Entry* __restrict__ out,
                                                                     const EarlyZero zero) {
+    after_previous();
     if (blockIdx.x >= kCluster) return zero_words(zero, blockIdx.x - kCluster);  // whole clusters
     extern __shared__ uint4 smem[];
     __shared__ uint32_t warp_sums[kSortWarps];
@@ -865,7 +871,7 @@ __device__ __forceinline__ uint32_t first_of(const Entry* entries, uint32_t lo, 
     return lo;
 }
 
-__device__ __forceinline__ void fill_range(const Entry* __restrict__ entries, uint32_t n, uint32_t r0, uint32_t r1,
+__device__ __forceinline__ void fill_range(const Entry* entries, uint32_t n, uint32_t r0, uint32_t r1,
                                            const ZeroRows& zero, uint8_t* touched, uint32_t* bounds) {
     if (threadIdx.x < 2) bounds[threadIdx.x] = first_of(entries, 0, n, threadIdx.x ? r1 : r0);
     for (uint32_t i = threadIdx.x; i < r1 - r0; i += kThreads) touched[i] = 0;
@@ -893,9 +899,10 @@ struct SortedShape {
 
 template <typename TG, typename TT, int V>
 __global__ void __launch_bounds__(kThreads) grad_sorted_kernel(
-    const TG* __restrict__ grad, uint32_t grad_stride, const Entry* __restrict__ entries, uint32_t n, float scale,
-    TT* __restrict__ dtable, uint64_t ldt, uint32_t num_rows, const TeamShape sh, const SortedShape so,
-    const ZeroRows zero, float* __restrict__ heads, float* __restrict__ tails, Border* __restrict__ borders) {
+    const TG* __restrict__ grad, uint32_t grad_stride, const Entry* entries, uint32_t n, float scale, TT* dtable,
+    uint64_t ldt, uint32_t num_rows, const TeamShape sh, const SortedShape so, const ZeroRows zero, float* heads,
+    float* tails, Border* borders) {
+    after_previous();
     extern __shared__ uint4 smem[];
     if (blockIdx.x < so.fills) {
         __shared__ uint32_t bounds[2];
@@ -923,11 +930,10 @@ __global__ void __launch_bounds__(kThreads) grad_sorted_kernel(
 // The threads are columns (of W floats) times groups; a group adds a contiguous
 // part of the ranges, and the groups' sums are added in order.
 template <typename TT, int W>
-__global__ void __launch_bounds__(kThreads) grad_join_kernel(const Border* __restrict__ borders, uint32_t sums,
-                                                             const float* __restrict__ heads,
-                                                             const float* __restrict__ tails, uint32_t width,
-                                                             float scale, TT* __restrict__ dtable, uint64_t ldt,
-                                                             uint32_t num_rows) {
+__global__ void __launch_bounds__(kThreads) grad_join_kernel(const Border* borders, uint32_t sums, const float* heads,
+                                                             const float* tails, uint32_t width, float scale,
+                                                             TT* dtable, uint64_t ldt, uint32_t num_rows) {
+    after_previous();
     const Border b = borders[blockIdx.x];
     if (!(b.flags & kTail) || b.row >= num_rows) return;
     // the ranges after it that hold a part: up to the first that is not passed through
@@ -1100,13 +1106,15 @@ const Entry* sort_by_tiles(const IndexSource& src, uint32_t n, const SortPlan& p
         if (pass == 0)
             digit_counts_kernel<<<p.tiles, kSortThreads, 0, s>>>(src, n, shift, p.digits, g.counts, totals);
         else
-            digit_counts_kernel<<<p.tiles, kSortThreads, 0, s>>>(from_entries, n, shift, p.digits, g.counts, totals);
-        digit_offsets_kernel<<<ceil_div(p.digits, 32), 1024, 0, s>>>(g.counts, p.tiles, p.digits, totals);
+            launch_after(digit_counts_kernel<EntrySource>, p.tiles, kSortThreads, 0, s, from_entries, n, shift,
+                         p.digits, g.counts, totals);
+        launch_after(digit_offsets_kernel, ceil_div(p.digits, 32), 1024, 0, s, g.counts, p.tiles, p.digits, totals);
         if (pass == 0)
-            digit_scatter_kernel<IndexSource, BITS><<<p.tiles, kSortThreads, smem, s>>>(src, n, shift, g.counts, out);
+            launch_after(digit_scatter_kernel<IndexSource, BITS>, p.tiles, kSortThreads, smem, s, src, n, shift,
+                         g.counts, out);
         else
-            digit_scatter_kernel<EntrySource, BITS>
-                <<<p.tiles, kSortThreads, smem, s>>>(from_entries, n, shift, g.counts, out);
+            launch_after(digit_scatter_kernel<EntrySource, BITS>, p.tiles, kSortThreads, smem, s, from_entries, n,
+                         shift, g.counts, out);
         std::swap(in, out);
     }
     TCC_CUDA(cudaGetLastError());
@@ -1136,13 +1144,13 @@ void launch_sorted(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
     static std::atomic<uint64_t> sums_done{0};
     const size_t sum_smem = sizeof(Ring<TG, V>) + (so.range + 2) * sizeof(Entry);
     allow_smem(grad_sorted_kernel<TG, TT, V>, sizeof(Ring<TG, V>) + (kRangeMax + 2) * sizeof(Entry), sums_done);
-    grad_sorted_kernel<TG, TT, V><<<dim3(so.fills + so.sums, sh.blocks), kThreads, sum_smem, s>>>(
-        static_cast<const TG*>(a.rows), (uint32_t)(a.ldr * sizeof(TG)), in, n, a.scale, static_cast<TT*>(a.table),
-        a.ldt, num_rows, sh, so, rows_to_zero(a), g.heads, g.tails, g.borders);
+    launch_after(grad_sorted_kernel<TG, TT, V>, dim3(so.fills + so.sums, sh.blocks), kThreads, sum_smem, s,
+                 static_cast<const TG*>(a.rows), (uint32_t)(a.ldr * sizeof(TG)), in, n, a.scale,
+                 static_cast<TT*>(a.table), a.ldt, num_rows, sh, so, rows_to_zero(a), g.heads, g.tails, g.borders);
     if (so.sums > 1) {
         auto join = a.F % 4 ? grad_join_kernel<TT, 1> : grad_join_kernel<TT, 4>;
-        join<<<so.sums, kThreads, 0, s>>>(g.borders, so.sums, g.heads, g.tails, a.F, a.scale,
-                                          static_cast<TT*>(a.table), a.ldt, num_rows);
+        launch_after(join, so.sums, kThreads, 0, s, g.borders, so.sums, g.heads, g.tails, a.F, a.scale,
+                     static_cast<TT*>(a.table), a.ldt, num_rows);
     }
     TCC_CUDA(cudaGetLastError());
 }

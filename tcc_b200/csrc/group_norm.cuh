@@ -420,6 +420,7 @@ __global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormA
 template <typename T, int V, int J>
 __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1) rows_backward_kernel(const GroupNormArgs a, const RowsShape sh,
                                                                  float* __restrict__ partial) {
+    after_previous();
     using Ring = RowsRing<T, V, J, 2>;
     extern __shared__ uint4 smem[];
     Ring& ring = *reinterpret_cast<Ring*>(smem);
@@ -584,8 +585,9 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
 
 // dweight, dbias [C] = column sums of partial [rows][2][C], in 64 bits; a CTA
 // takes 8 columns (a sector of a row) by 128 rows of threads.
-__global__ void __launch_bounds__(1024) param_grad_kernel(const float* __restrict__ partial, uint64_t rows,
-                                                          uint32_t C, void* dweight, void* dbias, int type) {
+__global__ void __launch_bounds__(1024) param_grad_kernel(const float* partial, uint64_t rows, uint32_t C,
+                                                          void* dweight, void* dbias, int type) {
+    after_previous();
     __shared__ double sm[32][8];
     const uint32_t tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
     const uint64_t c = (uint64_t)blockIdx.x * 8 + tx;  // of 2 C
@@ -604,6 +606,11 @@ __global__ void __launch_bounds__(1024) param_grad_kernel(const float* __restric
         void* out = c < C ? dweight : dbias;
         if (out) store_typed(out, type, c < C ? c : c - C, (float)t);
     }
+}
+
+inline void launch_param_grad(const GroupNormArgs& a, const float* partial, uint64_t rows, cudaStream_t s) {
+    launch_after(param_grad_kernel, (2 * a.C + 7) / 8, 1024, 0, s, partial, rows, a.C, a.dweight, a.dbias,
+                 a.param_type);
 }
 
 // ------------------------------------------------------------ split form --
@@ -787,7 +794,8 @@ __device__ __forceinline__ void block_moments(const SplitPlace& p, const SplitSh
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 3) split_moments_kernel(const GroupNormArgs a, const SplitShape sh,
-                                                                 Moments* __restrict__ partial) {
+                                                                    Moments* __restrict__ partial) {
+    after_previous();
     extern __shared__ uint4 smem[];
     const SplitPlace p = split_place<V>(a, sh, false);
     const T* const from[1] = {static_cast<const T*>(a.x) + (p.n * a.S + p.row0 + p.rb) * a.ldx + p.c};
@@ -803,8 +811,9 @@ __global__ void __launch_bounds__(kThreads, 3) split_moments_kernel(const GroupN
 }
 
 // A CTA of one or eight warps per (sample, group) merges its partial moments.
-__global__ void split_stats_kernel(const Moments* __restrict__ partial, uint32_t G, uint32_t SUB, uint32_t chunks,
-                                   float eps, float* __restrict__ mean, float* __restrict__ rstd) {
+__global__ void split_stats_kernel(const Moments* partial, uint32_t G, uint32_t SUB, uint32_t chunks, float eps, float* mean,
+                                   float* rstd) {
+    after_previous();
     __shared__ Moments sm[8];
     const uint64_t n = blockIdx.x / G;
     const uint32_t g = (uint32_t)(blockIdx.x - n * G);
@@ -831,8 +840,8 @@ __global__ void split_stats_kernel(const Moments* __restrict__ partial, uint32_t
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) split_apply_kernel(const GroupNormArgs a, const SplitShape sh,
-                                                               const float* __restrict__ mean_,
-                                                               const float* __restrict__ rstd_) {
+                                                               const float* mean_, const float* rstd_) {
+    after_previous();
     extern __shared__ uint4 smem[];
     const SplitPlace p = split_place<V>(a, sh, true);
     const uint32_t count = own_rows(p, sh);
@@ -854,7 +863,8 @@ __global__ void __launch_bounds__(kThreads) split_apply_kernel(const GroupNormAr
 // Per chunk and channel: sums of dz * h and of dz -> partial [N][chunks][2][C].
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 3) split_sums_kernel(const GroupNormArgs a, const SplitShape sh,
-                                                              float* __restrict__ partial) {
+                                                                 float* __restrict__ partial) {
+    after_previous();
     const SplitPlace p = split_place<V>(a, sh, false);
     extern __shared__ uint4 smem[];
     Vec<V> dw = splat<V>(0.f), db = dw;
@@ -899,8 +909,9 @@ __global__ void __launch_bounds__(kThreads, 3) split_sums_kernel(const GroupNorm
 // dz * h), from the chunks' sums; a CTA per (sample, group), `cw` channels at a
 // time (a power of two up to a warp) by blockDim.x / cw threads over the
 // chunks.  With one sample the channels' sums are the parameters' gradients.
-__global__ void split_groups_kernel(const GroupNormArgs a, const float* __restrict__ partial, uint32_t chunks,
-                                    uint32_t cw, float* __restrict__ group_sums, bool params) {
+__global__ void split_groups_kernel(const GroupNormArgs a, const float* partial, uint32_t chunks, uint32_t cw,
+                                    float* group_sums, bool params) {
+    after_previous();
     __shared__ double sm[2][32][32];
     const uint64_t n = blockIdx.x / a.G;
     const uint32_t g = (uint32_t)(blockIdx.x - n * a.G), Cg = a.C / a.G;
@@ -954,7 +965,8 @@ __global__ void split_groups_kernel(const GroupNormArgs a, const float* __restri
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 3) split_grad_kernel(const GroupNormArgs a, const SplitShape sh,
-                                                              const float* __restrict__ group_sums) {
+                                                                 const float* group_sums) {
+    after_previous();
     extern __shared__ uint4 smem[];
     const SplitPlace p = split_place<V>(a, sh, true);
     const uint32_t count = own_rows(p, sh);
@@ -1061,6 +1073,7 @@ __global__ void __launch_bounds__(kThreads) resident_forward_kernel(const GroupN
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const GroupNormArgs a, const SplitShape sh,
                                                                      float* __restrict__ partial) {
+    after_previous();
     extern __shared__ uint4 smem[];
     float(*sums)[kThreads * V] = reinterpret_cast<float(*)[kThreads * V]>(
         reinterpret_cast<char*>(smem) + resident_store<V>(sh, sizeof(Pack<T, V>), 2));  // [2]: per thread, then channel
@@ -1299,9 +1312,7 @@ void rows_launch(const GroupNormArgs& a, float* partial, bool backward, cudaStre
     }
     TCC_CUDA(cudaGetLastError());
     if (backward && partial) {
-        param_grad_kernel<<<(2 * a.C + 7) / 8, 1024, 0, s>>>(partial, grid.x * (rows_fold(sh) ? 1 : a.S), a.C, a.dweight, a.dbias,
-                                                              a.param_type);
-        TCC_CUDA(cudaGetLastError());
+        launch_param_grad(a, partial, grid.x * (rows_fold(sh) ? 1 : a.S), s);
     }
 }
 
@@ -1333,8 +1344,7 @@ void resident_launch(const GroupNormArgs& a, const SplitShape& sh, float* partia
         allow_smem(resident_backward_kernel<T, V>, kResidentBytes, backward_done);
         TCC_CUDA(cudaLaunchKernelEx(&cfg, resident_backward_kernel<T, V>, a, sh, partial));
         if (partial)
-            param_grad_kernel<<<(2 * a.C + 7) / 8, 1024, 0, s>>>(partial, cfg.gridDim.x, a.C, a.dweight, a.dbias,
-                                                                a.param_type);
+            launch_param_grad(a, partial, cfg.gridDim.x, s);
     } else {
         allow_smem(resident_forward_kernel<T, V>, kResidentBytes, forward_done);
         TCC_CUDA(cudaLaunchKernelEx(&cfg, resident_forward_kernel<T, V>, a, sh));
@@ -1370,8 +1380,9 @@ void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStrea
             rstd = mean + align256(a.N * a.G * 4) / 4;
         }
         split_moments_kernel<T, V><<<grid, kThreads, ring1, s>>>(a, sh, partial);
-        split_stats_kernel<<<groups, many ? kThreads : 32, 0, s>>>(partial, a.G, sh.SUB, sh.chunks, a.eps, mean, rstd);
-        split_apply_kernel<T, V><<<grid, kThreads, ring1, s>>>(a, sh, mean, rstd);
+        launch_after(split_stats_kernel, groups, many ? kThreads : 32, 0, s, partial, a.G, sh.SUB, sh.chunks, a.eps,
+                     mean, rstd);
+        launch_after(split_apply_kernel<T, V>, grid, kThreads, ring1, s, a, sh, mean, rstd);
     } else {
         float* partial = reinterpret_cast<float*>(scratch);
         float* group_sums = partial + align256(a.N * sh.chunks * 2 * a.C * 4) / 4;
@@ -1380,12 +1391,12 @@ void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStrea
         if (a.dx || one) {
             uint32_t cw = 1;
             while (cw < 32 && cw < a.C / a.G) cw <<= 1;
-            split_groups_kernel<<<groups, many ? 1024 : 128, 0, s>>>(a, partial, sh.chunks, cw, group_sums, one);
+            launch_after(split_groups_kernel, groups, many ? 1024 : 128, 0, s, a, partial, sh.chunks, cw, group_sums,
+                         one);
         }
-        if (a.dx) split_grad_kernel<T, V><<<grid, kThreads, ring2, s>>>(a, sh, group_sums);
+        if (a.dx) launch_after(split_grad_kernel<T, V>, grid, kThreads, ring2, s, a, sh, group_sums);
         if (params && !one)
-            param_grad_kernel<<<(2 * a.C + 7) / 8, 1024, 0, s>>>(partial, a.N * sh.chunks, a.C, a.dweight, a.dbias,
-                                                                a.param_type);
+            launch_param_grad(a, partial, a.N * sh.chunks, s);
     }
     TCC_CUDA(cudaGetLastError());
 }

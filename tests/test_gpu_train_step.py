@@ -203,3 +203,62 @@ def test_captured_before_any_other_call(gpu):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", COLD], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_back_to_back_calls_give_what_they_give_alone(gpu, captured):
+    """Kernels of one call overlap where they may; calls that follow each other, in scratch that the
+    allocator hands on, do not see each other's: the same bits as with the device idle before each."""
+    gen = torch.Generator(device=gpu).manual_seed(57)
+
+    def rand(*shape, dtype=torch.float32):
+        return torch.randn(shape, generator=gen, device=gpu).to(dtype)
+
+    jobs = []
+    for n, rows, width, dtype in [(200003, 30011, 64, torch.float32), (5003, 70001, 100, torch.bfloat16),
+                                  (90001, 47, 96, torch.float32), (3001, 9, 33, torch.float16)]:
+        idx, grad = torch.randint(rows, (n,), generator=gen, device=gpu), rand(n, width, dtype=dtype)
+        jobs.append(lambda idx=idx, grad=grad, rows=rows: (E.embedding_backward(grad, idx, rows),))
+    for shape, groups, act, dtype in [((1, 20011, 96), 6, "silu", torch.bfloat16), ((3, 9001, 64), 4, "gelu", torch.float32),
+                                      ((8, 517, 100), 10, "none", torch.float32), ((5003, 128), 8, "relu", torch.float16)]:
+        x, dy, w, b = rand(*shape, dtype=dtype), rand(*shape, dtype=dtype), rand(shape[-1]), rand(shape[-1])
+
+        def norm(x=x, dy=dy, w=w, b=b, groups=groups, act=act):
+            y, mean, rstd = N.group_norm_forward(x, groups, w, b, act=act)
+            return (y, mean, rstd, *N.group_norm_backward(dy, x, mean, rstd, groups, w, b, act=act))
+        jobs.append(norm)
+    for count in (40, 600):
+        grads = [rand(3001 + 7 * i) for i in range(count)]
+
+        def clipped(grads=grads):
+            copies = [g.clone() for g in grads]
+            norm = clip.grad_norm(copies)
+            clip.clip_grads_with_norm_(copies, 1.5, norm)
+            again = torch.nn.ParameterList([torch.nn.Parameter(c) for c in copies])
+            for p, g in zip(again, grads):
+                p.grad = g.clone()
+            return (norm, *copies, clip.clip_grad_norm_(list(again), 2.5), *[p.grad for p in again])
+        jobs.append(clipped)
+
+    def alone(job):
+        torch.cuda.synchronize()
+        out = job()
+        torch.cuda.synchronize()
+        return out
+    want = [alone(job) for job in jobs]
+
+    def all_of(times):
+        return [[job() for job in jobs] for _ in range(times)]
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = all_of(2)
+        for _ in range(3):
+            graph.replay()
+    else:
+        all_of(1)  # its memory is handed on
+        got = all_of(4)
+    torch.cuda.synchronize()
+    for outs in got:
+        for out, expect in zip(outs, want):
+            assert all(torch.equal(o, e) for o, e in zip(out, expect))
