@@ -721,14 +721,21 @@ __global__ void __launch_bounds__(kSortThreads) digit_scatter_kernel(const Sourc
 
 // The whole sort by one cluster of CTAs for up to kClusterMax entries: each CTA
 // holds `each` of them, ranks them by digit, and writes them to their places in
-// the CTAs' shared memory.  One launch in place of seven: the gradient of 2,049
-// indices takes 24 us in place of 62, most of it the host's; at 65,536 the sort
-// is bound by what eight SMs can do (42 us for two passes of 11 bits) and the
-// tiles of the larger form are as fast.
+// the CTAs' shared memory.  One launch in place of seven: the gradient of 8,193
+// indices in a table of 10,000 x 64 takes 26 us in place of 38, of 40,000 40
+// in place of 44, of 65,536 52 in place of 44: the sort is then bound by what
+// eight SMs can do.  From about 100 MB of table on it wins up to 65,536 all the
+// same, by what the other SMs zero meanwhile (1 M x 128: 136 in place of 140).
 constexpr uint32_t kCluster = 8;
 constexpr int kHeldEach = 16;  // entries of a thread
 constexpr uint32_t kHeld = kSortThreads * kHeldEach;
-constexpr uint32_t kClusterMax = kCluster * kHeld;
+constexpr uint32_t kClusterMax = kCluster * kHeld, kClusterSmall = 40960;
+constexpr uint64_t kClusterTable = 100000000;
+
+bool by_cluster(const EmbeddingArgs& a) {
+    return a.n <= kClusterSmall ||
+           (a.n <= kClusterMax && a.num_rows * a.F * type_bytes(a.table_type) >= kClusterTable);
+}
 
 size_t cluster_smem(uint32_t each, uint32_t digits) {
     return 2 * (size_t)each * sizeof(Entry) + (size_t)kSortWarps * digits * 2 + (size_t)digits * 12;
@@ -1057,11 +1064,11 @@ GradScratch lay_out(uint64_t n, uint64_t num_rows, uint32_t F, char* base) {
 
 // Rows that become zero beside the cluster's sort, which leaves most SMs idle:
 // about what is written in its time (more delays the sums: all 537 MB of 1 M x 128
-// first take 167 us for 65,536 indices, none 161, these 136; for 2,049 157, 132
+// first took 167 us for 65,536 indices, none 161, these 136; for 2,049 157, 132
 // and 107).  Beside the tiles' kernels the stores slow the sort by more than they
 // save (1 M indices: 277 to 300 us in place of 261).
 uint64_t early_rows(const EmbeddingArgs& a) {
-    if (a.n > kClusterMax || a.ldt != a.F || (uintptr_t)a.table % 16) return 0;
+    if (!by_cluster(a) || a.ldt != a.F || (uintptr_t)a.table % 16) return 0;
     const uint64_t most = 80000000 + 2000 * a.n;
     return std::min<uint64_t>(a.num_rows, most / (a.F * type_bytes(a.table_type))) & ~7ull;  // of whole words
 }
@@ -1123,8 +1130,8 @@ const Entry* sort_by_tiles(const IndexSource& src, uint32_t n, const SortPlan& p
 
 template <int BITS>
 const Entry* sort_entries(const IndexSource& src, uint32_t n, const SortPlan& p, const GradScratch& g,
-                          const EarlyZero& zero, cudaStream_t s) {
-    return n <= kClusterMax ? sort_by_cluster<BITS>(src, n, p, g, zero, s) : sort_by_tiles<BITS>(src, n, p, g, s);
+                          bool cluster, const EarlyZero& zero, cudaStream_t s) {
+    return cluster ? sort_by_cluster<BITS>(src, n, p, g, zero, s) : sort_by_tiles<BITS>(src, n, p, g, s);
 }
 
 template <typename TG, typename TT, int V>
@@ -1137,10 +1144,11 @@ void launch_sorted(const EmbeddingArgs& a, char* scratch, cudaStream_t s) {
     const EarlyZero zero{static_cast<uint4*>(a.table), early * row / 16, 0};
     const SortedShape so = sorted_shape(n, num_rows, sh, early);
     const IndexSource from_idx{a.idx, a.idx_type, a.padding, num_rows, a.bad};
-    const Entry* in = p.bits == 8    ? sort_entries<8>(from_idx, n, p, g, zero, s)
-                      : p.bits == 9  ? sort_entries<9>(from_idx, n, p, g, zero, s)
-                      : p.bits == 10 ? sort_entries<10>(from_idx, n, p, g, zero, s)
-                                     : sort_entries<11>(from_idx, n, p, g, zero, s);
+    const bool cluster = by_cluster(a);
+    const Entry* in = p.bits == 8    ? sort_entries<8>(from_idx, n, p, g, cluster, zero, s)
+                      : p.bits == 9  ? sort_entries<9>(from_idx, n, p, g, cluster, zero, s)
+                      : p.bits == 10 ? sort_entries<10>(from_idx, n, p, g, cluster, zero, s)
+                                     : sort_entries<11>(from_idx, n, p, g, cluster, zero, s);
     static std::atomic<uint64_t> sums_done{0};
     const size_t sum_smem = sizeof(Ring<TG, V>) + (so.range + 2) * sizeof(Entry);
     allow_smem(grad_sorted_kernel<TG, TT, V>, sizeof(Ring<TG, V>) + (kRangeMax + 2) * sizeof(Entry), sums_done);

@@ -175,7 +175,7 @@ def test_gradient_leaves_columns_beyond_the_width(gpu):
 
 
 @pytest.mark.parametrize("rows,width,dtype", [(300007, 100, F32), (13, 3, BF16), (60001, 5, F16), (1, 1, F32)])
-@pytest.mark.parametrize("n", [1025, 9001, 65537])
+@pytest.mark.parametrize("n", [1025, 9001, 40961, 65536, 65537])
 def test_gradient_covers_every_row_and_no_more(gpu, rows, width, dtype, n):
     """Rows without an index are written wherever the zeroing beside the sort ends; what lies behind the table stays."""
     gen = _gen(rows + n)
