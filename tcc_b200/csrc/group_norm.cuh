@@ -678,7 +678,7 @@ struct Moments {
 __device__ __forceinline__ Moments merge(const Moments& a, const Moments& b) {
     Moments o;
     o.n = a.n + b.n;
-    const float f = o.n > 0.f ? b.n / o.n : 0.f;
+    const float f = o.n > 0.f ? __fdividef(b.n, o.n) : 0.f;
     const float d = b.mean - a.mean;
     o.mean = a.mean + d * f;
     o.m2 = a.m2 + b.m2 + d * d * a.n * f;
@@ -755,6 +755,21 @@ constexpr size_t ring_bytes() {
 template <typename T, int V, typename Packs>
 __device__ __forceinline__ Moments block_of(const Packs& pk, uint32_t rows) {
     Vec<V> v[kBlockRows], t = splat<V>(0.f);
+    if (rows == kBlockRows) {  // all but a chunk's last: no row to leave out
+#pragma unroll
+        for (int u = 0; u < kBlockRows; ++u) {
+            v[u] = widen<T, V>(pk[u][0]);
+            t = add(t, v[u]);
+        }
+        const Vec<V> less = splat<V>(sum(t) * (-1.f / (kBlockRows * V)));
+        t = splat<V>(0.f);
+#pragma unroll
+        for (int u = 0; u < kBlockRows; ++u) {
+            const Vec<V> e = add(v[u], less);
+            t = fma(e, e, t);
+        }
+        return Moments{(float)(kBlockRows * V), -less.v[0], sum(t)};
+    }
 #pragma unroll
     for (uint32_t u = 0; u < kBlockRows; ++u) {
         v[u] = u < rows ? widen<T, V>(pk[u][0]) : splat<V>(0.f);
