@@ -104,12 +104,12 @@ __device__ __forceinline__ void store_pack_cs(T* p, const Pack<T, V>& v) {
 }
 
 // Asynchronous copies global -> shared of one pack (4 bytes at least); a
-// thread waits for its own.  L1: 16-byte copies go through the L1 cache too.
-template <typename T, int V, bool L1 = false>
+// thread waits for its own.
+template <typename T, int V>
 __device__ __forceinline__ void copy_pack_async(Pack<T, V>* smem, const T* global) {
     constexpr int bytes = sizeof(T) * V;
     const uint32_t to = (uint32_t)__cvta_generic_to_shared(smem);
-    if constexpr (bytes == 16 && !L1)
+    if constexpr (bytes == 16)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(global) : "memory");
     else if constexpr (bytes >= 4)
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(global), "n"(bytes) : "memory");

@@ -29,27 +29,12 @@ __device__ __forceinline__ int64_t load_index(const void* idx, int type, uint64_
 // ---------------------------------------------------------------- lookup --
 
 constexpr int kLookupThreads = 256;
-// Four parts ahead, through L1, so that a row that many indices share is not
-// fetched from one place of L2 each time: 2 M lookups of one row of 400 bytes
-// take 169 us in place of 2141 past L1, power-law ones 273 either way.  Eight
-// ahead leave L1 too little room (314 us).
-constexpr uint32_t kLookupAhead = 4;
 constexpr uint32_t kLookupRows = 1024;  // of a CTA, at most
 constexpr uint32_t kZeroRow = 0xFFFFFFFFu;  // of padding and of bad indices
 
-// A team of 8, 16 or 32 lanes copies `per` whole rows, a pack a lane, row by row
-// and part by part; the next kLookupAhead parts are on their way into the lane's
-// part of a ring in shared memory.  A CTA reads its indices once, before.
-template <typename TT, typename TO, int V>
-__global__ void __launch_bounds__(kLookupThreads) lookup_kernel(
-    const TT* __restrict__ table, uint32_t table_stride, uint32_t num_rows, const void* __restrict__ idx,
-    int idx_type, uint32_t n, int64_t padding, float scale, TO* __restrict__ out, uint32_t out_stride,
-    uint32_t packs, uint32_t lanes, uint32_t per, uint32_t* __restrict__ bad) {
-    constexpr bool kAsync = sizeof(Pack<TT, V>) >= 4;
-    __shared__ Pack<TT, V> ring[kLookupAhead][kLookupThreads];
-    __shared__ uint32_t ids[kLookupRows];
-    const uint32_t teams = kLookupThreads / lanes, first = blockIdx.x * teams * per;
-    const uint32_t rows = min(teams * per, n - first);
+// A CTA's indices, checked, in shared memory.
+__device__ __forceinline__ void load_ids(uint32_t* ids, const void* idx, int idx_type, uint32_t first, uint32_t rows,
+                                         int64_t padding, uint32_t num_rows, uint32_t* bad) {
     for (uint32_t i = threadIdx.x; i < rows; i += kLookupThreads) {
         const int64_t id = load_index(idx, idx_type, first + i);
         uint32_t row = kZeroRow;
@@ -60,53 +45,123 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(
         ids[i] = row;
     }
     __syncthreads();
-    const uint32_t lane = threadIdx.x % lanes, team = threadIdx.x / lanes;
-    const uint32_t r0 = min(team * per, rows), r1 = min(r0 + per, rows);
-    auto source = [&](uint32_t row, uint32_t c) {
-        return reinterpret_cast<const TT*>(reinterpret_cast<const char*>(table) + (uint64_t)row * table_stride) + c * V;
-    };
-    uint32_t fetch_row = r0, fetch_c = lane, put = 0;
-    auto fetch = [&] {
-        if (fetch_row < r1) {
-            const uint32_t row = ids[fetch_row];
-            if (fetch_c < packs && row != kZeroRow)
-                copy_pack_async<TT, V, true>(&ring[put][threadIdx.x], source(row, fetch_c));
-            fetch_c += lanes;
-            if (fetch_c - lane >= packs) {
-                fetch_c = lane;
-                ++fetch_row;
-            }
+}
+
+// The packs of a CTA's rows in order, whatever a row's length, so that rows of 25
+// packs leave no lane idle.  A thread loads its next kAhead packs (32 bytes) while
+// it writes those before: 65,537 x 602 fp32 take 55 us, 2 M power-law rows of
+// 100 266 at 6.1 TB/s of what they move (a team of lanes per row: 59 and 270).
+// Loads go through L1, so that a row that many indices share is not fetched from
+// one place of L2 each time (2 M lookups of one row of 400 bytes: 135 us, past L1
+// 2141).
+template <typename TT, typename TO, int V>
+__global__ void __launch_bounds__(kLookupThreads) lookup_kernel(
+    const TT* __restrict__ table, uint32_t table_stride, uint32_t num_rows, const void* __restrict__ idx,
+    int idx_type, uint32_t n, int64_t padding, float scale, TO* __restrict__ out, uint32_t out_stride,
+    uint32_t packs, uint32_t per_pack, uint32_t rows, uint32_t* __restrict__ bad) {
+    constexpr int kAhead = sizeof(Pack<TT, V>) == 16 ? 2 : sizeof(Pack<TT, V>) == 8 ? 4 : 8;
+    __shared__ uint32_t ids[kLookupRows];
+    const uint32_t first = blockIdx.x * rows;
+    rows = min(rows, n - first);
+    load_ids(ids, idx, idx_type, first, rows, padding, num_rows, bad);
+    const char* from = reinterpret_cast<const char*>(table);
+    char* to = reinterpret_cast<char*>(out) + (uint64_t)first * out_stride;
+    const uint32_t total = rows * packs;
+    auto fetch = [&](Pack<TT, V>(&v)[kAhead], uint32_t e0) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint32_t e = e0 + u * kLookupThreads, row = __umulhi(2 * e, per_pack), c = e - row * packs;
+            const uint32_t id = e < total ? ids[row] : kZeroRow;
+            v[u] = Pack<TT, V>{};
+            if (id != kZeroRow)
+                v[u] = load_pack_nc<TT, V>(
+                    reinterpret_cast<const TT*>(from + (uint64_t)id * table_stride + c * (uint32_t)sizeof(v[u])));
         }
-        commit_copies();
-        put = (put + 1) % kLookupAhead;
     };
-    // a slot is filled again one part after it was read, when its values are in use already
-    if constexpr (kAsync)
-        for (uint32_t k = 0; k + 1 < kLookupAhead; ++k) fetch();
-    uint32_t take = 0;
-#pragma unroll 1
-    for (uint32_t r = r0; r < r1; ++r) {
-        const uint32_t row = ids[r];
-        TO* to = reinterpret_cast<TO*>(reinterpret_cast<char*>(out) + (uint64_t)(first + r) * out_stride);
-#pragma unroll 1
-        for (uint32_t c = lane; c - lane < packs; c += lanes) {
-            Pack<TT, V> v;
-            if constexpr (kAsync) {
-                fetch();
-                wait_copies<kLookupAhead - 1>();
-                v = load_pack<TT, V>(ring[take][threadIdx.x].v);
-                take = (take + 1) % kLookupAhead;
-            } else if (c < packs && row != kZeroRow) {
-                v = load_pack_nc<TT, V>(source(row, c));
-            }
-            if (c >= packs) continue;
+    auto write = [&](const Pack<TT, V>(&v)[kAhead], uint32_t e0) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint32_t e = e0 + u * kLookupThreads, row = __umulhi(2 * e, per_pack), c = e - row * packs;
+            if (e >= total) break;
+            const float f = ids[row] != kZeroRow ? scale : 0.f;  // zeros, whatever the scale
             Pack<TO, V> o;
 #pragma unroll
-            for (int k = 0; k < V; ++k) o.v[k] = from_f32<TO>(row != kZeroRow ? to_f32(v.v[k]) * scale : 0.f);
-            store_pack_cs<TO, V>(to + c * V, o);
+            for (int k = 0; k < V; ++k) o.v[k] = from_f32<TO>(to_f32(v[u].v[k]) * f);
+            store_pack_cs<TO, V>(reinterpret_cast<TO*>(to + (uint64_t)row * out_stride + c * (uint32_t)sizeof(o)), o);
+        }
+    };
+    constexpr uint32_t kStep = kAhead * kLookupThreads;
+    Pack<TT, V> v[kAhead], w[kAhead];
+    uint32_t e = threadIdx.x;
+    fetch(v, e);
+#pragma unroll 1
+    while (e < total) {
+        fetch(w, e + kStep);
+        write(v, e);
+        if (e + kStep >= total) break;
+        fetch(v, e + 2 * kStep);
+        write(w, e + kStep);
+        e += 2 * kStep;
+    }
+}
+
+// Rows whose width or place no wider pack divides go value by value, where the flat
+// order is bound by its index arithmetic (300,000 rows of 333 values: 182 us).
+// Here a team of lanes takes whole rows, PARTS values of each a lane at a time and
+// as many rows as make eight: 74 us.
+template <typename TT, typename TO, int PARTS>
+__global__ void __launch_bounds__(kLookupThreads) lookup_odd_kernel(
+    const TT* __restrict__ table, uint32_t table_stride, uint32_t num_rows, const void* __restrict__ idx,
+    int idx_type, uint32_t n, int64_t padding, float scale, TO* __restrict__ out, uint32_t out_stride,
+    uint32_t width, uint32_t lanes, uint32_t rows, uint32_t* __restrict__ bad) {
+    constexpr int kRows = 8 / PARTS;
+    __shared__ uint32_t ids[kLookupRows];
+    const uint32_t first = blockIdx.x * rows;
+    rows = min(rows, n - first);
+    load_ids(ids, idx, idx_type, first, rows, padding, num_rows, bad);
+    const uint32_t teams = kLookupThreads / lanes, team = threadIdx.x / lanes, step = kRows * teams;
+    // with more than one part the team is a warp
+#pragma unroll 1
+    for (uint32_t c = threadIdx.x % lanes; c - threadIdx.x % lanes < width; c += PARTS * lanes) {
+        const char* from = reinterpret_cast<const char*>(table + c);
+        char* to = reinterpret_cast<char*>(out + c) + (uint64_t)first * out_stride;
+        auto fetch = [&](TT(&v)[8], uint32_t r0) {
+#pragma unroll
+            for (int q = 0; q < kRows; ++q) {
+                const uint32_t r = r0 + q * teams, id = r < rows ? ids[r] : kZeroRow;
+                const TT* at = reinterpret_cast<const TT*>(from + (uint64_t)id * table_stride);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    v[q * PARTS + p] = from_f32<TT>(0.f);
+                    if (id != kZeroRow && c + p * 32 < width) v[q * PARTS + p] = __ldg(at + p * 32);
+                }
+            }
+        };
+        auto write = [&](const TT(&v)[8], uint32_t r0) {
+#pragma unroll
+            for (int q = 0; q < kRows; ++q) {
+                const uint32_t r = r0 + q * teams;
+                if (r >= rows) break;
+                TO* at = reinterpret_cast<TO*>(to + (uint64_t)r * out_stride);
+                const float f = ids[r] != kZeroRow ? scale : 0.f;  // zeros, whatever the scale
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+                    if (c + p * 32 < width) __stcs(at + p * 32, from_f32<TO>(to_f32(v[q * PARTS + p]) * f));
+            }
+        };
+        TT v[8], w[8];
+        uint32_t r = team;
+        fetch(v, r);
+#pragma unroll 1
+        while (r < rows) {
+            fetch(w, r + step);
+            write(v, r);
+            if (r + step >= rows) break;
+            fetch(v, r + 2 * step);
+            write(w, r + step);
+            r += 2 * step;
         }
     }
-    if constexpr (kAsync) wait_copies<0>();
 }
 
 // Teams of at least as many lanes as rows in flight: narrower packs for
@@ -116,19 +171,35 @@ inline int team_width(int width, uint32_t F) {
     return width;
 }
 
+// As many rows a CTA as are asked for, fewer where that would leave less than eight CTAs per SM.
+inline uint32_t lookup_rows(uint64_t n, uint32_t rows) {
+    rows = std::clamp(rows, 1u, kLookupRows);
+    while (rows > 1 && n / rows < 148 * 8) rows >>= 1;
+    return rows;
+}
+
 template <typename TT, typename TO, int V>
 void launch_lookup(const EmbeddingArgs& a, cudaStream_t s) {
     const uint32_t packs = a.F / V;
-    uint32_t lanes = 8;
-    while (lanes < 32 && lanes < packs) lanes <<= 1;
-    // 32 rows a team, fewer where that would leave less than eight CTAs per SM
-    const uint32_t teams = kLookupThreads / lanes;
-    uint32_t per = kLookupRows / (kLookupThreads / 8);
-    while (per > 1 && a.n / per < 148ull * 8 * teams) per >>= 1;
-    lookup_kernel<TT, TO, V><<<ceil_div(a.n, (uint64_t)per * teams), kLookupThreads, 0, s>>>(
+    const uint32_t rows = lookup_rows(a.n, 4096 / packs);  // of 16,384 packs a CTA: 60 us in place of 53
+    // a pack's row is e / packs = the high half of 2 e * per_pack, exact for the e < 2^13 of several rows
+    const uint32_t per_pack = rows > 1 ? (uint32_t)(((1ull << 31) + packs - 1) / packs) : 0;
+    lookup_kernel<TT, TO, V><<<ceil_div(a.n, rows), kLookupThreads, 0, s>>>(
         static_cast<const TT*>(a.table), (uint32_t)(a.ldt * sizeof(TT)), (uint32_t)a.num_rows, a.idx, a.idx_type,
-        (uint32_t)a.n, a.padding, a.scale, static_cast<TO*>(a.rows), (uint32_t)(a.ldr * sizeof(TO)), packs, lanes,
-        per, a.bad);
+        (uint32_t)a.n, a.padding, a.scale, static_cast<TO*>(a.rows), (uint32_t)(a.ldr * sizeof(TO)), packs, per_pack,
+        rows, a.bad);
+    TCC_CUDA(cudaGetLastError());
+}
+
+template <typename TT, typename TO, int PARTS>
+void launch_lookup_odd(const EmbeddingArgs& a, cudaStream_t s) {
+    uint32_t lanes = 8;
+    while (lanes < 32 && lanes < a.F) lanes <<= 1;
+    const uint32_t rows = lookup_rows(a.n, 4 * (8 / PARTS) * kLookupThreads / lanes);
+    lookup_odd_kernel<TT, TO, PARTS><<<ceil_div(a.n, rows), kLookupThreads, 0, s>>>(
+        static_cast<const TT*>(a.table), (uint32_t)(a.ldt * sizeof(TT)), (uint32_t)a.num_rows, a.idx, a.idx_type,
+        (uint32_t)a.n, a.padding, a.scale, static_cast<TO*>(a.rows), (uint32_t)(a.ldr * sizeof(TO)), a.F, lanes, rows,
+        a.bad);
     TCC_CUDA(cudaGetLastError());
 }
 
@@ -140,13 +211,23 @@ void lookup_by_width(const EmbeddingArgs& a, cudaStream_t s) {
     rule.count(a.ldr);
     rule.pointer(a.table, sizeof(TT));
     rule.pointer(a.rows, sizeof(TO));
-    switch (team_width(rule.width(), a.F)) {
+    switch (rule.width()) {
         case 8:
             if constexpr (sizeof(TT) == 2 && sizeof(TO) == 2) launch_lookup<TT, TO, 8>(a, s);
             break;
         case 4: launch_lookup<TT, TO, 4>(a, s); break;
         case 2: launch_lookup<TT, TO, 2>(a, s); break;
-        default: launch_lookup<TT, TO, 1>(a, s);
+        default:
+            // whole rows by teams where at least two thirds of their places are taken: of 2 M rows
+            // 15 values wide in 64 us (in flat order 72), 1 M of 47 in 84 (98); 9 wide 53 (49), 17 92 (78)
+            if (uint32_t places = 8; a.F <= 128) {
+                while (places < a.F) places <<= 1;
+                if (3 * a.F < 2 * places) return launch_lookup<TT, TO, 1>(a, s);
+            }
+            if (a.F <= 32) launch_lookup_odd<TT, TO, 1>(a, s);
+            else if (a.F <= 64) launch_lookup_odd<TT, TO, 2>(a, s);
+            else if (a.F <= 128) launch_lookup_odd<TT, TO, 4>(a, s);
+            else launch_lookup_odd<TT, TO, 8>(a, s);
     }
 }
 

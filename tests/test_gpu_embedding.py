@@ -68,6 +68,23 @@ def _ids(rows, n, kind, gen, dtype):
     return idx.to(dtype)
 
 
+@pytest.mark.parametrize("types", [(F32, F32), (F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("width", [5, 7, 9, 13, 25, 33, 53, 89, 101, 127, 129, 257, 333, 523])
+def test_lookup_odd_widths(gpu, types, width):
+    gen = _gen(width)
+    table = torch.randn((301, width), generator=gen, device="cuda").to(types[0])
+    for n in (1, 37, 20011):
+        idx = torch.randint(-1, 302, (n,), generator=gen, device="cuda")
+        _check_lookup(E.embedding(table, idx, 1.7, padding_idx=-1, out_dtype=types[1]), table, idx, 1.7, -1)
+    idx.fill_(-1)
+    assert not E.embedding(table, idx, float("inf"), padding_idx=-1).any()
+    wide = torch.randn((301, width + 4), generator=gen, device="cuda").to(types[0])
+    for first in (1, 2):  # rows that begin anywhere
+        view = wide[:, first:first + width]
+        idx = torch.randint(301, (2003,), generator=gen, device="cuda")
+        _check_lookup(E.embedding(view, idx, out_dtype=types[1]), view, idx, 1.0, None)
+
+
 @pytest.mark.parametrize("types", [(F32, F32), (F16, F16), (F16, F32), (BF16, BF16), (BF16, F32)])
 @pytest.mark.parametrize("width", [1, 2, 3, 47, 100, 128, 602, 2056])
 def test_lookup_types_and_widths(gpu, types, width):
