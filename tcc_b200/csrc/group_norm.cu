@@ -26,8 +26,8 @@ size_t group_norm_scratch_bytes(uint64_t N, uint64_t S, uint32_t C, uint32_t G, 
                 continue;
             }
             const SplitShape sh = split_shape(N, S, C, G, V);
-            bytes = std::max(bytes, stats + (backward ? align256(N * sh.chunks * 2 * C * 4)
-                                                      : align256(N * sh.chunks * G * sh.SUB * sizeof(Moments))));
+            bytes = std::max(bytes, backward ? split_grad_plan(N, C, G, sh).bytes
+                                             : stats + align256(N * sh.chunks * G * sh.SUB * sizeof(Moments)));
         }
     return (size_t)bytes;
 }

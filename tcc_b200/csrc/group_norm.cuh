@@ -632,8 +632,9 @@ struct SplitPlace {
     uint32_t chunk;
 };
 
+// `item`: of the N * chunks chunks of all samples.
 template <int V>
-__device__ __forceinline__ SplitPlace split_place(const GroupNormArgs& a, const SplitShape& sh, bool reverse) {
+__device__ __forceinline__ SplitPlace split_place(const GroupNormArgs& a, const SplitShape& sh, uint32_t item) {
     SplitPlace p;
     const uint32_t tx = threadIdx.x % sh.TX;
     p.rb = threadIdx.x / sh.TX;
@@ -655,9 +656,8 @@ __device__ __forceinline__ SplitPlace split_place(const GroupNormArgs& a, const 
         p.c = ((uint64_t)p.g * sh.PG + first + tx) * V;
     }
     p.on = p.on && p.rb < sh.RB;
-    const uint32_t block = reverse ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-    p.n = block / sh.chunks;
-    p.chunk = block - (uint32_t)p.n * sh.chunks;
+    p.n = item / sh.chunks;
+    p.chunk = item - (uint32_t)p.n * sh.chunks;
     p.row0 = p.chunk * sh.chunk_rows;
     p.row1 = min(p.row0 + sh.chunk_rows, a.S);
     return p;
@@ -812,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 3) split_moments_kernel(const GroupN
                                                                     Moments* __restrict__ partial) {
     after_previous();
     extern __shared__ uint4 smem[];
-    const SplitPlace p = split_place<V>(a, sh, false);
+    const SplitPlace p = split_place<V>(a, sh, blockIdx.x);
     const T* const from[1] = {static_cast<const T*>(a.x) + (p.n * a.S + p.row0 + p.rb) * a.ldx + p.c};
     const int64_t inc[1] = {(int64_t)(sh.RB * a.ldx)};
     Moments m{0.f, 0.f, 0.f};
@@ -858,7 +858,7 @@ __global__ void __launch_bounds__(kThreads) split_apply_kernel(const GroupNormAr
                                                                const float* mean_, const float* rstd_) {
     after_previous();
     extern __shared__ uint4 smem[];
-    const SplitPlace p = split_place<V>(a, sh, true);
+    const SplitPlace p = split_place<V>(a, sh, gridDim.x - 1 - blockIdx.x);
     const uint32_t count = own_rows(p, sh);
     if (!count) return;
     const uint64_t last = p.n * a.S + p.row0 + p.rb + (uint64_t)(count - 1) * sh.RB;
@@ -880,7 +880,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 3) split_sums_kernel(const GroupNormArgs a, const SplitShape sh,
                                                                  float* __restrict__ partial) {
     after_previous();
-    const SplitPlace p = split_place<V>(a, sh, false);
+    const SplitPlace p = split_place<V>(a, sh, blockIdx.x);
     extern __shared__ uint4 smem[];
     Vec<V> dw = splat<V>(0.f), db = dw;
     if (const uint32_t count = own_rows(p, sh)) {
@@ -978,12 +978,128 @@ __global__ void split_groups_kernel(const GroupNormArgs a, const float* partial,
     }
 }
 
+// The sums of many samples: a CTA takes every gridDim.x-th chunk of its columns and
+// keeps the parameters' sums to itself, in 64 bits, so that it leaves one row of
+// partial [grid][2][C] (or NULL) however many samples there are; the row per chunk of
+// split_sums_kernel would be twice the input for samples of one row.  What dx
+// needs of a chunk are two sums per part of a group: parts [N][chunks][G * SUB] =
+// (sum of weight * dz, sum of weight * dz * h), or NULL.
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads, 3) split_samples_kernel(const GroupNormArgs a, const SplitShape sh,
+                                                                    float* __restrict__ partial,
+                                                                    float2* __restrict__ parts) {
+    after_previous();
+    extern __shared__ uint4 smem[];
+    double(*all)[kThreads] = reinterpret_cast<double(*)[kThreads]>(
+        reinterpret_cast<char*>(smem) + ring_bytes<T, V, 2>());  // [2 V]: this thread's dweight, dbias
+    __shared__ float2 sums[kThreads];
+    const uint32_t items = (uint32_t)a.N * sh.chunks, lane = threadIdx.x & 31;
+    SplitPlace p = split_place<V>(a, sh, 0);
+    Vec<V> w, b;
+    load_params<V>(a, p.c, p.on, w, b);
+#pragma unroll
+    for (int k = 0; k < 2 * V; ++k) all[k][threadIdx.x] = 0.0;
+    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+        p = split_place<V>(a, sh, item);
+        float s = 0.f, q = 0.f;
+        if (const uint32_t count = own_rows(p, sh)) {
+            const uint64_t first = p.n * a.S + p.row0 + p.rb;
+            const T* const from[2] = {static_cast<const T*>(a.x) + first * a.ldx + p.c,
+                                      static_cast<const T*>(a.dy) + first * a.lddy + p.c};
+            const int64_t inc[2] = {(int64_t)(sh.RB * a.ldx), (int64_t)(sh.RB * a.lddy)};
+            const Vec<V> less = splat<V>(-a.mean[p.n * a.G + p.g]), rstd = splat<V>(a.rstd[p.n * a.G + p.g]);
+            Vec<V> dw = splat<V>(0.f), db = dw;
+            auto keep = [&] {
+                s += dot(db, w);
+                q += dot(dw, w);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    all[k][threadIdx.x] += (double)dw.v[k];
+                    all[V + k][threadIdx.x] += (double)db.v[k];
+                }
+                dw = db = splat<V>(0.f);
+            };
+            uint32_t since = 0;
+            stream_rows<T, V, 2, kDepth2, 1>(smem, from, inc, count, [&](const auto& pk, uint32_t) {
+                const Vec<V> h = mul(add(widen<T, V>(pk[0][0]), less), rstd);
+                const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
+                db = add(db, d);
+                dw = fma(d, h, dw);
+                if (++since == 32) {
+                    since = 0;
+                    keep();
+                }
+            });
+            keep();
+        }
+        if (!parts) continue;
+        sums[threadIdx.x] = make_float2(s, q);
+        __syncthreads();
+        // entry e of group i: row e / len of the block's threads, pack e % len of the group's part
+        const uint32_t len = sh.SUB == 1 ? sh.PG : p.len, entries = len * sh.RB;
+        const uint32_t slots = a.G * sh.SUB, first = blockIdx.y * sh.GPB;  // GPB = 1 where SUB > 1
+        const bool alone = entries <= 32;  // a thread a group, or else a warp
+        for (uint32_t i = alone ? threadIdx.x : threadIdx.x >> 5; i < sh.GPB && first + i < slots;
+             i += alone ? kThreads : kThreads / 32) {
+            float2 t = make_float2(0.f, 0.f);
+            for (uint32_t e = alone ? 0 : lane; e < entries; e += alone ? 1 : 32) {
+                const uint32_t r = e / len;
+                const float2 o = sums[r * sh.TX + i * sh.PG + (e - r * len)];
+                t.x += o.x;
+                t.y += o.y;
+            }
+            if (!alone) {
+                t.x = lane_sum(t.x, 32);
+                t.y = lane_sum(t.y, 32);
+            }
+            if (alone || lane == 0) parts[(uint64_t)item * slots + first + i] = t;
+        }
+        __syncthreads();
+    }
+    if (!partial) return;
+    __syncthreads();
+    const uint32_t across = sh.TX * V, c0 = block_channel<V>(sh);
+    const uint32_t c1 = min(c0 + across, sh.SUB == 1 ? a.C : (blockIdx.y / sh.SUB + 1) * (a.C / a.G));
+    float* out = partial + (uint64_t)blockIdx.x * 2 * a.C;
+    for (uint32_t i = threadIdx.x; i < 2 * across; i += kThreads) {
+        const uint32_t which = i >= across, e = i - which * across;
+        if (c0 + e >= c1) continue;
+        double t = 0.0;
+        for (uint32_t r = 0; r < sh.RB; ++r) t += all[which * V + e % V][r * sh.TX + e / V];
+        out[which * a.C + c0 + e] = (float)t;
+    }
+}
+
+// group_sums [N][G][2] from the parts of split_samples_kernel, a warp per (sample, group).
+__global__ void __launch_bounds__(kThreads) split_parts_kernel(const float2* parts, uint32_t groups, uint32_t G,
+                                                               uint32_t SUB, uint32_t chunks, float* group_sums) {
+    after_previous();
+    const uint32_t i = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (i >= groups) return;
+    const uint32_t n = i / G, g = i - n * G;
+    double s = 0.0, q = 0.0;
+    for (uint32_t k = lane; k < chunks * SUB; k += 32) {
+        const uint32_t ch = k / SUB;
+        const float2 t = parts[(((uint64_t)n * chunks + ch) * G + g) * SUB + (k - ch * SUB)];
+        s += (double)t.x;
+        q += (double)t.y;
+    }
+    for (int o = 16; o; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        q += __shfl_xor_sync(0xffffffffu, q, o);
+    }
+    if (lane == 0) {
+        group_sums[2ull * i] = (float)s;
+        group_sums[2ull * i + 1] = (float)q;
+    }
+}
+
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 3) split_grad_kernel(const GroupNormArgs a, const SplitShape sh,
                                                                  const float* group_sums) {
     after_previous();
     extern __shared__ uint4 smem[];
-    const SplitPlace p = split_place<V>(a, sh, true);
+    const SplitPlace p = split_place<V>(a, sh, gridDim.x - 1 - blockIdx.x);
     const uint32_t count = own_rows(p, sh);
     if (!count) return;
     const uint64_t last = p.n * a.S + p.row0 + p.rb + (uint64_t)(count - 1) * sh.RB;
@@ -1040,7 +1156,7 @@ __global__ void __launch_bounds__(kThreads) resident_forward_kernel(const GroupN
     __shared__ Moments group[kThreads];  // of this CTA's chunk; G <= kThreads
     __shared__ float2 stats[kThreads];   // mean and rstd of the sample's groups
     cg::cluster_group cluster = cg::this_cluster();
-    const SplitPlace p = split_place<V>(a, sh, false);
+    const SplitPlace p = split_place<V>(a, sh, blockIdx.x);
     const uint32_t count = own_rows(p, sh);
     Pack<T, V>* store = reinterpret_cast<Pack<T, V>*>(smem) + threadIdx.x;
     const uint64_t first = p.n * a.S + p.row0 + p.rb;
@@ -1095,7 +1211,7 @@ __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const Group
     float2* group = reinterpret_cast<float2*>(sums + 2);  // [G]: of this CTA's chunk
     float2* total = group + a.G;                          // [G]: of the sample
     cg::cluster_group cluster = cg::this_cluster();
-    SplitPlace p = split_place<V>(a, sh, false);
+    SplitPlace p = split_place<V>(a, sh, blockIdx.x);
     const uint32_t count = own_rows(p, sh);
     Pack<T, V>* store = reinterpret_cast<Pack<T, V>*>(smem) + threadIdx.x;
     const uint64_t step[2] = {sh.RB * a.ldx, sh.RB * a.lddy};
@@ -1254,6 +1370,31 @@ inline SplitShape split_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, in
     return sh;
 }
 
+// Scratch of the split form's backward: rows of [2][C] for the parameters'
+// gradients, and two sums per (sample, group), of parts of it first where
+// there are several.  A row per chunk while there are few chunks (30 MB at most;
+// with one sample split_groups_kernel then gives the parameters' gradients
+// too) or long ones (a row is then at most a 64th of a 16-bit chunk, and CTAs that
+// the hardware hands out balance better than fixed turns: 3,000 x 2048 x 128 bf16
+// 1271 us, a row per CTA 1383); else a row per CTA (1,780 x 33 x 1040 fp32: 230 us, a
+// row per chunk 724; 232,965 x 602 fp32 in one group 3.25 and 6.04 ms).
+constexpr uint64_t kFewChunks = kSms * 12, kLongChunk = 256;
+struct SplitGradPlan {
+    bool few;
+    uint64_t rows;                             // of [2][C]
+    uint64_t parts_bytes, group_bytes, bytes;  // parts_bytes = 0: the sums themselves
+};
+inline SplitGradPlan split_grad_plan(uint64_t N, uint32_t C, uint32_t G, const SplitShape& sh) {
+    SplitGradPlan p{};
+    const uint64_t items = N * sh.chunks;
+    p.few = items * sh.cols <= kFewChunks || sh.chunk_rows >= kLongChunk;
+    p.rows = p.few ? items : std::max<uint64_t>(1, kSms * 3 / sh.cols);
+    p.parts_bytes = p.few || sh.chunks * sh.SUB == 1 ? 0 : align256(items * G * sh.SUB * 8);
+    p.group_bytes = align256(N * G * 8);
+    p.bytes = align256(p.rows * 2 * C * 4) + p.parts_bytes + p.group_bytes;
+    return p;
+}
+
 // The resident form's cluster, or chunks = 0 where a sample does not fit: two
 // CTAs per SM; more CTAs than a sample needs only until every SM has one, and
 // while a thread has rows left to share.
@@ -1399,19 +1540,32 @@ void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStrea
                      mean, rstd);
         launch_after(split_apply_kernel<T, V>, grid, kThreads, ring1, s, a, sh, mean, rstd);
     } else {
+        const SplitGradPlan plan = split_grad_plan(a.N, a.C, a.G, sh);
         float* partial = reinterpret_cast<float*>(scratch);
-        float* group_sums = partial + align256(a.N * sh.chunks * 2 * a.C * 4) / 4;
-        split_sums_kernel<T, V><<<grid, kThreads, std::max(ring2, 2 * kThreads * V * sizeof(float)), s>>>(a, sh, partial);
-        const bool one = params && a.N == 1;  // one sample: its channels' sums are the parameters' gradients
-        if (a.dx || one) {
-            uint32_t cw = 1;
-            while (cw < 32 && cw < a.C / a.G) cw <<= 1;
-            launch_after(split_groups_kernel, groups, many ? 1024 : 128, 0, s, a, partial, sh.chunks, cw, group_sums,
-                         one);
+        char* after = scratch + align256(plan.rows * 2 * a.C * 4);
+        float* group_sums = reinterpret_cast<float*>(after + plan.parts_bytes);
+        const bool one = plan.few && params && a.N == 1;  // one sample: its channels' sums are the parameters' gradients
+        if (plan.few) {
+            split_sums_kernel<T, V><<<grid, kThreads, std::max(ring2, 2 * kThreads * V * sizeof(float)), s>>>(a, sh, partial);
+            if (a.dx || one) {
+                uint32_t cw = 1;
+                while (cw < 32 && cw < a.C / a.G) cw <<= 1;
+                launch_after(split_groups_kernel, groups, many ? 1024 : 128, 0, s, a, partial, sh.chunks, cw,
+                             group_sums, one);
+            }
+        } else {
+            constexpr size_t smem = ring2 + 2 * V * kThreads * sizeof(double);
+            static std::atomic<uint64_t> done{0};
+            if (smem > 46 * 1024) allow_smem(split_samples_kernel<T, V>, smem, done);  // beside 2 KB of static ones
+            float2* parts = plan.parts_bytes ? reinterpret_cast<float2*>(after) : reinterpret_cast<float2*>(group_sums);
+            split_samples_kernel<T, V><<<dim3((unsigned)plan.rows, sh.cols), kThreads, smem, s>>>(
+                a, sh, params ? partial : nullptr, a.dx ? parts : nullptr);
+            if (a.dx && plan.parts_bytes)
+                launch_after(split_parts_kernel, ceil_div(groups, kThreads / 32), kThreads, 0, s, parts, groups, a.G,
+                             sh.SUB, sh.chunks, group_sums);
         }
         if (a.dx) launch_after(split_grad_kernel<T, V>, grid, kThreads, ring2, s, a, sh, group_sums);
-        if (params && !one)
-            launch_param_grad(a, partial, a.N * sh.chunks, s);
+        if (params && !one) launch_param_grad(a, partial, plan.rows, s);
     }
     TCC_CUDA(cudaGetLastError());
 }

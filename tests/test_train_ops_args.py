@@ -174,3 +174,18 @@ def test_rows_of_strides():
     copy, ld = rows_of(t[:1, 1:2, :4], 4)
     assert ld == 4
     assert rows_of(one, 4)[0].is_contiguous()
+
+
+@pytest.mark.parametrize("steps", [1, 2, 40])
+@pytest.mark.parametrize("channels,groups", [(257, 1), (512, 1), (602, 1), (1024, 1), (1024, 2), (2048, 2), (2048, 1),
+                                             (1040, 260)])
+def test_norm_scratch_is_small_beside_the_input(lib, steps, channels, groups):
+    """Wide groups of few rows: no row of parameter gradients per sample, whatever form the widths and
+    pointers of a call lead to (512 channels of 2.4 M nodes took 10 GB)."""
+    samples = 2_449_029
+    for backward in (0, 1):
+        got = lib.tcc_group_norm_scratch_bytes(samples, steps, channels, groups, backward)
+        statistics = samples * groups * 8  # a mean and a deviation, or two sums, each
+        # those, the parts of groups that CTAs of 256 values each see, and sums that do not grow with the samples
+        parts = samples * groups * -(-channels // groups // 256) * 12
+        assert got <= statistics + parts + (64 << 20), (got, backward)
