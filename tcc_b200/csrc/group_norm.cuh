@@ -285,6 +285,22 @@ __device__ __forceinline__ float lane_sum(float v, uint32_t L) {
     return v;
 }
 
+// n floats, `stride` apart, by four sums at a time: no chain of more than n / 4 + 4 additions.
+__device__ __forceinline__ float strided_sum(const float* p, uint32_t stride, uint32_t n) {
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    uint32_t r = 0;
+    for (; r + 4 <= n; r += 4)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) t[u] += p[(r + u) * stride];
+    for (; r < n; ++r) t[0] += p[r * stride];
+    return (t[0] + t[1]) + (t[2] + t[3]);
+}
+
+// Long fp32 sums are kept in two levels: a thread adds kLevel rows (or blocks of
+// rows, or samples), then that sum to a second one, and takes at most kLongest
+// in all, so that no chain of additions grows with the data.
+constexpr uint32_t kLevel = 32, kLongest = 2048;
+
 // The place of a thread: its slot's group and sample, its packs' rows and
 // channels in them.
 template <int V, int J>
@@ -522,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
                                                                           add(g[j], splat<V>(-s))))));
             dx_now = advance(dx_now, sh.dx_step);
         }
-        if (++since == 32) {
+        if (++since == kLevel) {
             since = 0;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
@@ -574,9 +590,7 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
             const uint32_t slot = e / V >> sh.log_L, lane = (e / V) & (sh.L - 1);
             const uint32_t g = blockIdx.y * sh.GB + slot, pk = j * sh.L + lane, row = pk / sh.PG;
             if (g >= a.G || pk >= (fold ? sh.PG : sh.packs)) continue;
-            float t = 0.f;
-#pragma unroll 4
-            for (uint32_t r = 0; r < sh.RB; ++r) t += sm[which * kThreads * V + r * across + e];
+            const float t = strided_sum(sm + which * kThreads * V + e, across, sh.RB);
             const uint64_t to = fold ? blockIdx.x : (uint64_t)blockIdx.x * a.S + row;
             partial[(to * 2 + which) * a.C + g * (a.C / a.G) + (pk - row * sh.PG) * V + e % V] = t;
         }
@@ -751,6 +765,12 @@ constexpr size_t ring_bytes() {
     return (A == 1 ? kDepth1 : kDepth2) * A * kThreads * sizeof(Pack<T, V>);
 }
 
+// The threads' sums of split_sums_kernel take the ring's place.
+template <typename T, int V>
+constexpr size_t sums_bytes() {
+    return std::max(ring_bytes<T, V, 2>(), 2 * kThreads * V * sizeof(float));
+}
+
 // Moments of a thread's block of up to kBlockRows rows, around the block's own mean.
 template <typename T, int V, typename Packs>
 __device__ __forceinline__ Moments block_of(const Packs& pk, uint32_t rows) {
@@ -815,21 +835,28 @@ __global__ void __launch_bounds__(kThreads, 3) split_moments_kernel(const GroupN
     const SplitPlace p = split_place<V>(a, sh, blockIdx.x);
     const T* const from[1] = {static_cast<const T*>(a.x) + (p.n * a.S + p.row0 + p.rb) * a.ldx + p.c};
     const int64_t inc[1] = {(int64_t)(sh.RB * a.ldx)};
+    __shared__ Moments sm[kThreads];  // the second level, then the CTA's
     Moments m{0.f, 0.f, 0.f};
+    sm[threadIdx.x] = m;
+    uint32_t since = 0;
     stream_rows<T, V, 1, kDepth1, kBlockRows>(smem, from, inc, own_rows(p, sh), [&](const auto& pk, uint32_t rows) {
         m = merge(m, block_of<T, V>(pk, rows));
+        if (++since == kLevel) {
+            since = 0;
+            sm[threadIdx.x] = merge(sm[threadIdx.x], m);
+            m = Moments{0.f, 0.f, 0.f};
+        }
     });
-    __shared__ Moments sm[kThreads];
-    block_moments(p, sh, m, sm);
+    block_moments(p, sh, merge(sm[threadIdx.x], m), sm);
     if (p.on && p.rb == 0 && p.gi == 0)
         partial[(p.n * sh.chunks + p.chunk) * ((uint64_t)a.G * sh.SUB) + p.slot] = sm[threadIdx.x];
 }
 
-// A CTA of one or eight warps per (sample, group) merges its partial moments.
+// A CTA of 1, 8 or 32 warps per (sample, group) merges its partial moments.
 __global__ void split_stats_kernel(const Moments* partial, uint32_t G, uint32_t SUB, uint32_t chunks, float eps, float* mean,
                                    float* rstd) {
     after_previous();
-    __shared__ Moments sm[8];
+    __shared__ Moments sm[32];
     const uint64_t n = blockIdx.x / G;
     const uint32_t g = (uint32_t)(blockIdx.x - n * G);
     Moments m{0.f, 0.f, 0.f};
@@ -882,6 +909,10 @@ __global__ void __launch_bounds__(kThreads, 3) split_sums_kernel(const GroupNorm
     after_previous();
     const SplitPlace p = split_place<V>(a, sh, blockIdx.x);
     extern __shared__ uint4 smem[];
+    float(*all)[kThreads] = reinterpret_cast<float(*)[kThreads]>(
+        reinterpret_cast<char*>(smem) + sums_bytes<T, V>());  // [2 V]: the second level
+#pragma unroll
+    for (int k = 0; k < 2 * V; ++k) all[k][threadIdx.x] = 0.f;
     Vec<V> dw = splat<V>(0.f), db = dw;
     if (const uint32_t count = own_rows(p, sh)) {
         const uint64_t first = p.n * a.S + p.row0 + p.rb;
@@ -891,19 +922,29 @@ __global__ void __launch_bounds__(kThreads, 3) split_sums_kernel(const GroupNorm
         const Vec<V> less = splat<V>(-a.mean[p.n * a.G + p.g]), rstd = splat<V>(a.rstd[p.n * a.G + p.g]);
         Vec<V> w, b;
         load_params<V>(a, p.c, true, w, b);
+        uint32_t since = 0;
         stream_rows<T, V, 2, kDepth2, 1>(smem, from, inc, count, [&](const auto& pk, uint32_t) {
             const Vec<V> h = mul(add(widen<T, V>(pk[0][0]), less), rstd);
             const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
             db = add(db, d);
             dw = fma(d, h, dw);
+            if (++since == kLevel) {
+                since = 0;
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    all[k][threadIdx.x] += dw.v[k];
+                    all[V + k][threadIdx.x] += db.v[k];
+                }
+                dw = db = splat<V>(0.f);
+            }
         });
     }
     __syncthreads();
     float(*sm)[kThreads * V] = reinterpret_cast<float(*)[kThreads * V]>(smem);  // [2], in the ring's place
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        sm[0][threadIdx.x * V + k] = dw.v[k];
-        sm[1][threadIdx.x * V + k] = db.v[k];
+        sm[0][threadIdx.x * V + k] = all[k][threadIdx.x] + dw.v[k];
+        sm[1][threadIdx.x * V + k] = all[V + k][threadIdx.x] + db.v[k];
     }
     __syncthreads();
     // channels of the block, then the rows of threads
@@ -913,10 +954,7 @@ __global__ void __launch_bounds__(kThreads, 3) split_sums_kernel(const GroupNorm
     for (uint32_t i = threadIdx.x; i < 2 * across; i += kThreads) {
         const uint32_t which = i >= across, e = i - which * across;
         if (c0 + e >= c1) continue;
-        float t = 0.f;
-#pragma unroll 4
-        for (uint32_t r = 0; r < sh.RB; ++r) t += sm[which][r * across + e];
-        out[which * a.C + c0 + e] = t;
+        out[which * a.C + c0 + e] = strided_sum(&sm[which][e], across, sh.RB);
     }
 }
 
@@ -1025,7 +1063,7 @@ __global__ void __launch_bounds__(kThreads, 3) split_samples_kernel(const GroupN
                 const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
                 db = add(db, d);
                 dw = fma(d, h, dw);
-                if (++since == 32) {
+                if (++since == kLevel) {
                     since = 0;
                     keep();
                 }
@@ -1229,11 +1267,21 @@ __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const Group
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < 2 * a.C; i += kThreads) {
             const uint32_t which = i >= a.C, c = i - which * a.C;
-            float t = 0.f;
-#pragma unroll 4
-            for (uint32_t r = 0; r < sh.RB; ++r) t += sums[which][r * a.C + c];
-            use(which, c, t);
+            use(which, c, strided_sum(&sums[which][c], a.C, sh.RB));
         }
+    };
+    // the parameters' sums of up to kLevel samples go to the CTA's row of partial, each by one thread
+    float* out = partial + (uint64_t)blockIdx.x * 2 * a.C;
+    uint32_t since = 0;
+    bool kept = false;
+    auto keep = [&] {
+        over_rows(all_dw, all_db, [&](uint32_t which, uint32_t c, float t) {
+            out[which * a.C + c] = kept ? out[which * a.C + c] + t : t;
+        });
+        kept = true;
+        since = 0;
+        all_dw = all_db = splat<V>(0.f);
+        __syncthreads();
     };
     for (; p.n < a.N; p.n += gridDim.x / sh.chunks) {  // the same for the whole cluster
         const uint64_t first = p.n * a.S + p.row0 + p.rb;
@@ -1256,6 +1304,7 @@ __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const Group
         }
         all_dw = add(all_dw, dw);
         all_db = add(all_db, db);
+        if (++since == kLevel && partial) keep();
         if (!a.dx) continue;
         // row 0 of the sums becomes the channels' sums: each is read by the thread that writes it
         over_rows(dw, db, [&](uint32_t which, uint32_t c, float t) {
@@ -1293,10 +1342,9 @@ __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const Group
             dx += sh.RB * a.lddx;
         }
     }
-    if (!partial) return;
+    if (!partial || (kept && !since)) return;
     __syncthreads();
-    float* out = partial + (uint64_t)blockIdx.x * 2 * a.C;
-    over_rows(all_dw, all_db, [&](uint32_t which, uint32_t c, float t) { out[which * a.C + c] = t; });
+    keep();
 }
 
 // ------------------------------------------------------------------ host --
@@ -1340,12 +1388,14 @@ inline RowsShape rows_shape(uint64_t S, uint32_t C, uint32_t G, int V) {
 inline bool rows_fold(const RowsShape& sh) { return sh.PG <= sh.L && (sh.PG & (sh.PG - 1)) == 0; }
 inline uint64_t rows_blocks(const RowsShape& sh, uint64_t N, uint32_t G) {
     const uint64_t y = (G + sh.GB - 1) / sh.GB;
-    return std::max<uint64_t>(1, std::min((N + sh.RB - 1) / sh.RB, kSms * 4 / std::min(kSms, y)));
+    return std::max<uint64_t>({1, std::min((N + sh.RB - 1) / sh.RB, kSms * 4 / std::min(kSms, y)),
+                               (N + (uint64_t)sh.RB * kLongest - 1) / (sh.RB * kLongest)});
 }
 
 // Chunks of a sample: three CTAs per SM over all samples, which run at once (a
 // whole number of waves for each of the four kernels; 185 us for 232,965 x 256
-// bf16 in place of 195 with eight per SM); at least eight rows a thread.
+// bf16 in place of 195 with eight per SM); at least eight rows a thread, at most
+// kLongest.
 inline SplitShape split_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, int V) {
     SplitShape sh;
     sh.PG = C / G / V;
@@ -1364,7 +1414,7 @@ inline SplitShape split_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G, in
     }
     const uint64_t want = std::max<uint64_t>(1, kSms * 3 / std::max<uint64_t>(1, std::min(N, kSms * 3) * sh.cols));
     const uint64_t most = std::max<uint64_t>(1, S / (8 * sh.RB));
-    const uint64_t chunks = std::min(want, most);
+    const uint64_t chunks = std::max(std::min(want, most), (S + (uint64_t)sh.RB * kLongest - 1) / (sh.RB * kLongest));
     sh.chunk_rows = (S + chunks - 1) / chunks;
     sh.chunks = (uint32_t)((S + sh.chunk_rows - 1) / sh.chunk_rows);
     return sh;
@@ -1430,7 +1480,9 @@ inline SplitShape resident_shape(uint64_t N, uint64_t S, uint32_t C, uint32_t G,
     return sh;
 }
 // CTAs of the backward: a cluster goes on with another sample.
-inline uint64_t resident_grid(uint64_t N, uint32_t chunks) { return std::min(N, kSms * 8 / chunks) * chunks; }
+inline uint64_t resident_grid(uint64_t N, uint32_t chunks) {
+    return std::max(std::min(N, kSms * 8 / chunks), (N + kLevel * kLevel - 1) / (kLevel * kLevel)) * chunks;
+}
 
 template <typename T, int V, int J>
 void rows_launch(const GroupNormArgs& a, float* partial, bool backward, cudaStream_t s) {
@@ -1536,7 +1588,8 @@ void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStrea
             rstd = mean + align256(a.N * a.G * 4) / 4;
         }
         split_moments_kernel<T, V><<<grid, kThreads, ring1, s>>>(a, sh, partial);
-        launch_after(split_stats_kernel, groups, many ? kThreads : 32, 0, s, partial, a.G, sh.SUB, sh.chunks, a.eps,
+        const uint32_t merged = sh.chunks * sh.SUB;
+        launch_after(split_stats_kernel, groups, merged > 16384 ? 1024 : many ? kThreads : 32, 0, s, partial, a.G, sh.SUB, sh.chunks, a.eps,
                      mean, rstd);
         launch_after(split_apply_kernel<T, V>, grid, kThreads, ring1, s, a, sh, mean, rstd);
     } else {
@@ -1546,7 +1599,7 @@ void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStrea
         float* group_sums = reinterpret_cast<float*>(after + plan.parts_bytes);
         const bool one = plan.few && params && a.N == 1;  // one sample: its channels' sums are the parameters' gradients
         if (plan.few) {
-            split_sums_kernel<T, V><<<grid, kThreads, std::max(ring2, 2 * kThreads * V * sizeof(float)), s>>>(a, sh, partial);
+            split_sums_kernel<T, V><<<grid, kThreads, sums_bytes<T, V>() + 2 * V * kThreads * sizeof(float), s>>>(a, sh, partial);
             if (a.dx || one) {
                 uint32_t cw = 1;
                 while (cw < 32 && cw < a.C / a.G) cw <<= 1;
