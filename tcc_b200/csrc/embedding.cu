@@ -1016,7 +1016,8 @@ __global__ void __launch_bounds__(kThreads) grad_sorted_kernel(
 
 // A block per range: where a run begins in it and goes on, its parts are added.
 // The threads are columns (of W floats) times groups; a group adds a contiguous
-// part of the ranges, and the groups' sums are added in order.
+// part of the ranges, and the groups' sums are added in order, in 64 bits: a hub's
+// run has as many parts as its rows allow, and a wide row one group.
 template <typename TT, int W>
 __global__ void __launch_bounds__(kThreads) grad_join_kernel(const Border* borders, uint32_t sums, const float* heads,
                                                              const float* tails, uint32_t width, float scale,
@@ -1026,7 +1027,7 @@ __global__ void __launch_bounds__(kThreads) grad_join_kernel(const Border* borde
     if (!(b.flags & kTail) || b.row >= num_rows) return;
     // the ranges after it that hold a part: up to the first that is not passed through
     __shared__ uint32_t last;
-    __shared__ Pack<float, W> part[kThreads];
+    __shared__ double part[W][kThreads];
     const uint32_t begin = blockIdx.x + 1;
     if (threadIdx.x == 0) last = sums;
     for (uint32_t from = begin;; from += kThreads) {
@@ -1045,27 +1046,32 @@ __global__ void __launch_bounds__(kThreads) grad_join_kernel(const Border* borde
     const uint32_t p0 = begin + min(group * each, parts), p1 = begin + min((group + 1) * each, parts);
     for (uint32_t c0 = 0; c0 < cols; c0 += across) {
         const uint32_t c = c0 + threadIdx.x % across;
-        Pack<float, W> acc;
+        double acc[W];
 #pragma unroll
-        for (int k = 0; k < W; ++k) acc.v[k] = 0.f;
+        for (int k = 0; k < W; ++k) acc[k] = 0.0;
         if (c < cols) {
-            if (group == 0) acc = load_pack<float, W>(tails + (uint64_t)blockIdx.x * width + c * W);
+            if (group == 0) {
+                const Pack<float, W> t = load_pack<float, W>(tails + (uint64_t)blockIdx.x * width + c * W);
+#pragma unroll
+                for (int k = 0; k < W; ++k) acc[k] = (double)t.v[k];
+            }
 #pragma unroll 4
             for (uint32_t i = p0; i < p1; ++i) {
                 const Pack<float, W> h = load_pack<float, W>(heads + (uint64_t)i * width + c * W);
 #pragma unroll
-                for (int k = 0; k < W; ++k) acc.v[k] += h.v[k];
+                for (int k = 0; k < W; ++k) acc[k] += (double)h.v[k];
             }
         }
-        part[threadIdx.x] = acc;
+#pragma unroll
+        for (int k = 0; k < W; ++k) part[k][threadIdx.x] = acc[k];
         __syncthreads();
         if (group == 0 && c < cols) {
             for (uint32_t g = 1; g < groups && g * each < parts; ++g)
 #pragma unroll
-                for (int k = 0; k < W; ++k) acc.v[k] += part[g * across + threadIdx.x].v[k];
+                for (int k = 0; k < W; ++k) acc[k] += part[k][g * across + threadIdx.x];
 #pragma unroll
             for (int k = 0; k < W; ++k)
-                dtable[(uint64_t)b.row * ldt + c * W + k] = from_f32<TT>(acc.v[k] * scale);
+                dtable[(uint64_t)b.row * ldt + c * W + k] = from_f32<TT>((float)(acc[k] * (double)scale));
         }
         __syncthreads();
     }

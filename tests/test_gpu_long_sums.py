@@ -7,6 +7,7 @@ some 500 u; the operators' chains, 192 operations at most, stay below 192 u."""
 import pytest
 import torch
 
+from tcc_b200 import embedding as E
 from tcc_b200 import norm as N
 from test_gpu_group_norm import D, F32, U, Oracle
 
@@ -70,3 +71,16 @@ def test_split_form_moments(gpu):
     _, mean, rstd = N.group_norm_forward(x, 1, eps=0.0)
     assert abs(float(mean)) <= D * U * a
     assert abs(float(rstd) * a - 1) <= D * U * 2  # |x| is the deviation: A rstd = 1
+
+
+@pytest.mark.parametrize("width", [1024, 257])
+def test_run_of_one_row(gpu, width):
+    """1.2 M gradient rows of one table row: 2,344 ranges of 512 to be joined, one thread a column.
+    A range's own sum is exact but for the 2^-23 of each value."""
+    n = 1_200_000
+    idx = torch.full((n,), 3, device="cuda")
+    grad = torch.full((n, width), 1 + 2.0 ** -14 - 2.0 ** -23, device="cuda")
+    out = E.embedding_backward(grad, idx, 7)
+    want = n * float(grad[0, 0])
+    assert float((out[3].double() - want).abs().max()) <= (D + 1) * U * want
+    assert not out[:3].any() and not out[4:].any()
