@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -17,6 +18,19 @@ def type_code(t: torch.Tensor, name: str) -> int:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     return code
+
+
+def tracked(*tensors) -> bool:
+    """Whether autograd has to see a call with these inputs (None for one left out): one requires a
+    gradient, or carries a tangent (forward mode, which the operators' functions refuse with an error;
+    past them its derivative would be lost in silence)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    # outside dual_level, 0.3 us a tensor less than asking each
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 _bound = {}

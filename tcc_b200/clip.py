@@ -67,7 +67,8 @@ def _written(tensors) -> None:
 
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm of all elements of the tensors (one, or an iterable), a float32 scalar on
-    their device; 64-bit sums in a fixed order.  Without tensors a CPU zero."""
+    their device; 64-bit sums in a fixed order.  Without tensors a CPU zero.  No derivative
+    flows through it."""
     words, count, device, _ = _table(_list(tensors))
     if count == 0:
         return torch.zeros(())

@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from ._args import TYPES, launch, rows_of, scratch_for, type_code
+from ._args import TYPES, launch, rows_of, scratch_for, tracked, type_code
 
 _INDEX = {torch.int32: L.I32, torch.int64: L.I64}
 
@@ -69,6 +69,7 @@ def embedding_backward(grad_out: torch.Tensor, idx: torch.Tensor, num_rows: int,
                        bad: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient [num_rows, F] of a table for ``embedding``'s output gradient
     ``grad_out`` [*idx.shape, F]: scale * the sum of the rows of each index.
+    Not differentiable itself.
     ``dtype``: the table's type (default grad_out's)."""
     code = type_code(grad_out, "grad_out")
     dtype = grad_out.dtype if dtype is None else dtype
@@ -110,14 +111,14 @@ class _Embedding(torch.autograd.Function):
 
 def embedding(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None,
               out_dtype: torch.dtype | None = None, bad: torch.Tensor | None = None) -> torch.Tensor:
-    """scale * table[idx] ([*idx.shape, F]), differentiable in the table.
+    """scale * table[idx] ([*idx.shape, F]), differentiable in the table (in reverse mode).
 
     ``padding_idx`` (any value, e.g. -1 for the filled-up end of a block): its
     rows are zero and give no gradient.  ``out_dtype``: the table's type
     (default) or float32, which the aggregation takes.  An index outside the
     table gives a zero row, no gradient, and sets ``bad`` (an int32 CUDA tensor,
     optional) to 1."""
-    if torch.is_grad_enabled() and table.requires_grad:
+    if tracked(table):
         return _Embedding.apply(table, idx, scale, padding_idx, out_dtype, bad)
     return _lookup(table, idx, scale, padding_idx, out_dtype, bad)
 

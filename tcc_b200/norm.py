@@ -14,7 +14,7 @@ import math
 import torch
 
 from . import _lib as L
-from ._args import launch, rows_of, scratch_for, type_code
+from ._args import launch, rows_of, scratch_for, tracked, type_code
 
 
 def _parameter(p, name: str, channels: int, x: torch.Tensor):
@@ -98,7 +98,8 @@ def _forward(x, num_groups, weight, bias, eps, act, stats):
 
 def group_norm_forward(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None,
                        bias: torch.Tensor | None = None, eps: float = 1e-5, act: str = "none"):
-    """(y, mean, rstd): ``group_norm`` and the fp32 [N, num_groups] statistics its backward reads."""
+    """(y, mean, rstd): ``group_norm`` and the fp32 [N, num_groups] statistics its backward reads.
+    Not differentiable: the pass by itself."""
     return _forward(x, num_groups, weight, bias, eps, act, True)
 
 
@@ -107,7 +108,7 @@ def group_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
                         bias: torch.Tensor | None = None, act: str = "none", need_dx: bool = True):
     """(dx, dweight, dbias) of ``group_norm`` for the output gradient dy, from the
     forward's x, mean and rstd.  None for a parameter that is None, and for dx
-    without ``need_dx``."""
+    without ``need_dx``.  Not differentiable itself."""
     code, act = type_code(x, "x"), _activation(act)
     n, steps, channels = _sizes(x, num_groups)
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
@@ -148,13 +149,12 @@ class _GroupNorm(torch.autograd.Function):
 
 def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None,
                bias: torch.Tensor | None = None, eps: float = 1e-5, act: str = "none") -> torch.Tensor:
-    """act(group norm of x * weight + bias), differentiable in x, weight and bias.
+    """act(group norm of x * weight + bias), differentiable in x, weight and bias (in reverse mode).
 
     x: [N, C] or [N, ..., C], float32, float16 or bfloat16; statistics per sample
     and group in fp32 with the population variance.  weight, bias: [C] of one
     type (x's or another), or None.  act: "none", "relu", "silu" or "gelu"."""
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if tracked(x, weight, bias):
         return _GroupNorm.apply(x, num_groups, weight, bias, eps, act)
     return _forward(x, num_groups, weight, bias, eps, act, False)[0]
 

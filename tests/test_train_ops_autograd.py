@@ -1,0 +1,53 @@
+"""What autograd sees of the training operators (CPU only: the launches are left out)."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from tcc_b200 import _lib as L
+from tcc_b200 import embedding, norm
+
+
+@pytest.fixture
+def no_launch(monkeypatch):
+    """The operators on CPU tensors: types are checked, nothing is computed."""
+    for module in (embedding, norm):
+        monkeypatch.setattr(module, "type_code", lambda t, name: L.F32)
+        monkeypatch.setattr(module, "launch", lambda *args: None)
+    monkeypatch.setattr(norm, "_scratch_bytes", lambda *args: 0)
+
+
+IDX = torch.tensor([2, 0, 1])
+CALLS = [lambda t: embedding.embedding(t, IDX), lambda t: norm.group_norm(t, 2),
+         lambda t: norm.group_norm(torch.ones(4, 6), 2, weight=t[0]),
+         lambda t: norm.group_norm(torch.ones(4, 6), 2, bias=t[0]), norm.GroupNorm(3, 6)]
+
+
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_forward_mode_is_refused(no_launch, call, requires_grad, grad_mode):
+    """A dual tensor never gives an output without a tangent, which would read as a derivative of zero."""
+    t = torch.randn(4, 6, requires_grad=requires_grad)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        with pytest.raises((RuntimeError, NotImplementedError), match="(?i)forward"):
+            call(forward_ad.make_dual(t, torch.ones(4, 6)))
+        assert forward_ad.unpack_dual(call(torch.randn(4, 6))).tangent is None  # one without: as outside
+    with torch.no_grad():
+        assert not call(t).requires_grad
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_reverse_mode_takes_the_functions_path(no_launch, call):
+    assert call(torch.randn(4, 6, requires_grad=True)).requires_grad
+    assert isinstance(call, norm.GroupNorm) or not call(torch.randn(4, 6)).requires_grad
+
+
+@pytest.mark.parametrize("call", CALLS[:2])
+def test_functional_transforms_are_refused(no_launch, call):
+    t = torch.randn(4, 6)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(call, (t,), (torch.ones(4, 6),))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(call)(torch.randn(2, 4, 6))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: call(t).sum())(t)
