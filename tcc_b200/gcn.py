@@ -22,7 +22,7 @@ import torch
 
 from . import spmm_cnic
 from . import tiles as T
-from .norm import GroupNorm, group_norm
+from .norm import GroupNorm
 
 CooData = namedtuple("CooData", ["f_row_indices", "f_col_indices",
                                  "s_row_indices", "s_col_indices"])
@@ -157,12 +157,14 @@ def relu_dropout(x: torch.Tensor, p: float, seed: int, training: bool = True) ->
 
 def hidden_activation(x: torch.Tensor, p: float, seed: int, training: bool = True,
                       norm: GroupNorm | None = None) -> torch.Tensor:
-    """relu_dropout(norm(x)); without dropout the relu is part of the norm's pass."""
+    """relu_dropout(norm(x)).  The norm is called as a module in every mode, so its hooks see the
+    same values; one with act="relu" (as GCN's) leaves no relu to do where nothing is dropped."""
     if norm is None:
         return relu_dropout(x, p, seed, training)
-    if not training or p == 0.0:
-        return group_norm(x, norm.num_groups, norm.weight, norm.bias, norm.eps, "relu")
-    return relu_dropout(norm(x), p, seed)
+    h = norm(x)
+    if norm.act == "relu" and (not training or p == 0.0):
+        return h
+    return relu_dropout(h, p, seed, training)
 
 
 # ------------------------------------------------------------- TiledGraph --
@@ -247,7 +249,7 @@ class GCN(torch.nn.Module):
     def __init__(self, num_features, hidden_dim, num_classes, dropout=0.5, seed=0, norm_groups=0):
         super().__init__()
         self.conv1 = GCNConv(num_features, hidden_dim, first_layer=True)
-        self.norm = GroupNorm(norm_groups, hidden_dim) if norm_groups else None
+        self.norm = GroupNorm(norm_groups, hidden_dim, act="relu") if norm_groups else None
         self.conv_final = GCNConv(hidden_dim, num_classes)
         self.p = dropout
         self._seed = seed

@@ -152,7 +152,7 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
     params = [W1, W2]
     norm = None
     if cfg.get("norm_groups"):
-        norm = GroupNorm(cfg["norm_groups"], cfg["hidden"], device=device)
+        norm = GroupNorm(cfg["norm_groups"], cfg["hidden"], act="relu", device=device)
         params += [norm.weight, norm.bias]
     opt = torch.optim.Adam(params, lr=cfg["lr"])
     start_epoch = 0

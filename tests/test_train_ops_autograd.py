@@ -4,7 +4,7 @@ import torch
 from torch.autograd import forward_ad
 
 from tcc_b200 import _lib as L
-from tcc_b200 import embedding, norm
+from tcc_b200 import embedding, gcn, norm
 
 
 @pytest.fixture
@@ -51,3 +51,28 @@ def test_functional_transforms_are_refused(no_launch, call):
         torch.func.vmap(call)(torch.randn(2, 4, 6))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda t: call(t).sum())(t)
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+def test_hidden_activation_calls_the_module(monkeypatch, act):
+    """Hooks of the norm run, and its own activation counts, in every mode; what they see is the
+    same in all (plain torch in the kernels' places)."""
+    acts = {"none": lambda z: z, "relu": torch.relu, "silu": torch.nn.functional.silu}
+
+    def plain(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
+        return acts[act](torch.nn.functional.group_norm(x, groups, weight, bias, eps))
+    monkeypatch.setattr(norm, "group_norm", plain)
+    if hasattr(gcn, "group_norm"):
+        monkeypatch.setattr(gcn, "group_norm", plain)
+    monkeypatch.setattr(gcn.ReluDropout, "apply", lambda x, p, seed: torch.relu(x) * 2)  # drops nothing here
+    layer, seen = norm.GroupNorm(2, 6, act=act), []
+    with torch.no_grad():
+        layer.weight.copy_(torch.linspace(-1, 2, 6))
+        layer.bias.copy_(torch.linspace(-0.5, 0.5, 6))
+    layer.register_forward_hook(lambda module, args, out: seen.append(out.detach()))
+    x = torch.randn(5, 6)
+    want = plain(x, 2, layer.weight, layer.bias, act=act)
+    for training, p in ((True, 0.5), (True, 0.0), (False, 0.5), (False, 0.0)):
+        out = gcn.hidden_activation(x, p, 3, training, layer)
+        assert torch.equal(out, torch.relu(want) * (2 if training and p else 1))
+    assert len(seen) == 4 and all(torch.equal(s, want) for s in seen)
