@@ -124,7 +124,7 @@ def embedding(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0, paddin
 
 
 class NodeEmbedding(torch.nn.Module):
-    """A learned row per node (or per node or edge type), read by index."""
+    """A learned row per node (or per node or edge type), read by index; ``bad`` as in ``embedding``."""
 
     def __init__(self, num_rows: int, width: int, scale: float = 1.0, padding_idx: int | None = None,
                  dtype: torch.dtype | None = None, out_dtype: torch.dtype | None = None, device=None):
@@ -133,5 +133,5 @@ class NodeEmbedding(torch.nn.Module):
         torch.nn.init.normal_(self.weight)
         self.scale, self.padding_idx, self.out_dtype = scale, padding_idx, out_dtype
 
-    def forward(self, idx: torch.Tensor) -> torch.Tensor:
-        return embedding(self.weight, idx, self.scale, self.padding_idx, self.out_dtype)
+    def forward(self, idx: torch.Tensor, bad: torch.Tensor | None = None) -> torch.Tensor:
+        return embedding(self.weight, idx, self.scale, self.padding_idx, self.out_dtype, bad)

@@ -208,8 +208,10 @@ def batch_feature_maps(store, input_ids: torch.Tensor):
     return store.cache_search_map[idx].contiguous(), store.id_map[idx].contiguous()
 
 
-def embedding_rows(table: torch.Tensor, block: Block, scale: float = 1.0) -> torch.Tensor:
+def embedding_rows(table: torch.Tensor, block: Block, scale: float = 1.0,
+                   bad: torch.Tensor | None = None) -> torch.Tensor:
     """Input rows [num_src, F] of a block from a learned node-embedding table (float32, as the
     aggregation takes them, whatever the table's type; F a multiple of 4 for it), differentiable
-    in the table.  Source ids of -1 (a block filled up to a fixed size) give zero rows."""
-    return embedding(table, block.src_ids, scale, padding_idx=-1, out_dtype=torch.float32)
+    in the table.  Source ids of -1 (a block filled up to a fixed size) give zero rows; an id
+    outside the table does too, and sets ``bad`` (an int32 CUDA tensor) to 1."""
+    return embedding(table, block.src_ids, scale, padding_idx=-1, out_dtype=torch.float32, bad=bad)

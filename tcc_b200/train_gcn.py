@@ -204,6 +204,7 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
     drop_seed = (cfg["seed"] * 1000 + rank) << 20  # dropout draw of epoch e: drop_seed + e
     epoch_no = [start_epoch]
     cls_pad = (cfg["classes"] + 3) // 4 * 4  # transform-first SpMM width, multiple of 4
+    bad_label = torch.zeros(1, dtype=torch.int32, device=device)  # set by a labelled row outside the rank's
 
     def epoch(stage_next: bool):
         opt.zero_grad(set_to_none=True)
@@ -227,7 +228,7 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
         else:
             scores = _DistAggregate.apply(R["dg"], H1) @ W2
         # the labelled rows first, then without the columns that fill them up
-        logits = embedding(scores, R["lab_idx"])[:, :cfg["classes"]]
+        logits = embedding(scores, R["lab_idx"], bad=bad_label)[:, :cfg["classes"]]
         loss = torch.nn.functional.cross_entropy(logits, R["lab_y"],
                                                  reduction="sum") / R["n_lab"]
         loss.backward()
@@ -261,6 +262,8 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
         b.synchronize()
         times.append(a.elapsed_time(b) / 1e3)
         losses.append(float(lt))
+        if int(bad_label):
+            raise IndexError("a labelled row lies outside the graph")
     if staged:
         side.synchronize()
     if cfg.get("save") and rank == 0:  # weights are identical on every rank

@@ -1,0 +1,39 @@
+"""What the trainer and the modules check of their inputs (GPU)."""
+import pytest
+import torch
+
+from tcc_b200 import embedding as E
+from tcc_b200 import train_gcn
+
+pytestmark = pytest.mark.gpu
+
+
+def _small(**kw):
+    cfg = train_gcn.config(shrink=10)
+    cfg.update(dropout=0.0, epochs=1)
+    cfg.update(kw)
+    return cfg
+
+
+@pytest.mark.parametrize("order", [True, False])
+def test_trainer_refuses_a_labelled_row_outside_the_graph(gpu, monkeypatch, order):
+    build = train_gcn.build
+
+    def broken(*args):
+        r = build(*args)
+        r["lab_idx"] = r["lab_idx"].clone()
+        r["lab_idx"][0] = r["r1"] - r["r0"]  # one past the last row: the lookup reads nothing there
+        return r
+    monkeypatch.setattr(train_gcn, "build", broken)
+    with pytest.raises(IndexError, match="labelled row"):
+        train_gcn.train(_small(), gpu, 1, 0, order)
+
+
+def test_module_reports_a_bad_index(gpu):
+    layer = E.NodeEmbedding(30, 10, padding_idx=-1, device="cuda")
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    idx = torch.tensor([3, -1, 29], device="cuda")
+    layer(idx, bad)
+    assert int(bad) == 0
+    idx[2] = 30
+    assert not layer(idx, bad)[2].any() and int(bad) == 1

@@ -4,7 +4,7 @@ import torch
 from torch.autograd import forward_ad
 
 from tcc_b200 import _lib as L
-from tcc_b200 import embedding, gcn, norm
+from tcc_b200 import embedding, gcn, minibatch, norm
 
 
 @pytest.fixture
@@ -76,3 +76,16 @@ def test_hidden_activation_calls_the_module(monkeypatch, act):
         out = gcn.hidden_activation(x, p, 3, training, layer)
         assert torch.equal(out, torch.relu(want) * (2 if training and p else 1))
     assert len(seen) == 4 and all(torch.equal(s, want) for s in seen)
+
+
+def test_every_lookup_can_report_a_bad_index(no_launch, monkeypatch):
+    """The module and the block's rows hand `bad` on to the call."""
+    flags = []
+    monkeypatch.setattr(embedding, "launch", lambda device, name, *args: flags.append(args[-1]))
+    bad = torch.zeros(1, dtype=torch.int32)
+    layer = embedding.NodeEmbedding(4, 6)
+    block = minibatch.Block(dst_ids=IDX, src_ids=IDX, edge_dst=IDX, edge_src=IDX)
+    for call in (lambda **kw: layer(IDX, **kw), lambda **kw: minibatch.embedding_rows(layer.weight, block, **kw)):
+        call()
+        call(bad=bad)
+    assert flags == [None, bad.data_ptr()] * 2
