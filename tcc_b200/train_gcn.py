@@ -138,6 +138,15 @@ def build(cfg: dict, device, world: int, rank: int):
                 nnz=int(lcol.numel()), gen_s=gen_s, conv_s=conv_s)
 
 
+def check_norm_groups(ck: dict, cfg: dict) -> None:
+    """The run goes on with the checkpoint's model: the same groups of the hidden norm, or none in both
+    (the norm's parameters fit any number of groups, so their shapes do not tell)."""
+    now = cfg.get("norm_groups") or 0
+    saved = ck.get("config", {}).get("norm_groups") or 0
+    if ("norm" in ck) != (now > 0) or ("config" in ck and saved != now):
+        raise ValueError(f"the checkpoint was trained with --norm-groups {saved}, this run has {now}")
+
+
 def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None = None):
     if transform_first is None:  # aggregate at the narrower width of layer 2
         transform_first = cfg["classes"] < cfg["hidden"]
@@ -158,11 +167,10 @@ def train(cfg: dict, device, world: int, rank: int, transform_first: bool | None
     start_epoch = 0
     if cfg.get("resume"):
         ck = torch.load(cfg["resume"], map_location=device)
+        check_norm_groups(ck, cfg)
         with torch.no_grad():
             W1.copy_(ck["W1"])
             W2.copy_(ck["W2"])
-            if (norm is not None) != ("norm" in ck):
-                raise ValueError("the checkpoint and this run differ in whether they normalise (--norm-groups)")
             if norm is not None:
                 norm.load_state_dict(ck["norm"])
         opt.load_state_dict(ck["opt"])

@@ -37,3 +37,12 @@ def test_module_reports_a_bad_index(gpu):
     assert int(bad) == 0
     idx[2] = 30
     assert not layer(idx, bad)[2].any() and int(bad) == 1
+
+
+def test_resume_with_other_groups_is_refused(gpu, tmp_path):
+    ck = str(tmp_path / "gcn.pt")
+    train_gcn.train(_small(norm_groups=8, save=ck), gpu, 1, 0)
+    for groups in (4, 0):
+        with pytest.raises(ValueError, match="norm-groups"):
+            train_gcn.train(_small(norm_groups=groups, epochs=2, resume=ck), gpu, 1, 0)
+    assert len(train_gcn.train(_small(norm_groups=8, epochs=2, resume=ck), gpu, 1, 0)["losses"]) == 1
