@@ -154,47 +154,72 @@ __device__ __forceinline__ Pack<T, V> narrow(const Vec<V>& a) {
 
 // ------------------------------------------------------------ activation --
 
-// 1 / (1 + 2^(-z log2 e)), off by a few units in the last place: the
-// hardware's exponential and reciprocal, which take one issue slot each.
+// The hardware's exponential and reciprocal, which take one issue slot each: off by
+// 4 u and 2 u of their results (u = 2^-24).
+template <int V>
+__device__ __forceinline__ void exp2_of(Vec<V>& a) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a.v[k]));
+}
+template <int V>
+__device__ __forceinline__ void reciprocal_of(Vec<V>& a) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a.v[k]));
+}
+
+// 1 / (1 + 2^(-z log2 e)).  The product is rounded, so for z < 0 the result is off by
+// up to (10 + |z|) u of itself (measured: 15 u at -10, 63 u at -80, where it is 1e-35);
+// for z > 0 by 5 u.  Taking the exponent in two parts instead keeps 10 u everywhere but
+// takes 13 % more time (2.4 M x 256 fp32: 1020 us forward in place of 898).
 template <int V>
 __device__ __forceinline__ Vec<V> sigmoid(const Vec<V>& z) {
     Vec<V> e = mul(z, splat<V>(-1.4426950408889634f));
-#pragma unroll
-    for (int k = 0; k < V; ++k) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.v[k]));
+    exp2_of(e);
     e = add(e, splat<V>(1.f));
-#pragma unroll
-    for (int k = 0; k < V; ++k) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.v[k]));
+    reciprocal_of(e);
     return e;
 }
 
 // The normal distribution function Phi(z), and e = exp(-z^2 / 2) for its
-// density, by Abramowitz and Stegun's rational approximation of erf (Handbook
-// of Mathematical Functions, 7.1.26): off by at most 0.75e-7, about one unit in
-// the last place of values near 1, with the hardware's exponential and
-// reciprocal.  (erff and expf in its place: 1095 us against 650 for 2.4 M x 256
-// bf16 values.)
-template <int V>
+// density: Phi(-|z|) = e * t * P(t) with t = 1 / (1 + p |z|), the form of Abramowitz and
+// Stegun (Handbook of Mathematical Functions, 7.1.26).  (erff and expf in its place:
+// 1095 us against 650 for 2.4 M x 256 bf16 values.)
+//  * 16-bit features: their p and five terms, off by 0.75e-7 in exact arithmetic and
+//    by up to 3e-7 with fp32's roundings, far below the features' own.
+//  * fp32 features (FINE): six terms, fitted here to erfcx(|z| / sqrt 2) / 2 over
+//    |z| <= 13.5 with the relative error weighted by 1 / (1 + z^4): Phi(-|z|) is off by
+//    at most (16 + 1.5 z^2 + 1.5 z^4) u of itself, the second part from the rounded
+//    exponent, where the five terms reach 870 u at -3 and 7,800 u at -4.  1 to 2 % more time
+//    (2.4 M x 256: backward 1325 -> 1343 us).
+template <bool FINE, int V>
 __device__ __forceinline__ Vec<V> normal_cdf(const Vec<V>& z, Vec<V>& e) {
-    Vec<V> x, t;
+    Vec<V> t, q;
 #pragma unroll
-    for (int k = 0; k < V; ++k) x.v[k] = fabsf(z.v[k]);
-    t = fma(x, splat<V>(0.3275911f * 0.70710678118654752f), splat<V>(1.f));
-#pragma unroll
-    for (int k = 0; k < V; ++k) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t.v[k]));
+    for (int k = 0; k < V; ++k) t.v[k] = fabsf(z.v[k]);
+    t = fma(t, splat<V>(FINE ? 0.4f : 0.3275911f * 0.70710678118654752f), splat<V>(1.f));
+    reciprocal_of(t);
     e = mul(mul(z, splat<V>(-0.72134752044448170f)), z);  // log2(e) / 2
-#pragma unroll
-    for (int k = 0; k < V; ++k) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.v[k]));
-    Vec<V> q = fma(t, splat<V>(0.5f * 1.061405429f), splat<V>(-0.5f * 1.453152027f));
-    q = fma(q, t, splat<V>(0.5f * 1.421413741f));
-    q = fma(q, t, splat<V>(-0.5f * 0.284496736f));
-    q = fma(q, t, splat<V>(0.5f * 0.254829592f));
+    exp2_of(e);
+    if constexpr (FINE) {
+        q = fma(t, splat<V>(0.0550596827387823f), splat<V>(-0.24951052190289993f));
+        q = fma(q, t, splat<V>(0.33170637217092475f));
+        q = fma(q, t, splat<V>(0.0192833073779339f));
+        q = fma(q, t, splat<V>(0.18641695632855948f));
+        q = fma(q, t, splat<V>(0.15704418169723153f));
+    } else {
+        q = fma(t, splat<V>(0.5f * 1.061405429f), splat<V>(-0.5f * 1.453152027f));
+        q = fma(q, t, splat<V>(0.5f * 1.421413741f));
+        q = fma(q, t, splat<V>(-0.5f * 0.284496736f));
+        q = fma(q, t, splat<V>(0.5f * 0.254829592f));
+    }
     q = mul(mul(q, t), e);  // Phi(-|z|)
 #pragma unroll
     for (int k = 0; k < V; ++k) q.v[k] = z.v[k] < 0.f ? q.v[k] : 1.f - q.v[k];
     return q;
 }
 
-template <int V>
+// act(z) of features of type T
+template <typename T, int V>
 __device__ __forceinline__ Vec<V> activate(int act, Vec<V> z) {
     if (act == TCC_ACT_RELU) {
 #pragma unroll
@@ -203,13 +228,13 @@ __device__ __forceinline__ Vec<V> activate(int act, Vec<V> z) {
         z = mul(z, sigmoid(z));
     } else if (act == TCC_ACT_GELU) {
         Vec<V> e;
-        z = mul(z, normal_cdf(z, e));
+        z = mul(z, normal_cdf<sizeof(T) == 4>(z, e));
     }
     return z;
 }
 
 // d * act'(z)
-template <int V>
+template <typename T, int V>
 __device__ __forceinline__ Vec<V> activate_grad(int act, const Vec<V>& z, Vec<V> d) {
     if (act == TCC_ACT_RELU) {
 #pragma unroll
@@ -219,7 +244,7 @@ __device__ __forceinline__ Vec<V> activate_grad(int act, const Vec<V>& z, Vec<V>
         d = mul(d, fma(mul(z, s), rest, s));
     } else if (act == TCC_ACT_GELU) {  // Phi(z) + z phi(z)
         Vec<V> e;
-        const Vec<V> cdf = normal_cdf(z, e);
+        const Vec<V> cdf = normal_cdf<sizeof(T) == 4>(z, e);
         d = mul(d, fma(mul(z, splat<V>(0.39894228040143268f)), e, cdf));
     }
     return d;
@@ -414,7 +439,7 @@ __global__ void __launch_bounds__(kThreads) rows_forward_kernel(const GroupNormA
         for (int j = 0; j < J; ++j)
             if (p.ok[j] && on)
                 store_pack_cs<T, V>(y + p.at(j, a.ldy),
-                                    narrow<T, V>(activate<V>(a.act, fma(mul(v[j], splat<V>(r)), p.w[j], p.b[j]))));
+                                    narrow<T, V>(activate<T, V>(a.act, fma(mul(v[j], splat<V>(r)), p.w[j], p.b[j]))));
         y = advance(y, sh.y_step);
     }
     if (!a.mean) return;
@@ -520,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
         float s = 0.f, q = 0.f;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            if (a.act != TCC_ACT_NONE) g[j] = activate_grad<V>(a.act, fma(h[j], p.w[j], p.b[j]), g[j]);
+            if (a.act != TCC_ACT_NONE) g[j] = activate_grad<T, V>(a.act, fma(h[j], p.w[j], p.b[j]), g[j]);
             db[j] = add(db[j], g[j]);
             dw[j] = fma(g[j], h[j], dw[j]);
             g[j] = mul(g[j], p.w[j]);
@@ -688,6 +713,9 @@ __device__ __forceinline__ uint32_t block_channel(const SplitShape& sh) {
 struct Moments {
     float n, mean, m2;
 };
+
+// The division is the hardware's, off by two units in the last place: what it
+// weighs is a difference of means, so it costs no more than the sums' own roundings.
 
 __device__ __forceinline__ Moments merge(const Moments& a, const Moments& b) {
     Moments o;
@@ -897,7 +925,7 @@ __global__ void __launch_bounds__(kThreads) split_apply_kernel(const GroupNormAr
     load_params<V>(a, p.c, true, w, b);
     stream_rows<T, V, 1, kDepth1, 1>(smem, from, inc, count, [&](const auto& pk, uint32_t) {
         const Vec<V> h = mul(add(widen<T, V>(pk[0][0]), less), rstd);
-        store_pack_cs<T, V>(y, narrow<T, V>(activate<V>(a.act, fma(h, w, b))));
+        store_pack_cs<T, V>(y, narrow<T, V>(activate<T, V>(a.act, fma(h, w, b))));
         y -= sh.RB * a.ldy;
     });
 }
@@ -925,7 +953,7 @@ __global__ void __launch_bounds__(kThreads, 3) split_sums_kernel(const GroupNorm
         uint32_t since = 0;
         stream_rows<T, V, 2, kDepth2, 1>(smem, from, inc, count, [&](const auto& pk, uint32_t) {
             const Vec<V> h = mul(add(widen<T, V>(pk[0][0]), less), rstd);
-            const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
+            const Vec<V> d = activate_grad<T, V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
             db = add(db, d);
             dw = fma(d, h, dw);
             if (++since == kLevel) {
@@ -1060,7 +1088,7 @@ __global__ void __launch_bounds__(kThreads, 3) split_samples_kernel(const GroupN
             uint32_t since = 0;
             stream_rows<T, V, 2, kDepth2, 1>(smem, from, inc, count, [&](const auto& pk, uint32_t) {
                 const Vec<V> h = mul(add(widen<T, V>(pk[0][0]), less), rstd);
-                const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
+                const Vec<V> d = activate_grad<T, V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
                 db = add(db, d);
                 dw = fma(d, h, dw);
                 if (++since == kLevel) {
@@ -1153,7 +1181,7 @@ __global__ void __launch_bounds__(kThreads, 3) split_grad_kernel(const GroupNorm
     load_params<V>(a, p.c, true, w, b);
     stream_rows<T, V, 2, kDepth2, 1>(smem, from, inc, count, [&](const auto& pk, uint32_t) {
         const Vec<V> h = mul(add(widen<T, V>(pk[0][0]), less), rstd);
-        const Vec<V> d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
+        const Vec<V> d = activate_grad<T, V>(a.act, fma(h, w, b), widen<T, V>(pk[0][1]));
         store_pack_cs<T, V>(dx, narrow<T, V>(mul(rstd, fma(h, q, fma(d, w, s)))));
         dx -= sh.RB * a.lddx;
     });
@@ -1232,7 +1260,7 @@ __global__ void __launch_bounds__(kThreads) resident_forward_kernel(const GroupN
     const Vec<V> less = splat<V>(-stats[p.g].x), rstd = splat<V>(stats[p.g].y);
     for (uint32_t k = 0; k < count; ++k) {
         const Vec<V> h = mul(add(widen<T, V>(load_pack<T, V>(store[k * kThreads].v)), less), rstd);
-        store_pack_cs<T, V>(y, narrow<T, V>(activate<V>(a.act, fma(h, w, b))));
+        store_pack_cs<T, V>(y, narrow<T, V>(activate<T, V>(a.act, fma(h, w, b))));
         y += sh.RB * a.ldy;
     }
 }
@@ -1292,7 +1320,7 @@ __global__ void __launch_bounds__(kThreads) resident_backward_kernel(const Group
         const Vec<V> rstd = splat<V>(p.on ? a.rstd[p.n * a.G + p.g] : 0.f);
         auto row = [&](uint32_t k, Vec<V>& h, Vec<V>& d) {
             h = mul(add(widen<T, V>(load_pack<T, V>(store[(2 * k) * kThreads].v)), less), rstd);
-            d = activate_grad<V>(a.act, fma(h, w, b), widen<T, V>(load_pack<T, V>(store[(2 * k + 1) * kThreads].v)));
+            d = activate_grad<T, V>(a.act, fma(h, w, b), widen<T, V>(load_pack<T, V>(store[(2 * k + 1) * kThreads].v)));
         };
         wait_copies<0>();
         Vec<V> dw = splat<V>(0.f), db = dw;
