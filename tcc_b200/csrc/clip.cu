@@ -177,9 +177,11 @@ __device__ __forceinline__ void span_scale(const Span& sp, float f) {
     }
 }
 
-// A factor of 1 changes no value, nor does any factor change zeros alone; a NaN
-// norm spreads, as it should.
-__device__ __forceinline__ bool must_scale(float norm, float factor) { return !(factor >= 1.f) && norm != 0.f; }
+// A factor of 1 changes no value.  One that is NaN spreads, as a NaN norm should,
+// but for 0 / 0, where there is nothing to clip.
+__device__ __forceinline__ bool must_scale(float norm, float factor) {
+    return factor < 1.f || (factor != factor && norm != 0.f);
+}
 
 template <int THREADS>
 __device__ __forceinline__ void scale_by(const Span& sp, float f) {
