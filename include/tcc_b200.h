@@ -304,7 +304,8 @@ tcc_status tcc_embedding_forward(const void* table, int table_type, uint64_t ld_
  * grad_out[i, :F] over the i with idx[i] = v; rows without an index become 0,
  * columns F..ld_table stay as they were.  grad_out has the table's type or
  * fp32; sums are fp32, in an order that depends on the indices alone (the same
- * call gives the same bits).  Padded and bad indices contribute nothing.  n and
+ * call gives the same bits).  Padded and bad indices contribute nothing, the
+ * latter set *bad_flag (not where num_rows = 0: nothing is done then).  n and
  * num_rows below 2^31; scratch 256-byte aligned, of at least
  * tcc_embedding_backward_scratch_bytes(n, num_rows, F) bytes, not shared with
  * a call that may run at the same time. */

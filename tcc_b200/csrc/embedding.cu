@@ -26,6 +26,11 @@ __device__ __forceinline__ int64_t load_index(const void* idx, int type, uint64_
                            : (int64_t)__ldg(static_cast<const int*>(idx) + i);
 }
 
+// What is the padding of a call without one, INT64_MIN, is an index like any other.
+__device__ __forceinline__ bool is_padding(int64_t id, int64_t padding) {
+    return id == padding && padding != TCC_NO_PADDING;
+}
+
 // ---------------------------------------------------------------- lookup --
 
 constexpr int kLookupThreads = 256;
@@ -38,7 +43,7 @@ __device__ __forceinline__ void load_ids(uint32_t* ids, const void* idx, int idx
     for (uint32_t i = threadIdx.x; i < rows; i += kLookupThreads) {
         const int64_t id = load_index(idx, idx_type, first + i);
         uint32_t row = kZeroRow;
-        if (id != padding) {
+        if (!is_padding(id, padding)) {
             if (id >= 0 && id < (int64_t)num_rows) row = (uint32_t)id;
             else if (bad) atomicExch(bad, 1u);
         }
@@ -541,7 +546,7 @@ __global__ void __launch_bounds__(kThreads) grad_owner_kernel(
         if (i < n) {
             const int64_t id = load_index(idx, idx_type, i);
             const bool inside = id >= 0 && id < (int64_t)num_rows;
-            if (!inside && id != padding && bad && blockIdx.x == 0) atomicExch(bad, 1u);
+            if (!inside && !is_padding(id, padding) && bad && blockIdx.x == 0) atomicExch(bad, 1u);
             if (inside && id != padding && id >= (int64_t)r0 && id < (int64_t)r1) {
                 mine[k] = (Entry)id << 32 | i;
                 ++hits;
@@ -642,7 +647,7 @@ struct IndexSource {  // pass 0: the indices themselves; rows without a gradient
         return (Entry)(real ? (uint32_t)id : num_rows) << 32 | i;
     }
     __device__ __forceinline__ void note(uint32_t i, Entry e) const {
-        if (bad && row_of(e) == num_rows && load_index(idx, type, i) != padding) atomicExch(bad, 1u);
+        if (bad && row_of(e) == num_rows && !is_padding(load_index(idx, type, i), padding)) atomicExch(bad, 1u);
     }
 };
 

@@ -31,10 +31,26 @@ def _index(idx: torch.Tensor, device: torch.device):
     return idx if idx.is_contiguous() else idx.contiguous(), code
 
 
+def _padding(padding_idx) -> int:
+    if not L.NO_PADDING < padding_idx < 1 << 63:
+        raise ValueError("padding_idx must lie between -2^63 and 2^63")
+    return padding_idx
+
+
 def _bad_flag(bad, device):
     if bad.dtype != torch.int32 or bad.device != device or bad.numel() < 1:
         raise ValueError("bad must be an int32 tensor of one element on the rows' device")
     return bad.data_ptr()
+
+
+def _flag_bad(idx, num_rows: int, padding_idx, bad) -> None:
+    """What a call that launches nothing (no columns, or no rows to write) has to say of its indices."""
+    if bad is None or idx.numel() == 0:
+        return
+    outside = (idx < 0) | (idx >= num_rows)
+    if padding_idx is not None:
+        outside &= idx != padding_idx
+    bad.view(-1)[:1] |= outside.any()
 
 
 def _lookup(table, idx, scale, padding_idx, out_dtype, bad):
@@ -57,10 +73,13 @@ def _lookup(table, idx, scale, padding_idx, out_dtype, bad):
     idx, idx_code = _index(idx, device)
     out = torch.empty((*idx.shape, width), dtype=out_dtype, device=device)
     n = idx.numel()
+    padding = L.NO_PADDING if padding_idx is None else _padding(padding_idx)
+    flag = None if bad is None else _bad_flag(bad, device)
     if n and width:
         launch(device, "tcc_embedding_forward", table.data_ptr(), code, ld, num_rows, idx.data_ptr(), idx_code, n,
-               L.NO_PADDING if padding_idx is None else padding_idx, scale, out.data_ptr(), out_code, width, width,
-               None if bad is None else _bad_flag(bad, device))
+               padding, scale, out.data_ptr(), out_code, width, width, flag)
+    else:
+        _flag_bad(idx, num_rows, padding_idx, bad)
     return out
 
 
@@ -70,7 +89,7 @@ def embedding_backward(grad_out: torch.Tensor, idx: torch.Tensor, num_rows: int,
     """Gradient [num_rows, F] of a table for ``embedding``'s output gradient
     ``grad_out`` [*idx.shape, F]: scale * the sum of the rows of each index.
     Not differentiable itself.
-    ``dtype``: the table's type (default grad_out's)."""
+    ``dtype``: the table's type (default grad_out's); ``bad`` as in ``embedding``."""
     code = type_code(grad_out, "grad_out")
     dtype = grad_out.dtype if dtype is None else dtype
     if dtype not in TYPES or (dtype != grad_out.dtype and code != L.F32):
@@ -83,13 +102,16 @@ def embedding_backward(grad_out: torch.Tensor, idx: torch.Tensor, num_rows: int,
     idx, idx_code = _index(idx, device)
     grad_out, ld = rows_of(grad_out, width)
     out = torch.empty((num_rows, width), dtype=dtype, device=device)
+    padding = L.NO_PADDING if padding_idx is None else _padding(padding_idx)
+    flag = None if bad is None else _bad_flag(bad, device)
     if out.numel():
         n = idx.numel()
         nbytes = L.lib().tcc_embedding_backward_scratch_bytes(n, num_rows, width)
         hold, scratch = scratch_for(nbytes, device)
         launch(device, "tcc_embedding_backward", grad_out.data_ptr(), code, ld, idx.data_ptr(), idx_code, n,
-               L.NO_PADDING if padding_idx is None else padding_idx, scale, out.data_ptr(), TYPES[dtype],
-               width, num_rows, width, scratch, nbytes, None if bad is None else _bad_flag(bad, device))
+               padding, scale, out.data_ptr(), TYPES[dtype], width, num_rows, width, scratch, nbytes, flag)
+    else:
+        _flag_bad(idx, num_rows, padding_idx, bad)
     return out
 
 

@@ -89,3 +89,14 @@ def test_every_lookup_can_report_a_bad_index(no_launch, monkeypatch):
         call()
         call(bad=bad)
     assert flags == [None, bad.data_ptr()] * 2
+
+
+def test_padding_beyond_64_bits_is_refused(no_launch):
+    """-2^64 + 3 would be taken for 3."""
+    t = torch.zeros(4, 6)
+    for wrong in (-(1 << 64) + 3, (1 << 64) - 1, 1 << 63, -(1 << 63)):
+        for call in (lambda: embedding.embedding(t, IDX, padding_idx=wrong),
+                     lambda: embedding.embedding_backward(t[:3], IDX, 4, padding_idx=wrong),
+                     lambda: embedding.embedding(t[:, :0], IDX, padding_idx=wrong)):
+            with pytest.raises(ValueError, match="padding_idx"):
+                call()
