@@ -291,6 +291,7 @@ __device__ __forceinline__ float inverse_root(float x) {
 // parameters' gradients stay in registers.
 struct RowsShape {
     uint32_t L, log_L, GB, RB, PG, packs;  // packs of a group in a row, in a sample
+    uint32_t level;                        // passes of the backward's first level of sums
     // bytes from one pass to the next, computed here so that they are constants there
     uint64_t x_step, y_step, dy_step, dx_step, stats_step;
 };
@@ -323,7 +324,9 @@ __device__ __forceinline__ float strided_sum(const float* p, uint32_t stride, ui
 
 // Long fp32 sums are kept in two levels: a thread adds kLevel rows (or blocks of
 // rows, or samples), then that sum to a second one, and takes at most kLongest
-// in all, so that no chain of additions grows with the data.
+// in all, so that no chain of additions grows with the data.  (The row form,
+// which leaves a row of sums per thread row, takes as many as there are: its
+// levels are the square root of that, 130 each for 10 M rows.)
 constexpr uint32_t kLevel = 32, kLongest = 2048;
 
 // The place of a thread: its slot's group and sample, its packs' rows and
@@ -563,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, V * J <= 4 ? 4 : V * J <= 8 ? 2 : 1)
                                                                           add(g[j], splat<V>(-s))))));
             dx_now = advance(dx_now, sh.dx_step);
         }
-        if (++since == kLevel) {
+        if (++since == sh.level) {
             since = 0;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
@@ -1416,8 +1419,7 @@ inline RowsShape rows_shape(uint64_t S, uint32_t C, uint32_t G, int V) {
 inline bool rows_fold(const RowsShape& sh) { return sh.PG <= sh.L && (sh.PG & (sh.PG - 1)) == 0; }
 inline uint64_t rows_blocks(const RowsShape& sh, uint64_t N, uint32_t G) {
     const uint64_t y = (G + sh.GB - 1) / sh.GB;
-    return std::max<uint64_t>({1, std::min((N + sh.RB - 1) / sh.RB, kSms * 4 / std::min(kSms, y)),
-                               (N + (uint64_t)sh.RB * kLongest - 1) / (sh.RB * kLongest)});
+    return std::max<uint64_t>(1, std::min((N + sh.RB - 1) / sh.RB, kSms * 4 / std::min(kSms, y)));
 }
 
 // Chunks of a sample: three CTAs per SM over all samples, which run at once (a
@@ -1526,6 +1528,8 @@ void rows_launch(const GroupNormArgs& a, float* partial, bool backward, cudaStre
         sh.dy_step = bytes * a.lddy;
         sh.dx_step = bytes * a.lddx;
         sh.stats_step = samples * a.G * sizeof(float);
+        sh.level = kLevel;
+        while ((uint64_t)sh.level * sh.level * samples < a.N) ++sh.level;
         // where nothing is copied ahead, room for the sums alone
         const size_t smem = std::max<size_t>(Ring::kAsync ? sizeof(Ring) : 0, 2 * kThreads * V * sizeof(float));
         static std::atomic<uint64_t> done{0};

@@ -50,7 +50,7 @@ def test_resident_form_sums(gpu):
 
 
 def test_rows_form_sums(gpu):
-    """4,000 rows to a thread; three values a row."""
+    """4,000 rows to a thread, in two levels of 64; three values a row."""
     n, c = 592 * 64 * 4000 + 5, 3
     x = torch.zeros((n, c), device="cuda")
     stats = torch.zeros((n, 1), device="cuda")
