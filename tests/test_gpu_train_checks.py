@@ -46,3 +46,23 @@ def test_resume_with_other_groups_is_refused(gpu, tmp_path):
         with pytest.raises(ValueError, match="norm-groups"):
             train_gcn.train(_small(norm_groups=groups, epochs=2, resume=ck), gpu, 1, 0)
     assert len(train_gcn.train(_small(norm_groups=8, epochs=2, resume=ck), gpu, 1, 0)["losses"]) == 1
+
+
+@pytest.mark.parametrize("clip", [None, 1e-3])
+def test_the_optimiser_sees_clipped_gradients(gpu, monkeypatch, clip):
+    """The norm of all gradients at Adam's step, with and without the option at the same model; the
+    tiny limit is far below the gradients' own norm."""
+    seen = []
+    step = torch.optim.Adam.step
+
+    def record(self, *args, **kw):
+        grads = [p.grad.double() for group in self.param_groups for p in group["params"]]
+        seen.append(float(torch.stack([g.square().sum() for g in grads]).sum().sqrt()))
+        return step(self, *args, **kw)
+    monkeypatch.setattr(torch.optim.Adam, "step", record)
+    train_gcn.train(_small(norm_groups=8, clip_norm=clip, epochs=3), gpu, 1, 0)
+    assert len(seen) == 3
+    if clip is None:
+        assert min(seen) > 2e-3
+    else:  # eps beside a norm above 2e-3, the factor's roundings and that of every product
+        assert all(abs(n / clip - 1) <= 1e-6 / 2e-3 + 4 * 2.0 ** -24 for n in seen)
