@@ -1172,7 +1172,8 @@ const Entry* sort_by_cluster(const IndexSource& src, uint32_t n, const SortPlan&
     static std::atomic<uint64_t> done{0};
     allow_smem(cluster_sort_kernel<BITS>, cluster_smem(kHeld, p.digits), done);
     cudaLaunchConfig_t cfg{};
-    // two CTAs per SM beside the sort's, and only as many as find work
+    // 264 CTAs, and only as many as find work.  They carry the sort's shared memory: two to an
+    // SM up to about 12,000 indices with 11-bit digits, above that one, in two turns.
     zero.ctas = (uint32_t)std::min<uint64_t>(33, (zero.words + 8191) / 8192) * kCluster;
     cfg.gridDim = dim3(kCluster + zero.ctas);
     cfg.blockDim = dim3(kSortThreads);
