@@ -16,7 +16,7 @@ size_t group_norm_scratch_bytes(uint64_t N, uint64_t S, uint32_t C, uint32_t G, 
     uint64_t bytes = 0;
     for (int V = 1; V <= 8 && (C / G) % V == 0; V <<= 1)
         for (uint32_t es = 2; es <= 4 && es * V <= 16; es += 2) {
-            if (rows_form(S, C / G, V)) {
+            if (rows_form(S, C, G, V)) {
                 if (backward) bytes = std::max(bytes, rows_blocks(rows_shape(S, C, G, V), N, G) * S * 2 * C * 4);
                 continue;
             }

@@ -1395,11 +1395,6 @@ inline int pick_width(const GroupNormArgs& a) {
     return rule.width();
 }
 
-// The rows form: up to 8 packs and 32 values a lane, up to 32 rows.
-inline bool rows_form(uint64_t S, uint32_t Cg, int V) {
-    return S <= 32 && S * Cg <= 32u * std::min(8u * (uint32_t)V, 32u);
-}
-
 inline RowsShape rows_shape(uint64_t S, uint32_t C, uint32_t G, int V) {
     RowsShape sh{};
     sh.PG = C / G / V;
@@ -1411,6 +1406,15 @@ inline RowsShape rows_shape(uint64_t S, uint32_t C, uint32_t G, int V) {
     sh.GB = std::min(G, slots);
     sh.RB = slots / sh.GB;
     return sh;
+}
+
+// The rows form: up to 8 packs and 32 values a lane, up to 32 rows; groups that
+// fit the grid's y (1 M groups of 32 rows do not).
+inline bool rows_form(uint64_t S, uint32_t C, uint32_t G, int V) {
+    const uint32_t Cg = C / G;
+    if (S > 32 || S * Cg > 32u * std::min(8u * (uint32_t)V, 32u)) return false;
+    const RowsShape sh = rows_shape(S, C, G, V);
+    return (G + sh.GB - 1) / sh.GB <= 65535;
 }
 
 // CTAs in x of the backward: four per SM, which is a whole number of waves (a
@@ -1518,7 +1522,6 @@ template <typename T, int V, int J>
 void rows_launch(const GroupNormArgs& a, float* partial, bool backward, cudaStream_t s) {
     RowsShape sh = rows_shape(a.S, a.C, a.G, V);
     const uint32_t cols = (a.G + sh.GB - 1) / sh.GB;
-    TCC_REQUIRE(cols <= 65535, "too many groups for samples of few rows");
     dim3 grid(1, cols);
     if (backward) {
         using Ring = RowsRing<T, V, J, 2>;
@@ -1595,7 +1598,7 @@ void resident_launch(const GroupNormArgs& a, const SplitShape& sh, float* partia
 template <typename T, int V>
 void norm_launch(const GroupNormArgs& a, char* scratch, bool backward, cudaStream_t s) {
     const bool params = backward && (a.dweight || a.dbias);
-    if (rows_form(a.S, a.C / a.G, V)) {
+    if (rows_form(a.S, a.C, a.G, V)) {
         rows_by_packs<T, V>(a, params ? reinterpret_cast<float*>(scratch) : nullptr, backward, s);
         return;
     }

@@ -65,3 +65,11 @@ def test_memory_of_a_backward(gpu):
     dx, dw, db = N.group_norm_backward(x, x, mean, rstd, 1, w, b)
     extra = torch.cuda.max_memory_allocated() - before - dx.numel() * 2
     assert extra < 64 << 20, extra
+
+
+@pytest.mark.parametrize("n,steps,c,groups,dtype", [(2, 32, 1 << 20, 1 << 20, F32), (1, 17, 1 << 20, 1 << 20, BF16),
+                                                    (1, 32, 524280, 524280, F32)])
+def test_a_million_groups(gpu, n, steps, c, groups, dtype):
+    """Every channel by itself, as many as a call takes: more groups than the row form's grid."""
+    x, w, b, dy = _inputs((n, steps, c), dtype, F32, 5)
+    _both(x, groups, w, b, dy, "none")
