@@ -13,6 +13,18 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA GPU (B200, sm_100a)")
 
 
+# Tests that compare with the reference's own kernels.  Where its build is missing they
+# fail, after all others, so that a run that stops at its first failure has run the rest.
+NEED_REFERENCE = ("test_forward_tensorcore_vs_reference_kernels", "test_swtcf_vs_reference_converter",
+                  "test_config2_vs_reference_kernel", "test_swtcf_spmm_vs_reference_kernel",
+                  "test_swtcf_spmm_prepared_pull", "test_push_heavy_hub_window")
+
+
+def pytest_collection_modifyitems(items):
+    if not os.path.exists(os.path.join(ROOT, "oracle", "_ref", "libtcc_ref.so")):
+        items.sort(key=lambda item: getattr(item, "originalname", item.name) in NEED_REFERENCE)  # stable
+
+
 @pytest.fixture(scope="session")
 def oracle():
     import oracle as O
