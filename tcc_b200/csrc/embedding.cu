@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(
 }
 
 // Rows whose width or place no wider pack divides go value by value, where the flat
-// order is bound by its index arithmetic (300,000 rows of 333 values: 182 us).
+// order is bound by its index arithmetic (300,000 rows of 333 values out of 50: 182 us).
 // Here a team of lanes takes whole rows, PARTS values of each a lane at a time and
 // as many rows as make eight: 74 us.
 template <typename TT, typename TO, int PARTS>

@@ -14,10 +14,11 @@
 // own mean, are merged pairwise (Chan, Golub and LeVeque, 1979).
 //
 // Three forms:
-//  * rows  (few rows a sample, S = 1 above all; a sample's group within a
-//    warp): every (sample, group) is reduced by a few lanes of one warp, x is
-//    read once; the next samples are on their way into a ring in shared memory
-//    meanwhile.
+//  * rows  (up to 32 rows a sample, S = 1 above all; a sample's group within a
+//    warp, which is 1,024 values in packs of four or more, 512 in packs of two, 256
+//    value by value): every (sample, group) is reduced by a few lanes of one warp,
+//    x is read once; the next samples are on their way into a ring in shared
+//    memory meanwhile.
 //  * resident (a sample that fits the shared memory of at most eight SMs): a
 //    cluster of CTAs holds a sample, x (and dy) are read once, the CTAs exchange
 //    their moments or sums through distributed shared memory.
@@ -736,8 +737,9 @@ __device__ __forceinline__ Moments merge(const Moments& a, const Moments& b) {
 // meanwhile.  Registers hold B rows only, so that enough warps fit to hide the
 // exponentials and the memory (rows prefetched into registers: 128 registers,
 // 100 us in place of 52 for the sums of 232,965 x 256 bf16).  Of the four passes
-// over that graph the first takes 31 us, the others 41, 52 and 52, at 55 to 65 %
-// of the issue slots and 57 to 75 % of the pipe of the exponentials.
+// over that graph the first takes 25 us, the others 41, 50 and 55, at 54 to 67 %
+// of the issue slots; in the last three the pipe of the exponentials is 54 to 73 %
+// busy, with 20 of 64 warps.
 template <typename T, int V, int A, int D, int B, typename Body>
 __device__ __forceinline__ void stream_rows(void* smem, const T* const (&from)[A], const int64_t (&inc)[A],
                                             uint32_t count, Body&& body) {

@@ -50,7 +50,7 @@ def _flag_bad(idx, num_rows: int, padding_idx, bad) -> None:
     outside = (idx < 0) | (idx >= num_rows)
     if padding_idx is not None:
         outside &= idx != padding_idx
-    bad.view(-1)[:1] |= outside.any()
+    bad.as_strided((1,), (1,)).bitwise_or_(outside.any())  # the word at its address, whatever its shape
 
 
 def _lookup(table, idx, scale, padding_idx, out_dtype, bad):
